@@ -37,6 +37,9 @@ enum { B200K_BIAS_NONE = 0, B200K_BIAS_ROW_F32 = 1 /* bias[N] fp32 */, B200K_BIA
 /* Activation applied to the fp32 accumulator (after a fp32 bias add). */
 enum { B200K_ACT_NONE = 0, B200K_ACT_RELU = 1, B200K_ACT_LEAKY_RELU = 2 /* x>=0 ? x : 0.01x */ };
 
+/* Element type of a tensor whose type is an argument of the call. */
+enum { B200K_DTYPE_F32 = 0, B200K_DTYPE_BF16 = 1, B200K_DTYPE_F16 = 2 };
+
 /* Library ABI version (major*100+minor). */
 int b200k_version(void);
 /* Reason of the last failed call on this thread ("" if none). */
@@ -225,6 +228,30 @@ int b200k_attn_bwd_bf16(const void* q, const void* k, const void* v, const void*
                         void* dq, void* dk, void* dv, float* delta_scratch, int Z, int H, int N_CTX, int D, int causal,
                         float sm_scale, void* stream);
 int b200k_attn_bwd_supported(int D, int N_CTX);
+
+/*
+ * Layer norm over rows of `cols` elements (no counterpart in the reference; the norm around its attention in a training or
+ * serving step):  mu = mean(x), rstd = 1 / sqrt(mean((x - mu)^2) + eps), y = (x - mu) rstd w + b, all sums in fp32, y rounded once.
+ *   x, y        [rows, cols] of type `dtype`, unit inner stride, row pitches ldx / ldy in elements; any alignment of the type; y must
+ *               not overlap x
+ *   w, b        [cols] of type `wdtype` (dtype or B200K_DTYPE_F32), either may be null (1 and 0)
+ *   mean, rstd  [rows] fp32 for the backward, either may be null
+ * rows = 0 is a valid call that does nothing.  One launch.
+ */
+int b200k_layer_norm_fwd(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, int64_t rows, int64_t cols,
+                         int64_t ldx, int64_t ldy, int dtype, int wdtype, float eps, void* stream);
+/*
+ * Its gradients: with h = (x - mean) rstd and u = dy w,
+ *   dx = rstd (u - mean(u) - h mean(u h)),   dw = sum over rows of dy h,   db = sum over rows of dy.
+ *   dx          [rows, cols] of type `dtype` (pitch lddx) or null; must not overlap dy or x
+ *   dw, db      [cols] of type `wdtype`, either may be null; zeros when rows = 0
+ *   workspace   b200k_layer_norm_bwd_workspace(rows, cols) floats for their partial sums (none needed when both are null)
+ * Deterministic: no atomics, the sums' order depends on the sizes only.
+ */
+int b200k_layer_norm_bwd(const void* dy, const void* x, const void* w, const float* mean, const float* rstd, void* dx, void* dw, void* db,
+                         float* workspace, int64_t workspace_floats, int64_t rows, int64_t cols, int64_t lddy, int64_t ldx, int64_t lddx,
+                         int dtype, int wdtype, void* stream);
+int64_t b200k_layer_norm_bwd_workspace(int64_t rows, int64_t cols);
 
 /*
  * Generic launch mirroring the argument list the reference launcher builds

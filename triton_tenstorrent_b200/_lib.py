@@ -21,6 +21,7 @@ ERR_DEVICE_TIMEOUT = -5
 
 BIAS_NONE, BIAS_ROW_F32, BIAS_FULL_BF16 = 0, 1, 2
 ACT_NONE, ACT_RELU, ACT_LEAKY_RELU = 0, 1, 2
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 ARG_PTR, ARG_I32, ARG_I64, ARG_F32 = 0, 1, 2, 3
 
 
@@ -90,6 +91,9 @@ SIGNATURES = {
     "b200k_attn_supported": (c_int, [c_int, c_int]),
     "b200k_attn_bwd_bf16": (c_int, [c_void_p] * 10 + [c_int, c_int, c_int, c_int, c_int, c_float, c_void_p]),
     "b200k_attn_bwd_supported": (c_int, [c_int, c_int]),
+    "b200k_layer_norm_fwd": (c_int, [c_void_p] * 6 + [c_int64] * 4 + [c_int, c_int, c_float, c_void_p]),
+    "b200k_layer_norm_bwd": (c_int, [c_void_p] * 9 + [c_int64] * 6 + [c_int, c_int, c_void_p]),
+    "b200k_layer_norm_bwd_workspace": (c_int64, [c_int64, c_int64]),
     "b200k_launch": (c_int, [c_char_p, c_int, c_int, c_int, c_void_p, POINTER(Arg), c_int]),
     "b200k_device_props": (c_int, [c_int, POINTER(Props)]),
     "b200k_ipc_export": (c_int, [c_void_p, POINTER(IpcHandle)]),

@@ -573,6 +573,32 @@ int b200k_attn_bwd_bf16(const void* q, const void* k, const void* v, const void*
 
 int b200k_attn_bwd_supported(int D, int N_CTX) { return attn_bwd_supported(D, N_CTX); }
 
+int b200k_layer_norm_fwd(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, int64_t rows, int64_t cols,
+                         int64_t ldx, int64_t ldy, int dtype, int wdtype, float eps, void* stream) {
+  clear_error();
+  LayerNormArgs a{};
+  a.x = x; a.w = w; a.b = b; a.y = y; a.mean = mean; a.rstd = rstd;
+  a.rows = rows; a.cols = cols; a.ldx = ldx; a.ldy = ldy;
+  a.dtype = dtype; a.wdtype = wdtype; a.eps = eps;
+  return layer_norm_fwd(a, static_cast<cudaStream_t>(stream));
+}
+
+int b200k_layer_norm_bwd(const void* dy, const void* x, const void* w, const float* mean, const float* rstd, void* dx, void* dw, void* db,
+                         float* workspace, int64_t workspace_floats, int64_t rows, int64_t cols, int64_t lddy, int64_t ldx, int64_t lddx,
+                         int dtype, int wdtype, void* stream) {
+  clear_error();
+  LayerNormArgs a{};
+  a.dy = dy; a.x = x; a.w = w; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
+  a.dx = dx; a.dw = dw; a.db = db; a.workspace = workspace; a.workspace_floats = workspace_floats;
+  a.rows = rows; a.cols = cols; a.lddy = lddy; a.ldx = ldx; a.lddx = lddx;
+  a.dtype = dtype; a.wdtype = wdtype;
+  return layer_norm_bwd(a, static_cast<cudaStream_t>(stream));
+}
+
+int64_t b200k_layer_norm_bwd_workspace(int64_t rows, int64_t cols) {
+  return rows < 0 || cols < 1 ? 0 : layer_norm_bwd_workspace(rows, cols);
+}
+
 int b200k_launch(const char* kernel_name, int grid_x, int grid_y, int grid_z, void* stream, const b200k_arg* args,
                  int nargs) {
   clear_error();

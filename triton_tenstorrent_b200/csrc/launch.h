@@ -136,6 +136,30 @@ int attn_supported(int D, int N_CTX);
 // Work-queue simulation that assigns the causal items (ZH * num_pairs, head-major, longest first) to `grid` CTAs:
 // returns the table [rounds][grid] of item numbers (-1 = none).  Pure host code.
 std::vector<int> attn_schedule(int ZH, int num_pairs, int num_mblk, int ntile, int grid, int* rounds_out);
+// Row pitches ld* in elements; weight / bias type wdtype; unused pointers are null.  Forward: x, w, b -> y, mean, rstd.  Backward: dy, x, w,
+// mean, rstd -> dx, dw, db, with `workspace_floats` floats at `workspace` for the partial sums of dw and db.
+struct LayerNormArgs {
+  const void* x;
+  const void* w;
+  const void* b;
+  void* y;
+  float* mean;
+  float* rstd;
+  const void* dy;
+  void* dx;
+  void* dw;
+  void* db;
+  float* workspace;
+  int64_t workspace_floats;
+  int64_t rows, cols;
+  int64_t ldx, ldy, lddy, lddx;
+  int dtype, wdtype;
+  float eps;
+};
+constexpr int LN_MAX_PARTS = 296;   // partial sums of dw / db the backward writes at most: two CTAs on each of 148 SMs
+int layer_norm_fwd(const LayerNormArgs& a, cudaStream_t s);
+int layer_norm_bwd(const LayerNormArgs& a, cudaStream_t s);
+int64_t layer_norm_bwd_workspace(int64_t rows, int64_t cols);
 int selftest_wait_timeout(long long budget_cycles, cudaStream_t s);
 // The same self-test reporting into `status_words` (device memory, at least two words: status, kernel's own outcome).
 int selftest_wait_timeout_at(uint32_t* status_words, long long budget_cycles, cudaStream_t s);

@@ -16,7 +16,7 @@ import torch
 from . import _lib
 
 __all__ = ["add", "add_loop", "sin", "memcpy", "mul_add", "matmul", "tilize", "untilize", "matmul_tma", "matmul_tma_host_rows", "matmul_multi", "matmul_fused", "matmul_tma_fused", "attention", "attention_multi",
-           "attention_with_lse", "attention_backward", "device_status"]
+           "attention_with_lse", "attention_backward", "layer_norm", "layer_norm_with_stats", "layer_norm_backward", "device_status"]
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -530,6 +530,131 @@ def attention(q, k, v, causal, sm_scale, warp_specialize: bool = True) -> torch.
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
         return _attention.apply(q, k, v, causal, sm_scale, warp_specialize)
     return attention_with_lse(q, k, v, causal, sm_scale, warp_specialize)[0]
+
+
+_DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+
+
+def _rows_of(t: torch.Tensor) -> torch.Tensor:
+    """The [rows, last dimension] view of t with unit inner stride; a copy where t's strides have no such view."""
+    n = t.shape[-1]
+    if t.dim() == 1:
+        t = t.unsqueeze(0)
+    if t.numel() == 0:
+        return t.reshape(t.numel() // n if n else 0, n)
+    if n > 1 and t.stride(-1) != 1:
+        t = t.contiguous()
+    try:
+        return t.view(-1, n)
+    except RuntimeError:
+        return t.contiguous().view(-1, n)
+
+
+def _pitch(t2: torch.Tensor) -> int:
+    return t2.stride(0) if t2.shape[0] > 1 else t2.shape[1]
+
+
+def _norm_weight(name, x, t, like=None):
+    """weight / bias of a norm: [last dimension], x's type or fp32, on x's device."""
+    if t is None:
+        return None
+    if t.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"layer_norm: {name} must be {x.dtype} or torch.float32, got {t.dtype}")
+    if like is not None and t.dtype != like.dtype:
+        raise TypeError(f"layer_norm: weight and bias have different types {like.dtype} and {t.dtype}")
+    if tuple(t.shape) != (x.shape[-1],):
+        raise ValueError(f"layer_norm: {name} must be [{x.shape[-1]}], got {tuple(t.shape)}")
+    if t.device != x.device:
+        raise ValueError("layer_norm: tensors on different devices")
+    return t
+
+
+def _norm_input(name, x):
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"{name}: fp32, bf16 or fp16 tensor expected, got {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{name}: the last dimension must have at least one element, got shape {tuple(x.shape)}")
+
+
+def layer_norm_with_stats(x, weight=None, bias=None, eps: float = 1e-5):
+    """Returns (y, mean, rstd): the layer norm of x over its last dimension and the fp32 row statistics (x's shape without its last
+    dimension) that layer_norm_backward takes."""
+    _norm_input("layer_norm", x)
+    if not eps >= 0:
+        raise ValueError(f"layer_norm: eps must be >= 0, got {eps}")
+    w = _norm_weight("weight", x, weight)
+    b = _norm_weight("bias", x, bias, weight)
+    lib = _lib.load()
+    w, b = (None if t is None else _to_device(t).contiguous() for t in (w, b))
+    xd = _rows_of(_to_device(x))
+    rows, cols = xd.shape
+    y = torch.empty((rows, cols), device=xd.device, dtype=x.dtype)
+    stats = torch.empty((2, rows), device=xd.device, dtype=torch.float32)
+    wdtype = _DTYPES[(w if w is not None else b if b is not None else xd).dtype]
+    with _on(xd.device):
+        _lib.check(lib.b200k_layer_norm_fwd(xd.data_ptr(), 0 if w is None else w.data_ptr(), 0 if b is None else b.data_ptr(), y.data_ptr(),
+                                            stats.data_ptr(), stats.data_ptr() + 4 * rows, rows, cols, _pitch(xd), cols, _DTYPES[x.dtype],
+                                            wdtype, float(eps), _stream()))
+    return (_like_input(y.view(x.shape), x), _like_input(stats[0].view(x.shape[:-1]), x), _like_input(stats[1].view(x.shape[:-1]), x))
+
+
+def layer_norm_backward(dy, x, weight, mean, rstd, need_dx: bool = True, need_dw: bool = True, need_db: bool = True):
+    """(dx, dw, db) from the gradient dy of layer_norm's result, its input x, its weight (or None) and the statistics that
+    layer_norm_with_stats returned.  dw and db have the weight's type (fp32 without a weight).  A gradient that is not needed is None; a
+    frozen norm then reads x and dy once only."""
+    _norm_input("layer_norm_backward", x)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError(f"layer_norm_backward: dy must be {x.dtype} {tuple(x.shape)} like x, got {dy.dtype} {tuple(dy.shape)}")
+    if any(t.dtype != torch.float32 or t.shape != x.shape[:-1] for t in (mean, rstd)):
+        raise ValueError(f"layer_norm_backward: mean and rstd must be fp32 {tuple(x.shape[:-1])}")
+    if any(t.device != x.device for t in (dy, mean, rstd)):
+        raise ValueError("layer_norm_backward: tensors on different devices")
+    w = _norm_weight("weight", x, weight)
+    lib = _lib.load()
+    w = None if w is None else _to_device(w).contiguous()
+    xd, gd = _rows_of(_to_device(x)), _rows_of(_to_device(dy))
+    md, rd = (_to_device(t).contiguous() for t in (mean, rstd))
+    rows, cols = xd.shape
+    wtype = torch.float32 if w is None else w.dtype
+    dx = torch.empty((rows, cols), device=xd.device, dtype=x.dtype) if need_dx else None
+    dw = torch.empty(cols, device=xd.device, dtype=wtype) if need_dw else None
+    db = torch.empty(cols, device=xd.device, dtype=wtype) if need_db else None
+    floats = lib.b200k_layer_norm_bwd_workspace(rows, cols) if need_dw or need_db else 0
+    work = torch.empty(floats, device=xd.device, dtype=torch.float32)
+    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    with _on(xd.device):
+        _lib.check(lib.b200k_layer_norm_bwd(gd.data_ptr(), xd.data_ptr(), ptr(w), md.data_ptr(), rd.data_ptr(), ptr(dx), ptr(dw), ptr(db),
+                                            work.data_ptr(), floats, rows, cols, _pitch(gd), _pitch(xd), cols, _DTYPES[x.dtype],
+                                            _DTYPES[wtype], _stream()))
+    return (None if dx is None else _like_input(dx.view(x.shape), x), None if dw is None else _like_input(dw, x),
+            None if db is None else _like_input(db, x))
+
+
+class _layer_norm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = layer_norm_with_stats(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx, dw, db = layer_norm_backward(dy, x, weight, mean, rstd, need_x, need_w, need_b)
+        if db is not None:
+            db = db.to(ctx.bias_dtype)      # fp32 without a weight
+        return dx, dw, db, None
+
+
+def layer_norm(x, weight=None, bias=None, eps: float = 1e-5) -> torch.Tensor:
+    """y = (x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x (fp32, bf16 or fp16; weight and bias in x's type or in
+    fp32, either may be None).  fp32 arithmetic, one rounding; differentiable in x, weight and bias."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _layer_norm.apply(x, weight, bias, eps)
+    return layer_norm_with_stats(x, weight, bias, eps)[0]
 
 
 def device_status() -> int:
