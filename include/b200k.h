@@ -254,6 +254,43 @@ int b200k_layer_norm_bwd(const void* dy, const void* x, const void* w, const flo
 int64_t b200k_layer_norm_bwd_workspace(int64_t rows, int64_t cols);
 
 /*
+ * One AdamW step over a list of tensors (no counterpart in the reference; the optimiser of the parameters whose gradients
+ * b200k_attn_bwd_bf16, b200k_layer_norm_bwd and b200k_lce_bwd produce):
+ *   m <- beta1 m + (1 - beta1) g,  v <- beta2 v + (1 - beta2) g^2,
+ *   p <- p - lr weight_decay p - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps),   g = grad_scale * gradient
+ * in fp32, p rounded once.  `tensors` is a HOST array, read before the call returns; one launch per 400 tensors.  All tensors of a call have
+ * the parameter type `dtype` and the gradient type `gdtype` (dtype or B200K_DTYPE_F32).
+ *   state_bits 32   m and v are fp32 [n]
+ *   state_bits 8    m and v are byte codes, padded to a multiple of 256 bytes, with one fp32 scale per 256 elements (m_scale, v_scale); v holds
+ *                   codes of sqrt(v).  Codes: 4 exponent and 3 (m, after a sign bit) or 4 mantissa bits, value(c) = (1 + mantissa / 2^bits)
+ *                   2^exponent, value(0) = 0, largest code NaN; an element is value(code) * scale, the scale a power of two.  Rounding is stochastic, with random
+ *                   bits from a hash of (seed, t, index, element); all zero bytes and scales are the zero state.
+ *   master          fp32 [n] copy that the step works on, p then being its rounded image; for all tensors of the call or for none;
+ *                   16-bit parameters only
+ * m, v and master are 16-byte aligned; p and g need the alignment of their type only (aligned ones are faster).
+ * state: 40 bytes of device memory {double beta1^t, beta2^t; int64 t; double 1/(1-beta1^(t+1)); float 1/sqrt(1-beta2^(t+1)); uint32 0}, read by
+ * every call and moved on to t + 1 by a call with advance = 1 (the last of a step), so that a captured step counts on when it is replayed.
+ * lr_dev, grad_scale_dev: one device float each that replaces lr / grad_scale, or null.
+ */
+typedef struct b200k_adamw_tensor {
+  void* p;
+  const void* g;
+  float* master;
+  void* m;
+  void* v;
+  float* m_scale;
+  float* v_scale;
+  int64_t n;
+  int64_t index; /* place in the optimiser's list, for the random bits */
+} b200k_adamw_tensor;
+int b200k_adamw(const b200k_adamw_tensor* tensors, int n, int dtype, int gdtype, int state_bits, void* state, double lr, const float* lr_dev,
+                double beta1, double beta2, double eps, double weight_decay, float grad_scale, const float* grad_scale_dev, uint32_t seed,
+                int advance, void* stream);
+/* The values of `blocks` blocks of 256 8-bit moments in fp32: m_out = m, v_out = (root)^2. */
+int b200k_adamw_moments(const void* m, const float* m_scale, const void* v, const float* v_scale, float* m_out, float* v_out, int64_t blocks,
+                        void* stream);
+
+/*
  * Generic launch mirroring the argument list the reference launcher builds
  * (backend/driver.py:98-170 TTLauncher.__call__: constexprs dropped, tensors as pointers,
  * TensorDescriptor flattened to base, shape.., strides.., padding flag, shape.., strides..).

@@ -6,7 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, Structure, Union, c_char, c_char_p, c_float, c_int, c_int32, c_int64, c_uint32, c_void_p
+from ctypes import POINTER, Structure, Union, c_char, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_uint32, c_void_p
 from pathlib import Path
 
 # B200K_LIBRARY selects another build of the same library (e.g. one compiled with debug defines).
@@ -94,6 +94,9 @@ SIGNATURES = {
     "b200k_layer_norm_fwd": (c_int, [c_void_p] * 6 + [c_int64] * 4 + [c_int, c_int, c_float, c_void_p]),
     "b200k_layer_norm_bwd": (c_int, [c_void_p] * 9 + [c_int64] * 6 + [c_int, c_int, c_void_p]),
     "b200k_layer_norm_bwd_workspace": (c_int64, [c_int64, c_int64]),
+    "b200k_adamw": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_double, c_void_p, c_double, c_double, c_double, c_double, c_float,
+                            c_void_p, c_uint32, c_int, c_void_p]),
+    "b200k_adamw_moments": (c_int, [c_void_p] * 6 + [c_int64, c_void_p]),
     "b200k_launch": (c_int, [c_char_p, c_int, c_int, c_int, c_void_p, POINTER(Arg), c_int]),
     "b200k_device_props": (c_int, [c_int, POINTER(Props)]),
     "b200k_ipc_export": (c_int, [c_void_p, POINTER(IpcHandle)]),

@@ -1,0 +1,391 @@
+// AdamW over a list of tensors in one launch, with the moments in fp32 or in 8 bits.
+//
+//   m <- b1 m + (1 - b1) g,   v <- b2 v + (1 - b2) g^2
+//   p <- p - lr wd p - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// All arithmetic is fp32.  Products and sums that reach a stored moment are rounded one by one (no fused multiply-add), so that the same
+// inputs give the same codes wherever the formula is evaluated in IEEE fp32.
+//
+// 8-bit moments.  ADAMW_BLOCK consecutive elements of a tensor share a scale.  m is held with a sign, 4 exponent and 3 mantissa bits;
+// of v its root r is held, with 4 exponent and 4 mantissa bits (the root halves the range in octaves, and r has no sign to store):
+//   value(c) = (1 + mantissa / 2^MB) 2^exponent, value(0) = 0, the largest code stands for NaN; element = value(c) * scale,
+//   scale = the smallest power of two with which the block's largest finite magnitude does not exceed the largest finite code.
+// Rounding is stochastic.  To nearest, a moment whose change per step is below half a step of its code would never move: r changes by at most
+// 0.05 % a step while v decays (b2 = 0.999) and a step is 3 to 6 %, so a v that was large once would stay large.  Rounded
+// up with a probability equal to the fraction, the stored moment follows the fp32 one on average.  A power of two as scale keeps that noise
+// small: a moment that has not changed has the same code in every step, whatever the largest element does.  The 16 random bits of an
+// element come from a hash of (seed, step, tensor, element): the result is a function of the inputs alone.
+// An r above zero takes code 1 at least: with r = 0 beside an m that is not, the next update would be unbounded.
+// A non-finite moment takes the NaN code and does not enter the scale, so that it stays with its element.
+//
+// Bound: HBM.  Bytes per element with 16-bit p and g: 6 + 16 (fp32 moments) or 6 + 4 (8 bits).
+#include <math.h>
+
+#include "dtypes.cuh"
+#include "launch.h"
+#include "ptx.cuh"
+
+namespace b200k {
+
+constexpr int ADAMW_BLOCK = 256;                      // elements that share a scale: one warp, 8 elements a lane
+constexpr int ADAMW_THREADS = 256;
+constexpr int ADAMW_CHUNK = 64 * ADAMW_BLOCK;         // elements of one CTA
+constexpr int ADAMW_SMALL_TABLE = 40, ADAMW_LARGE_TABLE = 400;
+
+// What the kernels read of the step number; one per optimiser, in device memory.
+struct AdamwState {
+  double b1_pow, b2_pow;   // b1^t, b2^t after t steps
+  int64_t step;            // t
+  double inv_bc1;          // 1 / (1 - b1^(t+1))
+  float inv_sqrt_bc2;      // 1 / sqrt(1 - b2^(t+1))
+  unsigned ticket;         // CTAs of the running launch that are done
+};
+static_assert(sizeof(AdamwState) == 40, "layout shared with the host");
+
+template <int CAP>
+struct AdamwTable {
+  b200k_adamw_tensor t[CAP];
+  int first_chunk[CAP + 1];
+};
+
+struct AdamwParams {
+  AdamwState* state;
+  const float* lr_dev;           // overrides lr when not null
+  const float* grad_scale_dev;   // overrides grad_scale when not null
+  double lr, weight_decay;
+  double b1d, b2d;
+  float b1, one_minus_b1, b2, one_minus_b2, eps, grad_scale;
+  uint32_t seed;
+  int n;                         // tensors in the table
+  int advance;                   // this launch ends the step
+};
+
+// 32-bit hash: two rounds of xor-shift and an odd multiplier (the leading bits of sqrt(3)/2 and sqrt(2)/2).
+__device__ __forceinline__ uint32_t mix32(uint32_t x) {
+  x ^= x >> 16;
+  x *= 0xDDB3D743u;
+  x ^= x >> 15;
+  x *= 0xB504F335u;
+  return x ^ (x >> 16);
+}
+
+// Exponent field E of the block's scale 2^(E - 142): the largest finite code has the value (2 - 2^(1 - MB)) 2^15, and adding what a mantissa may
+// lack of that carries a peak beyond it into the next octave.  E >= 16 keeps the scale and its inverse normal numbers.
+template <int MB>
+__device__ __forceinline__ uint32_t scale_exponent(float peak) {
+  const uint32_t e = (__float_as_uint(peak) + ((1u << (24 - MB)) - 1)) >> 23;
+  return e < 16 ? 16 : e;
+}
+__device__ __forceinline__ float scale_of(uint32_t e) { return __uint_as_float((e - 15) << 23); }
+__device__ __forceinline__ float inverse_scale_of(uint32_t e) { return __uint_as_float((269 - e) << 23); }
+
+template <int MB>
+__device__ __forceinline__ float code_value(uint32_t c) {
+  constexpr uint32_t MASK = (1u << (4 + MB)) - 1;
+  const uint32_t mag = c & MASK;
+  float v = __uint_as_float((mag << (23 - MB)) + (127u << 23));
+  v = mag == 0 ? 0.f : v;
+  v = mag == MASK ? __int_as_float(0x7FC00000) : v;
+  return (MB == 3 && (c & 0x80u)) ? -v : v;
+}
+
+// |x| * inverse scale -> code, given 16 random bits.
+template <int MB>
+__device__ __forceinline__ uint32_t code_of(float x, float inverse, uint32_t random16) {
+  constexpr float LEAST = 1.f + 1.f / (1 << MB);       // value of code 1
+  const float a = fabsf(x);
+  const float y = __fmul_rn(a, inverse);
+  // normal codes: add random bits below the kept ones, then cut them off
+  const uint32_t raw = (__float_as_uint(y) - (127u << 23) + (random16 << (7 - MB))) >> (23 - MB);
+  // below code 1: an m up to it with probability y / value(1), an r always
+  const uint32_t small = (MB == 4 ? 0.f : static_cast<float>(2 * random16 + 1) * (LEAST * 0x1p-17f)) < y ? 1u : 0u;
+  uint32_t c = y < LEAST ? small : raw;
+  if (!(a <= 3.4028234663852886e38f)) c = (1u << (4 + MB)) - 1;
+  if (MB == 3 && x < 0.f) c |= 0x80u;
+  return c;
+}
+
+__device__ __forceinline__ float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a <= 3.4028234663852886e38f ? a : 0.f;
+}
+__device__ __forceinline__ float warp_max_nonneg(float v) {   // floats >= 0 order like their bits
+  return __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v)));
+}
+
+// 4 consecutive elements at p[0..4) of which the first `left` exist.
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, bool vec, int left, float (&f)[4]) {
+  if (vec) {
+    unpack<T, 4>(*reinterpret_cast<const Pack<T, 4>*>(p), f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = i < left ? to_f32<T>(p[i]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, bool vec, int left, const float (&f)[4]) {
+  if (vec) {
+    *reinterpret_cast<Pack<T, 4>*>(p) = pack<T, 4>(f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < left) p[i] = from_f32<T>(f[i]);
+  }
+}
+
+template <typename P, typename G, bool MASTER, int BITS, int CAP>
+__global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const __grid_constant__ AdamwTable<CAP> table, const AdamwParams q) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const double lr = q.lr_dev != nullptr ? static_cast<double>(*q.lr_dev) : q.lr;
+  const float step_size = static_cast<float>(lr * q.state->inv_bc1);
+  const float decay = static_cast<float>(1.0 - lr * q.weight_decay);
+  const float inv_sqrt_bc2 = q.state->inv_sqrt_bc2;
+  const float grad_scale = q.grad_scale_dev != nullptr ? *q.grad_scale_dev : q.grad_scale;
+  const uint32_t step = static_cast<uint32_t>(q.state->step + 1);
+
+  // the tensor of this CTA's chunk: the last one whose first chunk is not beyond it
+  const int chunk = blockIdx.x;
+  int lo = 0, hi = q.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (table.first_chunk[mid] <= chunk) lo = mid; else hi = mid - 1;
+  }
+  const b200k_adamw_tensor& t = table.t[lo];
+  const int64_t begin = static_cast<int64_t>(chunk - table.first_chunk[lo]) * ADAMW_CHUNK;
+  const int64_t end = begin + ADAMW_CHUNK < t.n ? begin + ADAMW_CHUNK : t.n;
+  const uint32_t salt = BITS == 8 ? mix32(mix32(q.seed + step * 0x9E3779B9u) + static_cast<uint32_t>(t.index)) : 0u;
+  P* const tp = static_cast<P*>(t.p);
+  const G* const tg = static_cast<const G*>(t.g);
+  const uintptr_t odd = (reinterpret_cast<uintptr_t>(tp) & (4 * sizeof(P) - 1)) | (reinterpret_cast<uintptr_t>(tg) & (4 * sizeof(G) - 1));
+
+  for (int64_t base = begin + warp * ADAMW_BLOCK; base < end; base += (ADAMW_THREADS / 32) * ADAMW_BLOCK) {
+    const int64_t block = base / ADAMW_BLOCK;
+    float m1[2][4], root[2][4];
+    float peak_m = 0.f, peak_r = 0.f;
+    float scale_m = 0.f, scale_r = 0.f;
+    if (BITS == 8) {
+      scale_m = t.m_scale[block];
+      scale_r = t.v_scale[block];
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t i = base + h * 128 + lane * 4;
+      const int left = i >= end ? 0 : (end - i < 4 ? static_cast<int>(end - i) : 4);
+      const bool vec = odd == 0 && left == 4;
+      float p[4], g[4], m[4], v[4];
+      if (MASTER) load4<float>(t.master + i, left == 4, left, p); else load4<P>(tp + i, vec, left, p);
+      load4<G>(tg + i, vec, left, g);
+      if (BITS == 8) {
+        // the code buffers are padded to whole blocks
+        const uint32_t cm = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(t.m) + i);
+        const uint32_t cr = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(t.v) + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          m[j] = __fmul_rn(code_value<3>((cm >> (8 * j)) & 0xFFu), scale_m);
+          const float r = __fmul_rn(code_value<4>((cr >> (8 * j)) & 0xFFu), scale_r);
+          v[j] = __fmul_rn(r, r);
+        }
+      } else {
+        load4<float>(static_cast<const float*>(t.m) + i, left == 4, left, m);
+        load4<float>(static_cast<const float*>(t.v) + i, left == 4, left, v);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float gj = __fmul_rn(g[j], grad_scale);
+        m[j] = __fadd_rn(__fmul_rn(m[j], q.b1), __fmul_rn(gj, q.one_minus_b1));
+        v[j] = __fadd_rn(__fmul_rn(v[j], q.b2), __fmul_rn(__fmul_rn(gj, gj), q.one_minus_b2));
+        root[h][j] = __fsqrt_rn(v[j]);
+        m1[h][j] = m[j];
+        p[j] = p[j] * decay - (m[j] / (root[h][j] * inv_sqrt_bc2 + q.eps)) * step_size;
+        if (BITS == 8 && j < left) {
+          peak_m = fmaxf(peak_m, finite_abs(m[j]));
+          peak_r = fmaxf(peak_r, finite_abs(root[h][j]));
+        }
+      }
+      if (MASTER) store4<float>(t.master + i, left == 4, left, p);
+      store4<P>(tp + i, vec, left, p);
+      if (BITS == 32) {
+        store4<float>(static_cast<float*>(t.m) + i, left == 4, left, m);
+        store4<float>(static_cast<float*>(t.v) + i, left == 4, left, v);
+      }
+    }
+    if (BITS == 8) {
+      peak_m = warp_max_nonneg(peak_m);
+      peak_r = warp_max_nonneg(peak_r);
+      const uint32_t exp_m = scale_exponent<3>(peak_m), exp_r = scale_exponent<4>(peak_r);
+      const float inv_m = inverse_scale_of(exp_m), inv_r = inverse_scale_of(exp_r);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t i = base + h * 128 + lane * 4;
+        uint32_t cm = 0, cr = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t rnd = mix32(static_cast<uint32_t>(i + j) + salt);
+          if (i + j < end) {
+            cm |= code_of<3>(m1[h][j], inv_m, rnd & 0xFFFFu) << (8 * j);
+            cr |= code_of<4>(root[h][j], inv_r, rnd >> 16) << (8 * j);
+          }
+        }
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.m) + i) = cm;
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.v) + i) = cr;
+      }
+      if (lane == 0) {
+        t.m_scale[block] = scale_of(exp_m);
+        t.v_scale[block] = scale_of(exp_r);
+      }
+    }
+  }
+
+  // the last CTA to finish moves the step on: by then every CTA has read the old one
+  if (q.advance) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      __threadfence();
+      if (atomicAdd(&q.state->ticket, 1u) == gridDim.x - 1) {
+        AdamwState s = *q.state;
+        s.b1_pow *= q.b1d;
+        s.b2_pow *= q.b2d;
+        s.step += 1;
+        s.inv_bc1 = 1.0 / (1.0 - s.b1_pow * q.b1d);
+        s.inv_sqrt_bc2 = static_cast<float>(1.0 / sqrt(1.0 - s.b2_pow * q.b2d));
+        s.ticket = 0;
+        *q.state = s;
+      }
+    }
+  }
+}
+
+// The values that 8-bit moments stand for: m, and v = r^2.  One warp per block of ADAMW_BLOCK elements.
+__global__ void __launch_bounds__(256) adamw_moments_kernel(const uint8_t* __restrict__ m, const float* __restrict__ m_scale,
+                                                            const uint8_t* __restrict__ r, const float* __restrict__ r_scale,
+                                                            float* __restrict__ m_out, float* __restrict__ v_out, int64_t n4) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= n4) return;
+  const int64_t block = i / (ADAMW_BLOCK / 4);
+  const uint32_t cm = reinterpret_cast<const uint32_t*>(m)[i], cr = reinterpret_cast<const uint32_t*>(r)[i];
+  const float sm = m_scale[block], sr = r_scale[block];
+  float4 a, b;
+  float* fa = &a.x;
+  float* fb = &b.x;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    fa[j] = __fmul_rn(code_value<3>((cm >> (8 * j)) & 0xFFu), sm);
+    const float x = __fmul_rn(code_value<4>((cr >> (8 * j)) & 0xFFu), sr);
+    fb[j] = __fmul_rn(x, x);
+  }
+  reinterpret_cast<float4*>(m_out)[i] = a;
+  reinterpret_cast<float4*>(v_out)[i] = b;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------------------------
+template <typename P, typename G, bool MASTER, int BITS, int CAP>
+static int adamw_launch(const b200k_adamw_tensor* tensors, int n, AdamwParams q, cudaStream_t stream) {
+  AdamwTable<CAP> table;
+  int used = 0;
+  int64_t chunks = 0;
+  const int advance = q.advance;
+  for (int i = 0; i <= n; ++i) {
+    const int64_t more = i < n ? (tensors[i].n + ADAMW_CHUNK - 1) / ADAMW_CHUNK : 0;
+    if (i == n || used == CAP || chunks + more > 0x7FFFFFFF) {   // the table is full, or the list ends
+      for (int k = used; k <= CAP; ++k) table.first_chunk[k] = static_cast<int>(chunks);
+      q.n = used;
+      q.advance = i == n ? advance : 0;
+      adamw_kernel<P, G, MASTER, BITS, CAP><<<static_cast<unsigned>(chunks), ADAMW_THREADS, 0, stream>>>(table, q);
+      count_launch();
+      B200K_CHECK_LAUNCH("adamw_kernel");
+      if (i == n) break;
+      used = 0;
+      chunks = 0;
+    }
+    table.t[used] = tensors[i];
+    table.first_chunk[used] = static_cast<int>(chunks);
+    chunks += more;
+    ++used;
+  }
+  return B200K_OK;
+}
+
+template <typename P, typename G, bool MASTER>
+static int adamw_bits(const b200k_adamw_tensor* t, int n, int bits, const AdamwParams& q, cudaStream_t s) {
+  if (n <= ADAMW_SMALL_TABLE)
+    return bits == 8 ? adamw_launch<P, G, MASTER, 8, ADAMW_SMALL_TABLE>(t, n, q, s) : adamw_launch<P, G, MASTER, 32, ADAMW_SMALL_TABLE>(t, n, q, s);
+  return bits == 8 ? adamw_launch<P, G, MASTER, 8, ADAMW_LARGE_TABLE>(t, n, q, s) : adamw_launch<P, G, MASTER, 32, ADAMW_LARGE_TABLE>(t, n, q, s);
+}
+
+template <typename P>
+static int adamw_16bit(const b200k_adamw_tensor* t, int n, int gdtype, bool master, int bits, const AdamwParams& q, cudaStream_t s) {
+  if (gdtype == B200K_DTYPE_F32) return master ? adamw_bits<P, float, true>(t, n, bits, q, s) : adamw_bits<P, float, false>(t, n, bits, q, s);
+  return master ? adamw_bits<P, P, true>(t, n, bits, q, s) : adamw_bits<P, P, false>(t, n, bits, q, s);
+}
+
+int adamw(const AdamwArgs& a, cudaStream_t stream) {
+  if (a.n <= 0 || a.tensors == nullptr) return set_error(B200K_ERR_INVALID_ARG, "adamw: at least one tensor expected (got %d)", a.n);
+  if (a.dtype < B200K_DTYPE_F32 || a.dtype > B200K_DTYPE_F16) return set_error(B200K_ERR_INVALID_ARG, "adamw: bad parameter type %d", a.dtype);
+  if (a.gdtype != a.dtype && a.gdtype != B200K_DTYPE_F32)
+    return set_error(B200K_ERR_INVALID_ARG, "adamw: gradients have the parameters' type or fp32 (got %d for parameters of type %d)", a.gdtype, a.dtype);
+  if (a.state_bits != 8 && a.state_bits != 32) return set_error(B200K_ERR_INVALID_ARG, "adamw: state_bits must be 8 or 32 (got %d)", a.state_bits);
+  if (a.state == nullptr || (reinterpret_cast<uintptr_t>(a.state) & 7u)) return set_error(B200K_ERR_INVALID_ARG, "adamw: null or misaligned state");
+  if (!(a.beta1 >= 0.0 && a.beta1 < 1.0 && a.beta2 >= 0.0 && a.beta2 < 1.0))
+    return set_error(B200K_ERR_INVALID_ARG, "adamw: betas must be in [0, 1) (got %g, %g)", a.beta1, a.beta2);
+  if (!(a.eps >= 0.0) || !(a.weight_decay >= 0.0) || (a.lr_dev == nullptr && !(a.lr >= 0.0)))
+    return set_error(B200K_ERR_INVALID_ARG, "adamw: lr, eps and weight_decay must be >= 0 (got %g, %g, %g)", a.lr, a.eps, a.weight_decay);
+  const bool master = a.tensors[0].master != nullptr;
+  if (master && a.dtype == B200K_DTYPE_F32) return set_error(B200K_ERR_INVALID_ARG, "adamw: fp32 parameters take no master copy");
+  const size_t psize = a.dtype == B200K_DTYPE_F32 ? 4 : 2, gsize = a.gdtype == B200K_DTYPE_F32 ? 4 : 2;
+  for (int i = 0; i < a.n; ++i) {
+    const b200k_adamw_tensor& t = a.tensors[i];
+    if (t.n <= 0 || t.n > (int64_t(1) << 40)) return set_error(B200K_ERR_INVALID_ARG, "adamw: tensor %d has %lld elements", i, (long long)t.n);
+    if (t.p == nullptr || t.g == nullptr || t.m == nullptr || t.v == nullptr || (a.state_bits == 8 && (t.m_scale == nullptr || t.v_scale == nullptr)))
+      return set_error(B200K_ERR_INVALID_ARG, "adamw: tensor %d has a null pointer", i);
+    if ((t.master != nullptr) != master) return set_error(B200K_ERR_INVALID_ARG, "adamw: tensor %d differs in having a master copy", i);
+    if ((reinterpret_cast<uintptr_t>(t.p) & (psize - 1)) || (reinterpret_cast<uintptr_t>(t.g) & (gsize - 1)))
+      return set_error(B200K_ERR_INVALID_ARG, "adamw: tensor %d is not aligned to its element size", i);
+    if ((reinterpret_cast<uintptr_t>(t.m) | reinterpret_cast<uintptr_t>(t.v) | reinterpret_cast<uintptr_t>(t.master)) & 15u)
+      return set_error(B200K_ERR_INVALID_ARG, "adamw: moments and master copy of tensor %d must be 16-byte aligned", i);
+    if ((reinterpret_cast<uintptr_t>(t.m_scale) | reinterpret_cast<uintptr_t>(t.v_scale)) & 3u)
+      return set_error(B200K_ERR_INVALID_ARG, "adamw: scales of tensor %d must be 4-byte aligned", i);
+  }
+  const DeviceInfo* dev = current_device_info();
+  if (dev == nullptr) return B200K_ERR_NO_DEVICE;
+  AdamwParams q{};
+  q.state = static_cast<AdamwState*>(a.state);
+  q.lr_dev = a.lr_dev;
+  q.grad_scale_dev = a.grad_scale_dev;
+  q.lr = a.lr;
+  q.weight_decay = a.weight_decay;
+  q.b1d = a.beta1;
+  q.b2d = a.beta2;
+  q.b1 = static_cast<float>(a.beta1);
+  q.one_minus_b1 = static_cast<float>(1.0 - a.beta1);
+  q.b2 = static_cast<float>(a.beta2);
+  q.one_minus_b2 = static_cast<float>(1.0 - a.beta2);
+  q.eps = static_cast<float>(a.eps);
+  q.grad_scale = a.grad_scale;
+  q.seed = a.seed;
+  q.advance = a.advance;
+  if (a.dtype == B200K_DTYPE_F32) return adamw_bits<float, float, false>(a.tensors, a.n, a.state_bits, q, stream);
+  if (a.dtype == B200K_DTYPE_BF16) return adamw_16bit<__nv_bfloat16>(a.tensors, a.n, a.gdtype, master, a.state_bits, q, stream);
+  return adamw_16bit<__half>(a.tensors, a.n, a.gdtype, master, a.state_bits, q, stream);
+}
+
+int adamw_moments(const uint8_t* m, const float* m_scale, const uint8_t* r, const float* r_scale, float* m_out, float* v_out, int64_t blocks,
+                  cudaStream_t stream) {
+  if (blocks < 0 || blocks > (int64_t(1) << 32)) return set_error(B200K_ERR_INVALID_ARG, "adamw_moments: %lld blocks", (long long)blocks);
+  if (blocks == 0) return B200K_OK;
+  if (m == nullptr || m_scale == nullptr || r == nullptr || r_scale == nullptr || m_out == nullptr || v_out == nullptr)
+    return set_error(B200K_ERR_INVALID_ARG, "adamw_moments: null pointer");
+  if ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(r)) & 3u || (reinterpret_cast<uintptr_t>(m_out) | reinterpret_cast<uintptr_t>(v_out)) & 15u)
+    return set_error(B200K_ERR_INVALID_ARG, "adamw_moments: codes must be 4-byte and outputs 16-byte aligned");
+  const DeviceInfo* dev = current_device_info();
+  if (dev == nullptr) return B200K_ERR_NO_DEVICE;
+  const int64_t n4 = blocks * (ADAMW_BLOCK / 4);
+  adamw_moments_kernel<<<static_cast<unsigned>((n4 + 255) / 256), 256, 0, stream>>>(m, m_scale, r, r_scale, m_out, v_out, n4);
+  count_launch();
+  B200K_CHECK_LAUNCH("adamw_moments_kernel");
+  return B200K_OK;
+}
+
+}  // namespace b200k

@@ -599,6 +599,21 @@ int64_t b200k_layer_norm_bwd_workspace(int64_t rows, int64_t cols) {
   return rows < 0 || cols < 1 ? 0 : layer_norm_bwd_workspace(rows, cols);
 }
 
+int b200k_adamw(const b200k_adamw_tensor* tensors, int n, int dtype, int gdtype, int state_bits, void* state, double lr, const float* lr_dev,
+                double beta1, double beta2, double eps, double weight_decay, float grad_scale, const float* grad_scale_dev, uint32_t seed,
+                int advance, void* stream) {
+  clear_error();
+  AdamwArgs a{tensors, n, dtype, gdtype, state_bits, state, lr, lr_dev, beta1, beta2, eps, weight_decay, grad_scale, grad_scale_dev, seed, advance};
+  return adamw(a, static_cast<cudaStream_t>(stream));
+}
+
+int b200k_adamw_moments(const void* m, const float* m_scale, const void* v, const float* v_scale, float* m_out, float* v_out, int64_t blocks,
+                        void* stream) {
+  clear_error();
+  return adamw_moments(static_cast<const uint8_t*>(m), m_scale, static_cast<const uint8_t*>(v), v_scale, m_out, v_out, blocks,
+                       static_cast<cudaStream_t>(stream));
+}
+
 int b200k_launch(const char* kernel_name, int grid_x, int grid_y, int grid_z, void* stream, const b200k_arg* args,
                  int nargs) {
   clear_error();

@@ -160,6 +160,22 @@ constexpr int LN_MAX_PARTS = 296;   // partial sums of dw / db the backward writ
 int layer_norm_fwd(const LayerNormArgs& a, cudaStream_t s);
 int layer_norm_bwd(const LayerNormArgs& a, cudaStream_t s);
 int64_t layer_norm_bwd_workspace(int64_t rows, int64_t cols);
+struct AdamwArgs {
+  const b200k_adamw_tensor* tensors;
+  int n;
+  int dtype, gdtype, state_bits;
+  void* state;
+  double lr;
+  const float* lr_dev;
+  double beta1, beta2, eps, weight_decay;
+  float grad_scale;
+  const float* grad_scale_dev;
+  uint32_t seed;
+  int advance;
+};
+int adamw(const AdamwArgs& a, cudaStream_t s);
+int adamw_moments(const uint8_t* m, const float* m_scale, const uint8_t* r, const float* r_scale, float* m_out, float* v_out, int64_t blocks,
+                  cudaStream_t s);
 int selftest_wait_timeout(long long budget_cycles, cudaStream_t s);
 // The same self-test reporting into `status_words` (device memory, at least two words: status, kernel's own outcome).
 int selftest_wait_timeout_at(uint32_t* status_words, long long budget_cycles, cudaStream_t s);
