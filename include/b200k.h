@@ -254,6 +254,34 @@ int b200k_layer_norm_bwd(const void* dy, const void* x, const void* w, const flo
 int64_t b200k_layer_norm_bwd_workspace(int64_t rows, int64_t cols);
 
 /*
+ * Cross entropy of a linear output layer without keeping its logits (no counterpart in the reference; the loss behind the last
+ * product of a training step):  logits = h W^T, lse_i = log sum_v exp(logits[i, v]), losses_i = lse_i - logits[i, target_i].
+ *   h           [T, D], w [V, D] of type `dtype` (bf16 or fp16), unit inner stride, row pitches ldh / ldw in elements (multiples of 8, as is D;
+ *               base pointers 16-byte aligned); any T >= 0 and V >= 1
+ *   target      int64 [T]; a token whose target is ignore_index carries no loss: its loss, its lse and its row of dh are 0, and what its row
+ *               of h holds does not matter.  Any other target outside [0, V) makes the token's loss NaN, and with it what that enters.
+ *   losses, lse fp32 [T] (natural logarithm); loss: one float, the mean over the tokens that carry a loss (0 without any) or the sum,
+ *               unused with B200K_REDUCE_NONE
+ *   workspace   b200k_lce_workspace(T, D, V, 0) bytes, 256-byte aligned
+ * The logits stay in fp32 accumulators; lse and losses are fp32 throughout.
+ */
+enum { B200K_REDUCE_NONE = 0, B200K_REDUCE_MEAN = 1, B200K_REDUCE_SUM = 2 };
+int b200k_lce_fwd(const void* h, const void* w, const int64_t* target, float* losses, float* lse, float* loss, void* workspace,
+                  int64_t workspace_bytes, int T, int D, int V, int64_t ldh, int64_t ldw, int64_t ignore_index, int reduction, int dtype,
+                  void* stream);
+/*
+ * Its gradients dh [T, D] and dw [V, D] (contiguous, either may be null), from the lse of the forward and
+ *   d_loss      the gradient of each token's loss, fp32 [T] (B200K_REDUCE_NONE), or one float, the gradient of `loss`
+ * The logits are computed again, for one piece of the vocabulary at a time (at most 512 MiB of 16-bit dlogits, or 256 entries).
+ * workspace: b200k_lce_workspace(T, D, V, 1) bytes.  dlogits are rounded to `dtype` where they enter the two products, sums are fp32, dh and
+ * dw are rounded once.  Deterministic: no atomics.
+ */
+int b200k_lce_bwd(const void* h, const void* w, const int64_t* target, const float* lse, const float* d_loss, void* dh, void* dw,
+                  void* workspace, int64_t workspace_bytes, int T, int D, int V, int64_t ldh, int64_t ldw, int64_t ignore_index, int reduction,
+                  int dtype, void* stream);
+int64_t b200k_lce_workspace(int T, int D, int V, int backward);
+
+/*
  * One AdamW step over a list of tensors (no counterpart in the reference; the optimiser of the parameters whose gradients
  * b200k_attn_bwd_bf16, b200k_layer_norm_bwd and b200k_lce_bwd produce):
  *   m <- beta1 m + (1 - beta1) g,  v <- beta2 v + (1 - beta2) g^2,

@@ -22,6 +22,7 @@ ERR_DEVICE_TIMEOUT = -5
 BIAS_NONE, BIAS_ROW_F32, BIAS_FULL_BF16 = 0, 1, 2
 ACT_NONE, ACT_RELU, ACT_LEAKY_RELU = 0, 1, 2
 DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+REDUCE_NONE, REDUCE_MEAN, REDUCE_SUM = 0, 1, 2
 ARG_PTR, ARG_I32, ARG_I64, ARG_F32 = 0, 1, 2, 3
 
 
@@ -94,6 +95,9 @@ SIGNATURES = {
     "b200k_layer_norm_fwd": (c_int, [c_void_p] * 6 + [c_int64] * 4 + [c_int, c_int, c_float, c_void_p]),
     "b200k_layer_norm_bwd": (c_int, [c_void_p] * 9 + [c_int64] * 6 + [c_int, c_int, c_void_p]),
     "b200k_layer_norm_bwd_workspace": (c_int64, [c_int64, c_int64]),
+    "b200k_lce_fwd": (c_int, [c_void_p] * 7 + [c_int64, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int, c_int, c_void_p]),
+    "b200k_lce_bwd": (c_int, [c_void_p] * 8 + [c_int64, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int, c_int, c_void_p]),
+    "b200k_lce_workspace": (c_int64, [c_int, c_int, c_int, c_int]),
     "b200k_adamw": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_double, c_void_p, c_double, c_double, c_double, c_double, c_float,
                             c_void_p, c_uint32, c_int, c_void_p]),
     "b200k_adamw_moments": (c_int, [c_void_p] * 6 + [c_int64, c_void_p]),

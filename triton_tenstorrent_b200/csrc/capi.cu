@@ -599,6 +599,26 @@ int64_t b200k_layer_norm_bwd_workspace(int64_t rows, int64_t cols) {
   return rows < 0 || cols < 1 ? 0 : layer_norm_bwd_workspace(rows, cols);
 }
 
+int b200k_lce_fwd(const void* h, const void* w, const int64_t* target, float* losses, float* lse, float* loss, void* workspace,
+                  int64_t workspace_bytes, int T, int D, int V, int64_t ldh, int64_t ldw, int64_t ignore_index, int reduction, int dtype,
+                  void* stream) {
+  clear_error();
+  LceArgs a{h, w, target, losses, lse, loss, nullptr, nullptr, nullptr, workspace, workspace_bytes, T, D, V, ldh, ldw, ignore_index, reduction, dtype};
+  return lce_fwd(a, static_cast<cudaStream_t>(stream));
+}
+
+int b200k_lce_bwd(const void* h, const void* w, const int64_t* target, const float* lse, const float* d_loss, void* dh, void* dw,
+                  void* workspace, int64_t workspace_bytes, int T, int D, int V, int64_t ldh, int64_t ldw, int64_t ignore_index, int reduction,
+                  int dtype, void* stream) {
+  clear_error();
+  LceArgs a{h, w, target, nullptr, const_cast<float*>(lse), nullptr, d_loss, dh, dw, workspace, workspace_bytes, T, D, V, ldh, ldw, ignore_index, reduction, dtype};
+  return lce_bwd(a, static_cast<cudaStream_t>(stream));
+}
+
+int64_t b200k_lce_workspace(int T, int D, int V, int backward) {
+  return T < 1 || D < 1 || V < 1 ? 0 : lce_workspace(T, D, V, backward);
+}
+
 int b200k_adamw(const b200k_adamw_tensor* tensors, int n, int dtype, int gdtype, int state_bits, void* state, double lr, const float* lr_dev,
                 double beta1, double beta2, double eps, double weight_decay, float grad_scale, const float* grad_scale_dev, uint32_t seed,
                 int advance, void* stream) {

@@ -160,6 +160,26 @@ constexpr int LN_MAX_PARTS = 296;   // partial sums of dw / db the backward writ
 int layer_norm_fwd(const LayerNormArgs& a, cudaStream_t s);
 int layer_norm_bwd(const LayerNormArgs& a, cudaStream_t s);
 int64_t layer_norm_bwd_workspace(int64_t rows, int64_t cols);
+struct LceArgs {
+  const void* h;
+  const void* w;
+  const int64_t* target;
+  float* losses;        // forward
+  float* lse;           // forward: written; backward: read
+  float* loss;          // forward, reduced
+  const float* d_loss;  // backward: per token, or one number
+  void* dh;
+  void* dw;
+  void* workspace;
+  int64_t workspace_bytes;
+  int T, D, V;
+  int64_t ldh, ldw;
+  int64_t ignore_index;
+  int reduction, dtype;
+};
+int lce_fwd(const LceArgs& a, cudaStream_t s);
+int lce_bwd(const LceArgs& a, cudaStream_t s);
+int64_t lce_workspace(int T, int D, int V, int backward);
 struct AdamwArgs {
   const b200k_adamw_tensor* tensors;
   int n;

@@ -1,0 +1,828 @@
+// Cross entropy of a linear output layer, logits = h W^T over a vocabulary of V, forward and backward, without keeping the logits:
+//
+//   loss_i = lse_i - logits[i, y_i],   lse_i = log sum_v exp(logits[i, v])
+//   dlogits[i, v] = g_i (exp(logits[i, v] - lse_i) - [v = y_i]),   dh = dlogits W,   dW = dlogits^T h
+//
+// Forward: one matrix product whose epilogue reduces each 256-column tile of the fp32 accumulators to a maximum and a sum of exponentials per
+// row; a second kernel joins the tiles' pairs.  Backward, for one piece of the vocabulary after the other: the logits of the piece again,
+// turned in the epilogue into dlogits in 16 bits; then dW of the piece (all tokens summed in one accumulator) and the piece's share of dh
+// (summed over the pieces in fp32).  8 T V D multiply-adds of which 2 are the recomputation.
+//
+// Tokens whose target is `ignore_index` are left out before the first product: a gather kernel moves the rows that count to the front of a
+// copy of h and writes their number to device memory, where the products read it.  Work and time shrink with the tokens that carry a loss,
+// and whatever stands in the rows of the others (padding, infinities) is never read by a product.
+//
+// The products run on CTA pairs (tcgen05, cta_group::2, 256 x 256 tiles, fp32 accumulators in tensor memory): warp 0 loads both operands by
+// TMA into a six-stage ring, one thread of warp 1 issues the MMAs, warps 2-5 run the epilogue of tile i during the main loop of tile i + 1.
+// Bound: the tensor pipe; with few tokens the stream of W from HBM.
+#include <string.h>
+
+#include "launch.h"
+#include "ptx.cuh"
+
+namespace b200k {
+
+constexpr int LCE_THREADS = 192;
+constexpr int LCE_EPI_WARPS = 4;
+constexpr int LCE_STAGES = 6;
+constexpr int LCE_BOX_BYTES = 64 * 128;                     // 64 rows of 128 bytes
+constexpr int LCE_A_BYTES = 2 * LCE_BOX_BYTES;              // a CTA's 128 x 64 share of A
+constexpr int LCE_B_BYTES = 2 * LCE_BOX_BYTES;              // its half of B: 128 x 64
+constexpr int LCE_C_BUF_BYTES = 32 * 128;
+constexpr int LCE_A_OFF = 0;
+constexpr int LCE_B_OFF = LCE_STAGES * LCE_A_BYTES;
+constexpr int LCE_C_OFF = LCE_B_OFF + LCE_STAGES * LCE_B_BYTES;
+constexpr int LCE_BAR_OFF = LCE_C_OFF + LCE_EPI_WARPS * 2 * LCE_C_BUF_BYTES;
+constexpr int LCE_SMEM = LCE_BAR_OFF + (2 * LCE_STAGES + 4) * 8 + 16 + 1024;
+static_assert(LCE_SMEM <= 232448, "shared memory budget exceeded");
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+// dlogits are stored as dlogits / max|g| * 2^14 in fp16 (at most 2^14 in magnitude, and probabilities down to 2^-38 survive; unscaled ones below
+// 2^-24 would be lost) and without the power of two in bf16, whose range is fp32's.
+constexpr float LCE_F16_SCALE = 16384.f;
+
+enum { LCE_STATS = 0, LCE_DLOGITS = 1, LCE_DW = 2, LCE_DH = 3 };
+
+struct LceGemmParams {
+  const int* count;        // tokens that carry a loss (device memory)
+  int M, N, K;             // sizes of the launch; M of STATS, DLOGITS and DH and K of DW are bounds that `count` replaces
+  int group_m;             // tile rows of a group (their A panel stays in L2 while the tile columns stream)
+  int f16;
+  uint32_t idesc, idesc_half;
+  uint32_t* status;
+  const int* target;       // per row that counts: its target (STATS, DLOGITS)
+  int col_base;            // first vocabulary entry of the piece
+  float2* part;            // STATS: [tile column][rows] (maximum * log2 e, sum of exponentials)
+  int64_t part_ld;
+  float* target_logit;     // STATS
+  const float* lse2;       // DLOGITS: lse * log2 e
+  const float* row_scale;  // DLOGITS: factor of the row
+  const float* alpha;      // DW, DH: factor of the result (device memory)
+  const float* add;        // DH: fp32 sum over the earlier pieces, or null
+  float* sum;              // DH: where the sum so far goes, or null for the last piece
+  void* out;               // DH, last piece: dh
+  const int* token;        // DH: token of a row
+};
+
+struct LceWork {
+  int pid_m, pid_n, col0, width;
+};
+struct LceSchedule {
+  int num_pid_m, num_pid_n, group_m, full_work, num_work;
+};
+// Tiles in groups of group_m rows, odd groups backwards; the tiles of a last wave that occupy at most half of the pairs are cut in two column
+// halves (the order and the split of the matmul kernel).
+__device__ __forceinline__ LceSchedule lce_schedule(int M, int N, int group_m, int pairs) {
+  LceSchedule s;
+  s.num_pid_m = (M + 255) >> 8;
+  s.num_pid_n = (N + 255) >> 8;
+  s.group_m = group_m;
+  const int tiles = s.num_pid_m * s.num_pid_n;
+  const int rest = tiles % pairs;
+  s.full_work = s.num_work = tiles;
+  if (rest > 0 && 2 * rest <= pairs) {
+    s.full_work = tiles - rest;
+    s.num_work = tiles + rest;
+  }
+  return s;
+}
+__device__ __forceinline__ LceWork lce_work(const LceSchedule& s, int w) {
+  LceWork r;
+  int tile = w, half = 0;
+  r.width = 256;
+  if (w >= s.full_work) {
+    tile = s.full_work + ((w - s.full_work) >> 1);
+    half = (w - s.full_work) & 1;
+    r.width = 128;
+  }
+  const int per_group = s.group_m * s.num_pid_n;
+  const int group = tile / per_group;
+  const int first = group * s.group_m;
+  const int size = min(s.num_pid_m - first, s.group_m);
+  const int in = tile - group * per_group;
+  r.pid_m = first + in % size;
+  r.pid_n = in / size;
+  if (group & 1) r.pid_n = s.num_pid_n - 1 - r.pid_n;
+  r.col0 = r.pid_n * 256 + half * 128;
+  return r;
+}
+
+__device__ __forceinline__ uint32_t lce_pack2(float lo, float hi, int f16) { return f16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi); }
+
+// 64 columns of a warp's 32 rows, packed to 16 bits, through the warp's staging buffer to the tensor map.
+__device__ __forceinline__ void lce_store_chunk(const CUtensorMap* map, const float (&f)[64], int f16, int row0, int col0, int rows, int cols,
+                                                uint8_t* stage, int& buf, uint32_t lane) {
+  if (lane == 0) tma_store_wait_read<1>();   // the buffer's store of two chunks ago
+  __syncwarp();
+  uint8_t* dst = stage + buf * LCE_C_BUF_BYTES;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint4 v = make_uint4(lce_pack2(f[8 * j], f[8 * j + 1], f16), lce_pack2(f[8 * j + 2], f[8 * j + 3], f16),
+                               lce_pack2(f[8 * j + 4], f[8 * j + 5], f16), lce_pack2(f[8 * j + 6], f[8 * j + 7], f16));
+    *reinterpret_cast<uint4*>(dst + lane * 128 + ((j ^ (lane & 7)) << 4)) = v;
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    if (row0 < rows && col0 < cols) tma_store_2d(map, dst, col0, row0);
+    tma_store_commit();
+  }
+  buf ^= 1;
+}
+
+// A_MN / B_MN: the operand's tile is contiguous along M / N in memory (else along K).
+template <int EPI, bool A_MN, bool B_MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LCE_THREADS, 1)
+lce_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                const __grid_constant__ CUtensorMap tmap_c, const LceGemmParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smem_a = smem + LCE_A_OFF;
+  uint8_t* smem_b = smem + LCE_B_OFF;
+  uint8_t* smem_c = smem + LCE_C_OFF;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + LCE_BAR_OFF);   // used in the leader only
+  uint64_t* empty_bar = full_bar + LCE_STAGES;                            // one set per CTA
+  uint64_t* tmem_full_bar = empty_bar + LCE_STAGES;                       // one set per CTA
+  uint64_t* tmem_empty_bar = tmem_full_bar + 2;                           // used in the leader only
+  uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(tmem_empty_bar + 2);
+  uint32_t* abort_smem = tmem_ptr_smem + 1;
+
+  const int warp_idx = threadIdx.x >> 5;
+  const uint32_t lane = lane_id();
+  const uint32_t rank = cluster_ctarank();   // 0 = pair leader
+  const int pair = blockIdx.x >> 1;
+  const int num_pairs = gridDim.x >> 1;
+  WaitCtx ctx{abort_smem, p.status};
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < LCE_STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tmem_full_bar[a], 1);
+      mbar_init(&tmem_empty_bar[a], 2 * LCE_EPI_WARPS);
+    }
+    *abort_smem = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tmap_a);
+    prefetch_tmap(&tmap_b);
+    if (EPI == LCE_DLOGITS || EPI == LCE_DW) prefetch_tmap(&tmap_c);
+  }
+  if (warp_idx == 1) {
+    tmem_alloc_2cta(tmem_ptr_smem, 512);
+    tmem_relinquish_2cta();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_arrive();   // both CTAs' barriers must exist before either CTA signals the other
+  cluster_wait();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_ptr_smem;
+
+  const int count = *p.count;
+  const int M = EPI == LCE_DW ? p.M : count;
+  const int num_kb = ((EPI == LCE_DW ? count : p.K) + 63) >> 6;
+  const LceSchedule sched = lce_schedule(M, p.N, p.group_m, num_pairs);
+
+  if (warp_idx == 0) {
+    // ---------------------------------------------------------------- TMA producer (both CTAs)
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const uint64_t pol_a = l2_policy_evict_last();     // a group's A panel is read again by every tile column
+    const uint64_t pol_b = l2_policy_evict_normal();
+    for (int work = pair; ok && work < sched.num_work; work += num_pairs) {
+      const LceWork wk = lce_work(sched, work);
+      const int m0 = wk.pid_m * 256 + static_cast<int>(rank) * 128;
+      const int n0 = wk.col0 + static_cast<int>(rank) * (wk.width / 2);
+      const int b_boxes = wk.width / 128;
+      for (int kb = 0; kb < num_kb; ++kb) {
+        ok = mbar_wait(&empty_bar[stage], phase ^ 1u, ctx, 61);
+        if (!ok) break;
+        if (lane == 0) {
+          const uint32_t leader_full = mapa_shared(smem_u32(&full_bar[stage]), 0);
+          if (rank == 0) mbar_expect_tx(&full_bar[stage], 2 * (LCE_A_BYTES + b_boxes * LCE_BOX_BYTES));
+          uint8_t* da = smem_a + stage * LCE_A_BYTES;
+          uint8_t* db = smem_b + stage * LCE_B_BYTES;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            tma_load_2d_2cta_hint(da + i * LCE_BOX_BYTES, &tmap_a, leader_full, A_MN ? m0 + i * 64 : kb * 64, A_MN ? kb * 64 : m0 + i * 64, pol_a);
+          for (int i = 0; i < b_boxes; ++i)
+            tma_load_2d_2cta_hint(db + i * LCE_BOX_BYTES, &tmap_b, leader_full, B_MN ? n0 + i * 64 : kb * 64, B_MN ? kb * 64 : n0 + i * 64, pol_b);
+        }
+        __syncwarp();
+        if (++stage == LCE_STAGES) { stage = 0; phase ^= 1u; }
+      }
+    }
+  } else if (warp_idx == 1) {
+    // ---------------------------------------------------------------- MMA issuer (leader only)
+    if (rank == 0 && num_kb > 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int it = 0;
+      bool ok = true;
+      for (int work = pair; ok && work < sched.num_work; work += num_pairs, ++it) {
+        const uint32_t idesc = work >= sched.full_work ? p.idesc_half : p.idesc;
+        const int acc = it & 1;
+        ok = mbar_wait(&tmem_empty_bar[acc], ((it >> 1) & 1) ^ 1u, ctx, 62);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * 256;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          ok = mbar_wait(&full_bar[stage], phase, ctx, 63);
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t a_addr = smem_u32(smem_a + stage * LCE_A_BYTES);
+            const uint32_t b_addr = smem_u32(smem_b + stage * LCE_B_BYTES);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              // K-major: a k step is 32 bytes along the 128-byte rows; M/N-major: 16 rows down, 64-wide chunks one box apart
+              const uint64_t a_desc = umma_smem_desc_sw128(a_addr + k * (A_MN ? 2048 : 32), A_MN ? LCE_BOX_BYTES : 16, 1024);
+              const uint64_t b_desc = umma_smem_desc_sw128(b_addr + k * (B_MN ? 2048 : 32), B_MN ? LCE_BOX_BYTES : 16, 1024);
+              umma_ss_2cta(d_tmem, a_desc, b_desc, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+            }
+            const uint32_t e = smem_u32(&empty_bar[stage]);
+            umma_commit_2cta(mapa_shared(e, 0));
+            umma_commit_2cta(mapa_shared(e, 1));
+            if (kb == num_kb - 1) {
+              const uint32_t f = smem_u32(&tmem_full_bar[acc]);
+              umma_commit_2cta(mapa_shared(f, 0));
+              umma_commit_2cta(mapa_shared(f, 1));
+            }
+          }
+          __syncwarp();
+          if (++stage == LCE_STAGES) { stage = 0; phase ^= 1u; }
+        }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- epilogue (warps 2..5, both CTAs)
+    const int q = warp_idx & 3;
+    uint8_t* my_stage = smem_c + (warp_idx - 2) * 2 * LCE_C_BUF_BYTES;
+    int it = 0, buf = 0;
+    bool ok = true;
+    const float alpha = (EPI == LCE_DW || EPI == LCE_DH) ? *p.alpha : 1.f;
+    for (int work = pair; ok && work < sched.num_work; work += num_pairs, ++it) {
+      const LceWork wk = lce_work(sched, work);
+      const int row0 = wk.pid_m * 256 + static_cast<int>(rank) * 128 + q * 32;
+      const int row = row0 + static_cast<int>(lane);
+      const int chunks = wk.width / 64;
+      const int acc = it & 1;
+      const bool live = row < M;
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * 256;
+      // what the row needs, fetched while the main loop still runs
+      int target = -1, token = 0;
+      float lse2 = 0.f, scale = 0.f;
+      if (EPI == LCE_STATS || EPI == LCE_DLOGITS) target = live ? p.target[row] - p.col_base - wk.col0 : -1;
+      if (EPI == LCE_DLOGITS && live) {
+        lse2 = p.lse2[row];
+        scale = p.row_scale[row];
+      }
+      if (EPI == LCE_DH && live) token = p.token[row];
+      float run_max = -INFINITY, run_sum = 0.f;     // STATS: maximum in units of log2, sum of 2^(x - maximum)
+      if (num_kb > 0) {
+        ok = mbar_wait(&tmem_full_bar[acc], (it >> 1) & 1, ctx, 64);
+        if (!ok) break;
+        tc_fence_after();
+      }
+#pragma unroll 1
+      for (int c = 0; c < chunks; ++c) {
+        float f[64];
+        if (num_kb > 0) {
+          uint32_t v0[32], v1[32];
+          tmem_ld_x32(t_row + c * 64, v0);
+          tmem_ld_x32(t_row + c * 64 + 32, v1);
+          tmem_wait_ld();
+          if (c == chunks - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&tmem_empty_bar[acc]), 0));
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            f[j] = __uint_as_float(v0[j]);
+            f[32 + j] = __uint_as_float(v1[j]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 64; ++j) f[j] = 0.f;
+        }
+        const int col0 = wk.col0 + c * 64;
+        const int in = target - c * 64;              // the target's place in this chunk
+        if constexpr (EPI == LCE_STATS) {
+          if (in >= 0 && in < 64 && col0 + in < p.N) {
+            float t = 0.f;
+#pragma unroll
+            for (int j = 0; j < 64; ++j) t = j == in ? f[j] : t;
+            p.target_logit[row] = t;
+          }
+          if (col0 + 64 > p.N) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) f[j] = col0 + j < p.N ? f[j] : -INFINITY;
+          }
+          float m = f[0];
+#pragma unroll
+          for (int j = 1; j < 63; j += 2) m = fmax3(m, f[j], f[j + 1]);
+          m = fmaxf(m, f[63]);
+          const float new_max = fmaxf(run_max, m * LOG2E);
+          const float shift = new_max == -INFINITY ? 0.f : new_max;     // a row of -inf: the sum stays 0
+          float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll
+          for (int j = 0; j < 64; j += 4) {
+            s0 += exp2f(fmaf(f[j], LOG2E, -shift));
+            s1 += exp2f(fmaf(f[j + 1], LOG2E, -shift));
+            s2 += exp2f(fmaf(f[j + 2], LOG2E, -shift));
+            s3 += exp2f(fmaf(f[j + 3], LOG2E, -shift));
+          }
+          run_sum = fmaf(run_sum, exp2f(run_max - shift), (s0 + s1) + (s2 + s3));
+          run_max = new_max;
+        } else if constexpr (EPI == LCE_DLOGITS) {
+#pragma unroll
+          for (int j = 0; j < 64; ++j) {
+            const float e = exp2f(fmaf(f[j], LOG2E, -lse2)) - (j == in ? 1.f : 0.f);
+            f[j] = live ? e * scale : 0.f;           // rows behind the last one that counts: zeros, for the K tail of dW
+          }
+          if (col0 + 64 > p.N) {                       // columns behind the piece: zeros, for the K tail of dh
+#pragma unroll
+            for (int j = 0; j < 64; ++j) f[j] = col0 + j < p.N ? f[j] : 0.f;
+          }
+          lce_store_chunk(&tmap_c, f, p.f16, row0, col0, p.M, p.N, my_stage, buf, lane);   // the map ends on a multiple of 8 columns
+        } else if constexpr (EPI == LCE_DW) {
+#pragma unroll
+          for (int j = 0; j < 64; ++j) f[j] *= alpha;
+          lce_store_chunk(&tmap_c, f, p.f16, row0, col0, p.M, p.N, my_stage, buf, lane);
+        } else {
+          // K (= D) is a multiple of 8, so a row of the result ends on a multiple of 8 columns
+          if (live) {
+            const int cols = min(64, p.N - col0);
+            const int64_t at = static_cast<int64_t>(row) * p.N + col0;
+            if (p.add != nullptr) {
+#pragma unroll
+              for (int j = 0; j < 64; j += 4)
+                if (j < cols) {
+                  const float4 a = *reinterpret_cast<const float4*>(p.add + at + j);
+                  f[j] += a.x; f[j + 1] += a.y; f[j + 2] += a.z; f[j + 3] += a.w;
+                }
+            }
+            if (p.sum != nullptr) {
+#pragma unroll
+              for (int j = 0; j < 64; j += 4)
+                if (j < cols) *reinterpret_cast<float4*>(p.sum + at + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+            } else {
+              uint16_t* out = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(token) * p.N + col0;
+#pragma unroll
+              for (int j = 0; j < 64; j += 8)
+                if (j < cols)
+                  *reinterpret_cast<uint4*>(out + j) =
+                      make_uint4(lce_pack2(f[j] * alpha, f[j + 1] * alpha, p.f16), lce_pack2(f[j + 2] * alpha, f[j + 3] * alpha, p.f16),
+                                 lce_pack2(f[j + 4] * alpha, f[j + 5] * alpha, p.f16), lce_pack2(f[j + 6] * alpha, f[j + 7] * alpha, p.f16));
+            }
+          }
+        }
+      }
+      if (EPI == LCE_STATS && live) p.part[static_cast<int64_t>(wk.col0 >> 7) * p.part_ld + row] = make_float2(run_max, run_sum);
+      // a whole tile spans two 128-column slots of `part`
+      if (EPI == LCE_STATS && live && wk.width == 256)
+        p.part[static_cast<int64_t>((wk.col0 >> 7) + 1) * p.part_ld + row] = make_float2(-INFINITY, 0.f);
+    }
+    if (lane == 0) tma_store_wait_all<0>();
+    __syncwarp();
+  }
+
+  // ------------------------------------------------------------------ teardown
+  drain_after_abort(abort_smem);
+  tc_fence_before();
+  __syncthreads();
+  cluster_arrive();   // neither CTA may exit while its partner can still signal its barriers
+  cluster_wait();
+  if (warp_idx == 1) {
+    tc_fence_after();
+    tmem_dealloc_2cta(tmem_base, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Gather: the rows that count move to the front of `hc`, in order; the other rows of `hc` become zeros.
+// ---------------------------------------------------------------------------------------------
+constexpr int LCE_GATHER_ROWS = 32;
+
+struct LceGatherParams {
+  const uint4* h;
+  int64_t ldh8;            // row pitch of h in 16-byte units
+  const int64_t* target;
+  int64_t ignore;
+  int T, D8, V;            // D8: 16-byte units of a row
+  uint4* hc;
+  int* count;
+  int* token;
+  int* row_target;
+  // forward
+  float* target_logit;
+  float* losses;
+  float* lse;
+  // backward
+  const float* lse_in;
+  const float* d_loss;     // per token when gmax is not null, else one number
+  const float* gmax;
+  float* row_lse2;
+  float* row_scale;
+  uint4* dh;
+  float* alpha;
+  float unit;              // 1 or LCE_F16_SCALE
+  int mean;
+};
+
+template <bool BACKWARD>
+__global__ void __launch_bounds__(256) lce_gather_kernel(const LceGatherParams p) {
+  __shared__ int warp_counts[8];
+  __shared__ int place[LCE_GATHER_ROWS];       // row of hc; valid ones >= 0, others -1 - row
+  __shared__ int total_smem;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first = blockIdx.x * LCE_GATHER_ROWS;
+  const bool last_cta = blockIdx.x == gridDim.x - 1;
+  // tokens that count before this CTA's rows
+  int n = 0;
+  for (int i = threadIdx.x; i < first; i += 256) n += p.target[i] != p.ignore ? 1 : 0;
+  n = __reduce_add_sync(0xFFFFFFFFu, n);
+  if (lane == 0) warp_counts[warp] = n;
+  __syncthreads();
+  if (warp == 0) {
+    int before = __reduce_add_sync(0xFFFFFFFFu, lane < 8 ? warp_counts[lane] : 0);
+    const int t = first + lane;
+    const int64_t y = t < p.T ? p.target[t] : p.ignore;
+    const bool counts = t < p.T && y != p.ignore;
+    const unsigned mask = __ballot_sync(0xFFFFFFFFu, counts);
+    const int at = before + __popc(mask & ((1u << lane) - 1u));   // rows that count before this one
+    if (t < p.T) {
+      const int row = counts ? at : p.T - 1 - (t - at);           // the k-th row that does not count takes the k-th place from the back
+      place[lane] = counts ? row : -1 - row;
+      const bool valid = y >= 0 && y < p.V;
+      p.row_target[row] = counts && valid ? static_cast<int>(y) : -(1 << 29);   // matches no column
+      p.token[row] = t;
+      if (BACKWARD) {
+        p.row_lse2[row] = counts ? p.lse_in[t] * LOG2E : 0.f;
+        float g = 1.f;
+        if (p.gmax != nullptr) {
+          const float m = *p.gmax;
+          g = m > 0.f ? p.d_loss[t] / m : p.d_loss[t];
+        }
+        // a target outside the vocabulary: NaN, in the loss and in every gradient that it enters
+        p.row_scale[row] = counts ? (valid ? g * p.unit : __int_as_float(0x7FC00000)) : 0.f;
+      } else {
+        p.target_logit[row] = __int_as_float(0x7FC00000);         // the product's epilogue puts the logit here
+        if (!counts) {
+          p.losses[t] = 0.f;
+          p.lse[t] = 0.f;
+        }
+      }
+    }
+    if (lane == 0) total_smem = before + __popc(mask);
+  }
+  __syncthreads();
+  if (last_cta && threadIdx.x == 0) {
+    const int total = total_smem;
+    *p.count = total;
+    if (BACKWARD) {
+      float a = p.gmax != nullptr ? (*p.gmax > 0.f ? *p.gmax : 1.f) : *p.d_loss;
+      if (p.mean) a /= static_cast<float>(total > 0 ? total : 1);
+      *p.alpha = a / p.unit;
+    }
+  }
+  const int rows = min(LCE_GATHER_ROWS, p.T - first);
+  for (int r = warp; r < rows; r += 8) {
+    const int code = place[r];
+    const bool counts = code >= 0;
+    uint4* dst = p.hc + static_cast<int64_t>(counts ? code : -1 - code) * p.D8;
+    const uint4* src = p.h + static_cast<int64_t>(first + r) * p.ldh8;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    for (int i = lane; i < p.D8; i += 32) {
+      dst[i] = counts ? src[i] : zero;
+      if (BACKWARD && !counts && p.dh != nullptr) p.dh[static_cast<int64_t>(first + r) * p.D8 + i] = zero;
+    }
+  }
+}
+
+// Largest magnitude of the tokens' gradients, of those that count and are finite.
+__global__ void __launch_bounds__(1024) lce_gmax_kernel(const float* __restrict__ g, const int64_t* __restrict__ target, int64_t ignore, int T,
+                                                        float* __restrict__ gmax) {
+  __shared__ float warps[32];
+  float m = 0.f;
+  for (int i = threadIdx.x; i < T; i += 1024) {
+    const float a = fabsf(g[i]);
+    if (target[i] != ignore && a <= 3.4028234663852886e38f) m = fmaxf(m, a);
+  }
+  m = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(m)));
+  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = m;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    m = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(warps[threadIdx.x])));
+    if (threadIdx.x == 0) *gmax = m;
+  }
+}
+
+// Joins the tile columns' (maximum, sum) of 32 rows: 32 slices of the slots, one row per lane.
+__global__ void __launch_bounds__(1024) lce_join_kernel(const float2* __restrict__ part, int64_t part_ld, int slots, const int* __restrict__ count,
+                                                        const float* __restrict__ target_logit, const int* __restrict__ token,
+                                                        float* __restrict__ losses, float* __restrict__ lse) {
+  __shared__ float2 joined[32][33];
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const int row = blockIdx.x * 32 + lane;
+  const bool live = row < *count;
+  float m = -INFINITY, s = 0.f;
+  if (live)
+    for (int i = slice; i < slots; i += 32) {
+      const float2 v = part[static_cast<int64_t>(i) * part_ld + row];
+      const float top = fmaxf(m, v.x);
+      const float shift = top == -INFINITY ? 0.f : top;
+      s = s * exp2f(m - shift) + v.y * exp2f(v.x - shift);
+      m = top;
+    }
+  joined[slice][lane] = make_float2(m, s);
+  __syncthreads();
+  if (slice == 0 && live) {
+    for (int i = 1; i < 32; ++i) {
+      const float2 v = joined[i][lane];
+      const float top = fmaxf(m, v.x);
+      const float shift = top == -INFINITY ? 0.f : top;
+      s = s * exp2f(m - shift) + v.y * exp2f(v.x - shift);
+      m = top;
+    }
+    const float lse2 = m + log2f(s);
+    const int t = token[row];
+    lse[t] = lse2 * LN2;
+    losses[t] = fmaf(-target_logit[row], LOG2E, lse2) * LN2;
+  }
+}
+
+// Sum or mean of the losses, in an order that depends on T only.
+__global__ void __launch_bounds__(1024) lce_reduce_kernel(const float* __restrict__ losses, int T, const int* __restrict__ count, int mean,
+                                                          float* __restrict__ loss) {
+  __shared__ double warps[32];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < T; i += 1024) s += static_cast<double>(losses[i]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    s = warps[threadIdx.x];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+    if (threadIdx.x == 0) {
+      const int n = *count;
+      *loss = static_cast<float>(mean ? s / (n > 0 ? n : 1) : s);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------------------------
+// Bytes of dlogits that a piece of the vocabulary may take.
+constexpr int64_t LCE_PIECE_BYTES = int64_t(512) << 20;
+
+static int lce_piece(int T, int V) {
+  const int64_t most = LCE_PIECE_BYTES / (2 * static_cast<int64_t>(T)) / 256 * 256;
+  const int64_t piece = most < 256 ? 256 : most;
+  if (piece >= V) return V;
+  const int64_t pieces = (V + piece - 1) / piece;
+  return static_cast<int>(((V + pieces - 1) / pieces + 255) / 256 * 256);     // pieces of about one size
+}
+
+struct LceLayout {
+  int64_t hc, token, row_target, count, alpha, gmax, a, b, part, dl, sum, total;   // byte offsets
+  int slots, piece, pieces;
+  int64_t ld_dl;
+};
+static LceLayout lce_layout(int T, int D, int V, bool backward) {
+  LceLayout l{};
+  int64_t at = 0;
+  auto take = [&at](int64_t bytes) {
+    const int64_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  l.count = take(4);
+  l.alpha = take(4);
+  l.gmax = take(4);
+  l.token = take(4ll * T);
+  l.row_target = take(4ll * T);
+  l.a = take(4ll * T);           // forward: target logits; backward: lse * log2 e
+  l.hc = take(2ll * T * D);
+  if (!backward) {
+    l.slots = 2 * ((V + 255) / 256);
+    l.part = take(8ll * T * l.slots);
+  } else {
+    l.b = take(4ll * T);         // row factors
+    l.piece = lce_piece(T, V);
+    l.pieces = (V + l.piece - 1) / l.piece;
+    l.ld_dl = (l.piece + 7) / 8 * 8;
+    l.dl = take(2ll * T * l.ld_dl);
+    if (l.pieces > 1) l.sum = take(4ll * T * D);
+  }
+  l.total = at;
+  return l;
+}
+
+int64_t lce_workspace(int T, int D, int V, int backward) { return lce_layout(T, D, V, backward != 0).total; }
+
+static int lce_check(const LceArgs& a, const char* what) {
+  if (a.T < 0 || a.D < 8 || a.V < 1 || (a.D & 7)) return set_error(B200K_ERR_INVALID_ARG, "%s: T >= 0, V >= 1 and D a positive multiple of 8 expected (got %d, %d, %d)", what, a.T, a.V, a.D);
+  if (a.V > (1 << 30) || a.T > (1 << 30)) return set_error(B200K_ERR_INVALID_ARG, "%s: at most 2^30 tokens and vocabulary entries", what);
+  if (a.dtype != B200K_DTYPE_BF16 && a.dtype != B200K_DTYPE_F16) return set_error(B200K_ERR_INVALID_ARG, "%s: bf16 or fp16 operands expected (got type %d)", what, a.dtype);
+  if (a.reduction < B200K_REDUCE_NONE || a.reduction > B200K_REDUCE_SUM) return set_error(B200K_ERR_INVALID_ARG, "%s: bad reduction %d", what, a.reduction);
+  if (static_cast<int64_t>((a.T + 255) / 256) * ((a.V + 255) / 256) > 0x3FFFFFFF || static_cast<int64_t>((a.V + 255) / 256) * ((a.D + 255) / 256) > 0x3FFFFFFF)
+    return set_error(B200K_ERR_INVALID_ARG, "%s: too many tiles", what);
+  if (a.T > 0) {
+    if (a.h == nullptr || a.w == nullptr || a.target == nullptr) return set_error(B200K_ERR_INVALID_ARG, "%s: null pointer", what);
+    if (a.ldh < a.D || a.ldw < a.D || (a.ldh & 7) || (a.ldw & 7))
+      return set_error(B200K_ERR_INVALID_ARG, "%s: row pitches must be multiples of 8 elements and at least D (got %lld, %lld)", what, (long long)a.ldh, (long long)a.ldw);
+    if ((reinterpret_cast<uintptr_t>(a.h) | reinterpret_cast<uintptr_t>(a.w) | reinterpret_cast<uintptr_t>(a.dh) | reinterpret_cast<uintptr_t>(a.dw)) & 15u)
+      return set_error(B200K_ERR_INVALID_ARG, "%s: h, w and their gradients must be 16-byte aligned", what);
+    if (reinterpret_cast<uintptr_t>(a.workspace) & 255u) return set_error(B200K_ERR_INVALID_ARG, "%s: the workspace must be 256-byte aligned", what);
+  }
+  return B200K_OK;
+}
+
+static int lce_check_workspace(const LceArgs& a, const LceLayout& l, const char* what) {
+  if (a.workspace == nullptr || a.workspace_bytes < l.total)
+    return set_error(B200K_ERR_INVALID_ARG, "%s: a workspace of %lld bytes is needed (got %lld)", what, (long long)l.total, (long long)(a.workspace == nullptr ? 0 : a.workspace_bytes));
+  return B200K_OK;
+}
+
+template <int EPI, bool A_MN, bool B_MN>
+static int lce_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, LceGemmParams p, const DeviceInfo* dev, cudaStream_t stream) {
+  p.group_m = 8;
+  p.idesc = umma_idesc_16bit_f32(256, 256, A_MN, B_MN, p.f16);
+  p.idesc_half = umma_idesc_16bit_f32(256, 128, A_MN, B_MN, p.f16);
+  p.status = dev->status_word;
+  B200K_CHECK_CUDA(cudaFuncSetAttribute(lce_gemm_kernel<EPI, A_MN, B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, LCE_SMEM));
+  const int64_t tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256);
+  const int max_pairs = dev->sm_count / 2;
+  // twice the tiles: a short launch is one wave of column halves
+  const int pairs = static_cast<int>(2 * tiles < max_pairs ? 2 * tiles : max_pairs);
+  lce_gemm_kernel<EPI, A_MN, B_MN><<<2 * pairs, LCE_THREADS, LCE_SMEM, stream>>>(ta, tb, tc, p);
+  count_launch();
+  B200K_CHECK_LAUNCH("lce_gemm_kernel");
+  return B200K_OK;
+}
+
+static const DeviceInfo* lce_device(const char* what) {
+  const DeviceInfo* dev = current_device_info();
+  if (dev != nullptr && dev->cc_major != 10) {
+    set_error(B200K_ERR_NO_DEVICE, "%s: needs an sm_100 device (found sm_%d%d)", what, dev->cc_major, dev->cc_minor);
+    return nullptr;
+  }
+  return dev;
+}
+
+int lce_fwd(const LceArgs& a, cudaStream_t stream) {
+  const char* what = "linear_cross_entropy";
+  int rc = lce_check(a, what);
+  if (rc != B200K_OK) return rc;
+  if (a.reduction != B200K_REDUCE_NONE && a.loss == nullptr) return set_error(B200K_ERR_INVALID_ARG, "%s: null loss", what);
+  if (a.T == 0) {
+    if (lce_device(what) == nullptr) return B200K_ERR_NO_DEVICE;
+    if (a.reduction != B200K_REDUCE_NONE) B200K_CHECK_CUDA(cudaMemsetAsync(a.loss, 0, sizeof(float), stream));
+    return B200K_OK;
+  }
+  const LceLayout l = lce_layout(a.T, a.D, a.V, false);
+  if (a.losses == nullptr || a.lse == nullptr) return set_error(B200K_ERR_INVALID_ARG, "%s: null losses or lse", what);
+  if ((rc = lce_check_workspace(a, l, what)) != B200K_OK) return rc;
+  const DeviceInfo* dev = lce_device(what);
+  if (dev == nullptr) return B200K_ERR_NO_DEVICE;
+  char* ws = static_cast<char*>(a.workspace);
+  int* count = reinterpret_cast<int*>(ws + l.count);
+  int* token = reinterpret_cast<int*>(ws + l.token);
+
+  LceGatherParams g{};
+  g.h = static_cast<const uint4*>(a.h);
+  g.ldh8 = a.ldh / 8;
+  g.target = a.target;
+  g.ignore = a.ignore_index;
+  g.T = a.T; g.D8 = a.D / 8; g.V = a.V;
+  g.hc = reinterpret_cast<uint4*>(ws + l.hc);
+  g.count = count;
+  g.token = token;
+  g.row_target = reinterpret_cast<int*>(ws + l.row_target);
+  g.target_logit = reinterpret_cast<float*>(ws + l.a);
+  g.losses = a.losses;
+  g.lse = a.lse;
+  lce_gather_kernel<false><<<(a.T + LCE_GATHER_ROWS - 1) / LCE_GATHER_ROWS, 256, 0, stream>>>(g);
+  count_launch();
+  B200K_CHECK_LAUNCH("lce_gather_kernel");
+
+  CUtensorMap th, tw;
+  if ((rc = make_tmap_bf16_2d(&th, ws + l.hc, a.D, a.T, a.D, 64, 64)) != 0) return rc;
+  if ((rc = make_tmap_bf16_2d(&tw, a.w, a.D, a.V, a.ldw, 64, 64)) != 0) return rc;
+  LceGemmParams p{};
+  p.count = count;
+  p.M = a.T; p.N = a.V; p.K = a.D;
+  p.f16 = a.dtype == B200K_DTYPE_F16;
+  p.target = g.row_target;
+  p.part = reinterpret_cast<float2*>(ws + l.part);
+  p.part_ld = a.T;
+  p.target_logit = g.target_logit;
+  if ((rc = lce_gemm<LCE_STATS, false, false>(th, tw, th, p, dev, stream)) != 0) return rc;
+
+  lce_join_kernel<<<(a.T + 31) / 32, 1024, 0, stream>>>(p.part, p.part_ld, l.slots, count, g.target_logit, token, a.losses, a.lse);
+  count_launch();
+  B200K_CHECK_LAUNCH("lce_join_kernel");
+  if (a.reduction != B200K_REDUCE_NONE) {
+    lce_reduce_kernel<<<1, 1024, 0, stream>>>(a.losses, a.T, count, a.reduction == B200K_REDUCE_MEAN, a.loss);
+    count_launch();
+    B200K_CHECK_LAUNCH("lce_reduce_kernel");
+  }
+  return B200K_OK;
+}
+
+int lce_bwd(const LceArgs& a, cudaStream_t stream) {
+  const char* what = "linear_cross_entropy_backward";
+  int rc = lce_check(a, what);
+  if (rc != B200K_OK) return rc;
+  if (a.T == 0) {
+    if (lce_device(what) == nullptr) return B200K_ERR_NO_DEVICE;
+    if (a.dw != nullptr) B200K_CHECK_CUDA(cudaMemsetAsync(a.dw, 0, 2ll * a.V * a.D, stream));
+    return B200K_OK;
+  }
+  if (a.lse == nullptr || a.d_loss == nullptr) return set_error(B200K_ERR_INVALID_ARG, "%s: null lse or d_loss", what);
+  const LceLayout l = lce_layout(a.T, a.D, a.V, true);
+  if ((rc = lce_check_workspace(a, l, what)) != B200K_OK) return rc;
+  const DeviceInfo* dev = lce_device(what);
+  if (dev == nullptr) return B200K_ERR_NO_DEVICE;
+  if (a.dh == nullptr && a.dw == nullptr) return B200K_OK;
+  char* ws = static_cast<char*>(a.workspace);
+  float* gmax = reinterpret_cast<float*>(ws + l.gmax);
+  const bool each = a.reduction == B200K_REDUCE_NONE;
+  if (each) {
+    lce_gmax_kernel<<<1, 1024, 0, stream>>>(a.d_loss, a.target, a.ignore_index, a.T, gmax);
+    count_launch();
+    B200K_CHECK_LAUNCH("lce_gmax_kernel");
+  }
+  LceGatherParams g{};
+  g.h = static_cast<const uint4*>(a.h);
+  g.ldh8 = a.ldh / 8;
+  g.target = a.target;
+  g.ignore = a.ignore_index;
+  g.T = a.T; g.D8 = a.D / 8; g.V = a.V;
+  g.hc = reinterpret_cast<uint4*>(ws + l.hc);
+  g.count = reinterpret_cast<int*>(ws + l.count);
+  g.token = reinterpret_cast<int*>(ws + l.token);
+  g.row_target = reinterpret_cast<int*>(ws + l.row_target);
+  g.lse_in = a.lse;
+  g.d_loss = a.d_loss;
+  g.gmax = each ? gmax : nullptr;
+  g.row_lse2 = reinterpret_cast<float*>(ws + l.a);
+  g.row_scale = reinterpret_cast<float*>(ws + l.b);
+  g.dh = static_cast<uint4*>(a.dh);
+  g.alpha = reinterpret_cast<float*>(ws + l.alpha);
+  g.unit = a.dtype == B200K_DTYPE_F16 ? LCE_F16_SCALE : 1.f;
+  g.mean = a.reduction == B200K_REDUCE_MEAN;
+  lce_gather_kernel<true><<<(a.T + LCE_GATHER_ROWS - 1) / LCE_GATHER_ROWS, 256, 0, stream>>>(g);
+  count_launch();
+  B200K_CHECK_LAUNCH("lce_gather_kernel");
+
+  CUtensorMap th;
+  if ((rc = make_tmap_bf16_2d(&th, ws + l.hc, a.D, a.T, a.D, 64, 64)) != 0) return rc;
+  float* sum = l.pieces > 1 ? reinterpret_cast<float*>(ws + l.sum) : nullptr;
+  for (int k = 0; k < l.pieces; ++k) {
+    const int v0 = k * l.piece;
+    const int n = a.V - v0 < l.piece ? a.V - v0 : l.piece;
+    const int cols = (n + 7) / 8 * 8;     // dlogits of the piece, its last columns zeros
+    CUtensorMap tw, tdl, tdl_store, tdw;
+    const uint16_t* w = static_cast<const uint16_t*>(a.w) + static_cast<int64_t>(v0) * a.ldw;
+    if ((rc = make_tmap_bf16_2d(&tw, w, a.D, n, a.ldw, 64, 64)) != 0) return rc;
+    if ((rc = make_tmap_bf16_2d(&tdl, ws + l.dl, cols, a.T, l.ld_dl, 64, 64)) != 0) return rc;
+    if ((rc = make_tmap_bf16_2d(&tdl_store, ws + l.dl, cols, a.T, l.ld_dl, 64, 32)) != 0) return rc;
+    LceGemmParams p{};
+    p.count = g.count;
+    p.f16 = a.dtype == B200K_DTYPE_F16;
+    p.alpha = g.alpha;
+    p.M = a.T; p.N = n; p.K = a.D;
+    p.target = g.row_target;
+    p.col_base = v0;
+    p.lse2 = g.row_lse2;
+    p.row_scale = g.row_scale;
+    if ((rc = lce_gemm<LCE_DLOGITS, false, false>(th, tw, tdl_store, p, dev, stream)) != 0) return rc;
+    if (a.dw != nullptr) {
+      uint16_t* dw = static_cast<uint16_t*>(a.dw) + static_cast<int64_t>(v0) * a.D;
+      if ((rc = make_tmap_bf16_2d(&tdw, dw, a.D, n, a.D, 64, 32)) != 0) return rc;
+      p.M = n; p.N = a.D; p.K = a.T;
+      if ((rc = lce_gemm<LCE_DW, true, true>(tdl, th, tdw, p, dev, stream)) != 0) return rc;
+    }
+    if (a.dh != nullptr) {
+      p.M = a.T; p.N = a.D; p.K = n;
+      p.add = k > 0 ? sum : nullptr;
+      p.sum = k + 1 < l.pieces ? sum : nullptr;
+      p.out = a.dh;
+      p.token = g.token;
+      if ((rc = lce_gemm<LCE_DH, false, true>(tdl, tw, tw, p, dev, stream)) != 0) return rc;
+    }
+  }
+  return B200K_OK;
+}
+
+}  // namespace b200k

@@ -16,7 +16,8 @@ import torch
 from . import _lib
 
 __all__ = ["add", "add_loop", "sin", "memcpy", "mul_add", "matmul", "tilize", "untilize", "matmul_tma", "matmul_tma_host_rows", "matmul_multi", "matmul_fused", "matmul_tma_fused", "attention", "attention_multi",
-           "attention_with_lse", "attention_backward", "layer_norm", "layer_norm_with_stats", "layer_norm_backward", "device_status"]
+           "attention_with_lse", "attention_backward", "layer_norm", "layer_norm_with_stats", "layer_norm_backward",
+           "linear_cross_entropy", "linear_cross_entropy_with_lse", "linear_cross_entropy_backward", "device_status"]
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -655,6 +656,112 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5) -> torch.Tensor:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return _layer_norm.apply(x, weight, bias, eps)
     return layer_norm_with_stats(x, weight, bias, eps)[0]
+
+
+_REDUCTIONS = {"none": _lib.REDUCE_NONE, "mean": _lib.REDUCE_MEAN, "sum": _lib.REDUCE_SUM}
+
+
+def _lce_check(name, h, weight, targets, reduction):
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"{name}: unknown reduction {reduction!r} (expected 'none', 'mean' or 'sum')")
+    if h.dtype not in (torch.bfloat16, torch.float16) or weight.dtype != h.dtype:
+        raise TypeError(f"{name}: h and weight must both be bf16 or both fp16, got {h.dtype} and {weight.dtype}")
+    if targets.dtype != torch.int64:
+        raise TypeError(f"{name}: targets must be int64, got {targets.dtype}")
+    if h.dim() < 1 or weight.dim() != 2 or h.shape[-1] != weight.shape[1] or weight.shape[0] < 1:
+        raise ValueError(f"{name}: h [..., D] and weight [V, D] expected, got {tuple(h.shape)} and {tuple(weight.shape)}")
+    if weight.shape[1] < 8 or weight.shape[1] % 8:
+        raise ValueError(f"{name}: D must be a positive multiple of 8 (16-byte rows); got {weight.shape[1]}")
+    if targets.shape != h.shape[:-1]:
+        raise ValueError(f"{name}: targets must be {tuple(h.shape[:-1])} like h without its last dimension, got {tuple(targets.shape)}")
+    if weight.device != h.device or targets.device != h.device:
+        raise ValueError(f"{name}: tensors on different devices")
+
+
+def _tma_rows(t: torch.Tensor) -> torch.Tensor:
+    """The [rows, D] view of t with unit inner stride and separate 16-byte rows, or a copy."""
+    t2 = _rows_of(t)
+    if t2.shape[0] > 0 and (t2.data_ptr() % 16 or _pitch(t2) % 8 or _pitch(t2) < t2.shape[1]):
+        t2 = t2.clone(memory_format=torch.contiguous_format)
+    return t2
+
+
+def _lce_forward(h, weight, targets, ignore_index, reduction):
+    """(losses, lse, loss), on the device."""
+    lib = _lib.load()
+    hd, wd, td = _tma_rows(_to_device(h)), _tma_rows(_to_device(weight)), _to_device(targets).contiguous()
+    (T, D), V = hd.shape, wd.shape[0]
+    out = torch.empty((2, T), device=hd.device, dtype=torch.float32)
+    loss = torch.empty((), device=hd.device, dtype=torch.float32)
+    size = lib.b200k_lce_workspace(T, D, V, 0)
+    work = torch.empty(size, device=hd.device, dtype=torch.uint8)
+    with _on(hd.device):
+        _lib.check(lib.b200k_lce_fwd(hd.data_ptr(), wd.data_ptr(), td.data_ptr(), out.data_ptr(), out.data_ptr() + 4 * T, loss.data_ptr(),
+                                     work.data_ptr(), size, T, D, V, _pitch(hd), _pitch(wd), ignore_index, _REDUCTIONS[reduction],
+                                     _DTYPES[h.dtype], _stream()))
+    return out[0].view(targets.shape), out[1].view(targets.shape), loss
+
+
+def linear_cross_entropy_with_lse(h, weight, targets, ignore_index: int = -100):
+    """Returns (losses, lse), fp32 in the shape of targets: lse = log sum_v exp(h . weight[v]) and losses = lse - h . weight[target].  Both are 0
+    for a token whose target is ignore_index.  Not differentiable; lse is what linear_cross_entropy_backward takes."""
+    _lce_check("linear_cross_entropy", h, weight, targets, "none")
+    losses, lse, _ = _lce_forward(h, weight, targets, ignore_index, "none")
+    return _like_input(losses, h), _like_input(lse, h)
+
+
+def linear_cross_entropy_backward(h, weight, targets, lse, d_loss, ignore_index: int = -100, reduction: str = "none", need_dh: bool = True,
+                                  need_dw: bool = True):
+    """(dh, dw) from the lse of the forward and the fp32 gradient of the losses (reduction "none": in the shape of targets) or of their mean or
+    sum (one element).  A gradient that is not needed is None."""
+    _lce_check("linear_cross_entropy_backward", h, weight, targets, reduction)
+    if lse.dtype != torch.float32 or lse.shape != targets.shape or lse.device != h.device:
+        raise ValueError(f"linear_cross_entropy_backward: lse must be fp32 {tuple(targets.shape)} on h's device")
+    if d_loss.dtype != torch.float32 or d_loss.device != h.device or (d_loss.shape != targets.shape if reduction == "none" else d_loss.numel() != 1):
+        raise ValueError("linear_cross_entropy_backward: d_loss must be fp32 on h's device, " +
+                         (f"{tuple(targets.shape)}" if reduction == "none" else "one element") + f"; got {d_loss.dtype} {tuple(d_loss.shape)}")
+    lib = _lib.load()
+    hd, wd, td = _tma_rows(_to_device(h)), _tma_rows(_to_device(weight)), _to_device(targets).contiguous()
+    ld, gd = _to_device(lse).contiguous(), _to_device(d_loss).contiguous()
+    (T, D), V = hd.shape, wd.shape[0]
+    dh = torch.empty((T, D), device=hd.device, dtype=h.dtype) if need_dh else None
+    dw = torch.empty((V, D), device=hd.device, dtype=h.dtype) if need_dw else None
+    size = lib.b200k_lce_workspace(T, D, V, 1) if need_dh or need_dw else 0
+    work = torch.empty(size, device=hd.device, dtype=torch.uint8)
+    if need_dh or need_dw:
+        with _on(hd.device):
+            _lib.check(lib.b200k_lce_bwd(hd.data_ptr(), wd.data_ptr(), td.data_ptr(), ld.data_ptr(), gd.data_ptr(),
+                                         0 if dh is None else dh.data_ptr(), 0 if dw is None else dw.data_ptr(), work.data_ptr(), size, T, D, V,
+                                         _pitch(hd), _pitch(wd), ignore_index, _REDUCTIONS[reduction], _DTYPES[h.dtype], _stream()))
+    return (None if dh is None else _like_input(dh.view(h.shape), h), None if dw is None else _like_input(dw, h))
+
+
+class _linear_cross_entropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, weight, targets, ignore_index, reduction):
+        losses, lse, loss = _lce_forward(h, weight, targets, ignore_index, reduction)
+        ctx.save_for_backward(h, weight, targets, _like_input(lse, h))
+        ctx.ignore_index, ctx.reduction = ignore_index, reduction
+        return _like_input(losses if reduction == "none" else loss, h)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_loss):
+        h, weight, targets, lse = ctx.saved_tensors
+        dh, dw = linear_cross_entropy_backward(h, weight, targets, lse, d_loss, ctx.ignore_index, ctx.reduction, *ctx.needs_input_grad[:2])
+        return dh, dw, None, None, None
+
+
+def linear_cross_entropy(h, weight, targets, ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+    """Cross entropy of the logits h . weight^T without ever storing them: h [..., D] and weight [V, D] in bf16 or fp16, targets int64.
+    reduction "mean" (over the tokens whose target is not ignore_index; 0 without any), "sum", or "none" (fp32 in the shape of targets, 0 for
+    ignored tokens).  What h holds for ignored tokens does not matter, NaN included; any other target outside [0, V) makes its token's loss
+    NaN.  Differentiable in h and weight."""
+    _lce_check("linear_cross_entropy", h, weight, targets, reduction)
+    if torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad):
+        return _linear_cross_entropy.apply(h, weight, targets, ignore_index, reduction)
+    losses, _, loss = _lce_forward(h, weight, targets, ignore_index, reduction)
+    return _like_input(losses if reduction == "none" else loss, h)
 
 
 def device_status() -> int:
