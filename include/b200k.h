@@ -245,7 +245,7 @@ int b200k_layer_norm_fwd(const void* x, const void* w, const void* b, void* y, f
  *   dx = rstd (u - mean(u) - h mean(u h)),   dw = sum over rows of dy h,   db = sum over rows of dy.
  *   dx          [rows, cols] of type `dtype` (pitch lddx) or null; must not overlap dy or x
  *   dw, db      [cols] of type `wdtype`, either may be null; zeros when rows = 0
- *   workspace   b200k_layer_norm_bwd_workspace(rows, cols) floats for their partial sums (none needed when both are null)
+ *   workspace   b200k_layer_norm_bwd_workspace(rows, cols) floats, 16-byte aligned, for their partial sums (none needed when both are null)
  * Deterministic: no atomics, the sums' order depends on the sizes only.
  */
 int b200k_layer_norm_bwd(const void* dy, const void* x, const void* w, const float* mean, const float* rstd, void* dx, void* dw, void* db,

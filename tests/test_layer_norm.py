@@ -264,7 +264,7 @@ def test_entry_point_refusals():
     fwd = lambda x=16, y=16, rows=4, cols=8, ldx=8, ldy=8, dt=0, wdt=0, eps=1e-5: lib.b200k_layer_norm_fwd(  # noqa: E731
         x, None, None, y, None, None, rows, cols, ldx, ldy, dt, wdt, eps, None)
     for bad in [dict(dt=3), dict(dt=-1), dict(dt=1, wdt=2), dict(rows=-1), dict(cols=0), dict(cols=2 ** 31), dict(rows=2 ** 60, cols=2 ** 20), dict(x=None),
-                dict(y=None), dict(ldx=-8), dict(ldy=7), dict(eps=-1.0), dict(eps=float("nan"))]:
+                dict(y=None), dict(x=18), dict(y=17, dt=1, wdt=1), dict(ldx=-8), dict(ldy=7), dict(eps=-1.0), dict(eps=float("nan"))]:
         assert fwd(**bad) == _lib.ERR_INVALID_ARG and "layer_norm" in _lib.last_error(), bad
     assert fwd(rows=0) == _lib.OK
     floats = lib.b200k_layer_norm_bwd_workspace(1000, 64)

@@ -117,7 +117,7 @@ __device__ __forceinline__ float warp_max_nonneg(float v) {   // floats >= 0 ord
 template <typename T>
 __device__ __forceinline__ void load4(const T* p, bool vec, int left, float (&f)[4]) {
   if (vec) {
-    unpack<T, 4>(*reinterpret_cast<const Pack<T, 4>*>(p), f);
+    load_vec<T, 4>(p, f);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = i < left ? to_f32<T>(p[i]) : 0.f;
@@ -126,7 +126,7 @@ __device__ __forceinline__ void load4(const T* p, bool vec, int left, float (&f)
 template <typename T>
 __device__ __forceinline__ void store4(T* p, bool vec, int left, const float (&f)[4]) {
   if (vec) {
-    *reinterpret_cast<Pack<T, 4>*>(p) = pack<T, 4>(f);
+    store_vec<T, 4>(p, f);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)

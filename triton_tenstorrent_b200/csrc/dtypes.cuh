@@ -4,6 +4,9 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <string.h>
+
+#include "ptx.cuh"
 
 namespace b200k {
 
@@ -26,23 +29,86 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
-// N consecutive elements moved as one access (N * sizeof(T) is 2, 4, 8, 16 or 32 bytes; 32 bytes are two 16-byte accesses).
-template <typename T, int N>
-struct alignas(sizeof(T) * N > 16 ? 16 : sizeof(T) * N) Pack {
-  T v[N];
-};
+// Two 16-bit elements of one word (the low one first) and back.
+template <typename T>
+__device__ __forceinline__ void unpack_word(uint32_t w, float& lo, float& hi);
+template <>
+__device__ __forceinline__ void unpack_word<__nv_bfloat16>(uint32_t w, float& lo, float& hi) {
+  lo = __uint_as_float(w << 16);
+  hi = __uint_as_float(w & 0xFFFF0000u);
+}
+template <>
+__device__ __forceinline__ void unpack_word<__half>(uint32_t w, float& lo, float& hi) {
+  __half2 h;
+  memcpy(&h, &w, 4);
+  const float2 f = __half22float2(h);
+  lo = f.x;
+  hi = f.y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack_word(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack_word<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
+template <>
+__device__ __forceinline__ uint32_t pack_word<__half>(float lo, float hi) { return pack_f16x2(lo, hi); }
 
+// N consecutive elements at p, moved in accesses of up to 16 bytes (p is aligned to min(16, N * sizeof(T)) bytes).  The accesses are spelled out as
+// words: a struct of 16-bit elements would be copied element by element.
 template <typename T, int N>
-__device__ __forceinline__ void unpack(const Pack<T, N>& p, float (&f)[N]) {
+__device__ __forceinline__ void load_vec(const T* p, float (&f)[N]) {
+  constexpr int BYTES = N * static_cast<int>(sizeof(T));
+  if constexpr (N == 1) {
+    f[0] = to_f32<T>(*p);
+  } else {
+    constexpr int WORDS = BYTES / 4;
+    uint32_t w[WORDS];
+    if constexpr (BYTES % 16 == 0) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) f[i] = to_f32<T>(p.v[i]);
+      for (int i = 0; i < BYTES / 16; ++i) {
+        const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+        w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+      }
+    } else if constexpr (BYTES == 8) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      w[0] = v.x; w[1] = v.y;
+    } else {
+      static_assert(BYTES == 4, "access size");
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) unpack_word<T>(w[i], f[2 * i], f[2 * i + 1]);
+    }
+  }
 }
 template <typename T, int N>
-__device__ __forceinline__ Pack<T, N> pack(const float (&f)[N]) {
-  Pack<T, N> p;
+__device__ __forceinline__ void store_vec(T* p, const float (&f)[N]) {
+  constexpr int BYTES = N * static_cast<int>(sizeof(T));
+  if constexpr (N == 1) {
+    *p = from_f32<T>(f[0]);
+  } else {
+    constexpr int WORDS = BYTES / 4;
+    uint32_t w[WORDS];
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) p.v[i] = from_f32<T>(f[i]);
-  return p;
+      for (int i = 0; i < N; ++i) w[i] = __float_as_uint(f[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) w[i] = pack_word<T>(f[2 * i], f[2 * i + 1]);
+    }
+    if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+      for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    } else if constexpr (BYTES == 8) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else {
+      static_assert(BYTES == 4, "access size");
+      *reinterpret_cast<uint32_t*>(p) = w[0];
+    }
+  }
 }
 
 }  // namespace b200k

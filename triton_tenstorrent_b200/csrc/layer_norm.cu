@@ -6,6 +6,9 @@
 // Everything between a load and a store is fp32; each output is rounded once.  The variance is summed over centred values
 // (never as E[x^2] - mu^2, which cancels when |mu| is large against the spread).
 // Bound: HBM.  Forward: x read, y written; backward: x and dy read, dx written; w, b and the row statistics are small.
+#include <initializer_list>
+#include <type_traits>
+
 #include "dtypes.cuh"
 #include "launch.h"
 #include "ptx.cuh"
@@ -108,24 +111,440 @@ __global__ void __launch_bounds__(256) ln_dw_loop_kernel(const T* __restrict__ d
   part[static_cast<int64_t>(parts + blockIdx.y) * cols + c] = sb;
 }
 
+// ---------------------------------------------------------------------------------------------
+// Rows of up to TPR * PER * VEC elements.  A CTA has one warp that fetches and TPR (or, with a warp per row, LN_GROUPS * 32) threads that work:
+// the fetching warp keeps a ring of rows in shared memory filled, whatever the others wait for.
+//
+// A row is worked on in steps that wait for one another (load, row sum, second sum, store), and registers for enough rows at a time do not exist
+// next to the backward's 2 N running sums; the ring keeps 60 to 190 KB per SM on their way instead.  (Fetching by one of the working warps,
+// between two row sums, was measured at 2800 GB/s for 16384 x 4096 bf16: the address arithmetic then sits on the path that every row waits for.)
+// Rows come as untiled bulk copies of the 16-byte blocks that they touch, so that any length and alignment arrives at full rate; only the
+// reads from shared memory and the stores go by VEC, the widest access that the operands' alignment allows.
+// ---------------------------------------------------------------------------------------------
+constexpr int LN_GROUPS = 8;          // rows at a time of a CTA whose warps take a row each
+constexpr int LN_MAX_STAGES = 8;
+template <int TPR>
+__host__ __device__ constexpr int ln_groups() { return TPR == 32 ? LN_GROUPS : 1; }
+template <int TPR>
+__host__ __device__ constexpr int ln_threads() { return TPR * ln_groups<TPR>() + 32; }
+// CTAs of one SM.  The backward writes a partial sum per CTA, so that it takes fewer.
+template <int TPR, bool BWD>
+__host__ __device__ constexpr int ln_per_sm() {
+  return TPR == 32 ? (BWD ? 2 : 3) : TPR == 128 ? (BWD ? 4 : 5) : TPR == 256 ? (BWD ? 2 : 3) : 1;
+}
+
+struct LnRing {
+  int stage_rows, stages, row_bytes;   // rows of a stage; row_bytes: a row's place in it, a multiple of 16
+};
+
+// One operand's rows, and where its memory ends (nothing outside [base, end) is read).
+struct LnSource {
+  const char* base;
+  int64_t pitch;        // bytes
+  const char* end;
+};
+// Where in its 16-byte block row r begins.
+__device__ __forceinline__ uint32_t ln_offset(const LnSource& s, int r) {
+  return (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(s.base)) + static_cast<uint32_t>(r) * static_cast<uint32_t>(s.pitch)) & 15u;
+}
+// The 16-byte blocks of the row at `a` that lie inside the operand: [*from, *from + bytes).
+__device__ __forceinline__ uint32_t ln_span(const LnSource& s, const char* a, int row_len, const char** from) {
+  uintptr_t lo = reinterpret_cast<uintptr_t>(a) & ~uintptr_t(15);
+  uintptr_t hi = (reinterpret_cast<uintptr_t>(a) + row_len + 15) & ~uintptr_t(15);
+  if (lo < reinterpret_cast<uintptr_t>(s.base)) lo += 16;
+  if (hi > reinterpret_cast<uintptr_t>(s.end)) hi -= 16;
+  *from = reinterpret_cast<const char*>(lo);
+  return hi > lo ? static_cast<uint32_t>(hi - lo) : 0u;
+}
+// What ln_span left out (less than 16 bytes at the operand's first and last row), element by element.
+template <typename T>
+__device__ __noinline__ void ln_patch(const char* a, int row_len, const char* from, uint32_t bytes, char* dst) {
+  const char* z = a + row_len;
+  const char* head = bytes == 0 || from < a ? a : from;                       // [a, head) and [tail, z) are missing
+  const char* tail = bytes == 0 || from + bytes < a ? a : from + bytes;
+  for (const char* q = a; q < head; q += sizeof(T)) *reinterpret_cast<T*>(dst + (q - a)) = *reinterpret_cast<const T*>(q);
+  for (const char* q = tail; q < z; q += sizeof(T)) *reinterpret_cast<T*>(dst + (q - a)) = *reinterpret_cast<const T*>(q);
+}
+
+// The fetching warp: blocks of stage_rows rows, a lane per row.
+template <typename T, int NSRC>
+__device__ __forceinline__ void ln_fetch_all(const LnSource (&src)[NSRC], const LnRing& ring, int rows, int row_len, char* ring_mem, uint64_t* full,
+                                             uint64_t* empty, const WaitCtx& ctx) {
+  const int lane = threadIdx.x & 31;
+  const int blocks = (rows + ring.stage_rows - 1) / ring.stage_rows;
+  const int stage_bytes = NSRC * ring.stage_rows * ring.row_bytes;
+  int stage = 0;
+  uint32_t phase = 0;
+  for (int blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
+    if (!mbar_wait(&empty[stage], phase ^ 1u, ctx, 73)) return;
+    const int r = blk * ring.stage_rows + lane;
+    const bool mine = lane < ring.stage_rows && r < rows;
+    char* dst[NSRC];
+    const char* from[NSRC];
+    uint32_t bytes[NSRC], total = 0;
+#pragma unroll
+    for (int i = 0; i < NSRC; ++i) {
+      bytes[i] = 0;
+      if (mine) {
+        const char* a = src[i].base + r * src[i].pitch;
+        bytes[i] = ln_span(src[i], a, row_len, &from[i]);
+        char* row = ring_mem + stage * stage_bytes + (lane * NSRC + i) * ring.row_bytes + (reinterpret_cast<uintptr_t>(a) & 15u);
+        dst[i] = row + (from[i] - a);
+        if (from[i] > a || from[i] + bytes[i] < a + row_len) ln_patch<T>(a, row_len, from[i], bytes[i], row);
+      }
+      total += bytes[i];
+    }
+    if (ring.stage_rows > 1) total = __reduce_add_sync(0xFFFFFFFFu, total);
+    __syncwarp();
+    if (lane == 0) mbar_expect_tx(&full[stage], total);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < NSRC; ++i)
+      if (mine && bytes[i] > 0) bulk_load(dst[i], from[i], bytes[i], &full[stage]);
+    if (++stage == ring.stages) { stage = 0; phase ^= 1u; }
+  }
+}
+
+// Sums over the TPR threads of a row; every thread gets them.  A CTA-wide sum takes a slot of `scratch` of its own per call in a row of calls (two
+// suffice: a barrier lies between the reads of one call and the writes of the call after the next).
+template <int WARPS>
+__device__ __forceinline__ float2 join_warps(const float2* scratch) {
+  float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < WARPS; i += 2) {
+    const float4 t = *reinterpret_cast<const float4*>(scratch + i);
+    v.x += t.x + t.z;
+    v.y += t.y + t.w;
+  }
+  return v;
+}
+template <int TPR>
+__device__ __forceinline__ float2 row_sum2(float2 v, float2 (*scratch)[32], int slot) {
+  const int lane = threadIdx.x & 31;
+  // the lower half of the warp goes on with x, the upper half with y
+  const bool upper = lane >= 16;
+  float t = (upper ? v.y : v.x) + __shfl_xor_sync(0xFFFFFFFFu, upper ? v.x : v.y, 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
+  if constexpr (TPR > 32) {
+    float* mine = &scratch[slot][threadIdx.x >> 5].x;
+    if ((lane & 15) == 0) mine[lane >> 4] = t;
+    named_bar_sync(1, TPR);
+    return join_warps<TPR / 32>(scratch[slot]);
+  } else {
+    return make_float2(__shfl_sync(0xFFFFFFFFu, t, 0), __shfl_sync(0xFFFFFFFFu, t, 16));
+  }
+}
+
+// A thread's elements of a row: PER accesses of VEC elements, TPR accesses apart; zeros behind the row's end.
+template <typename T, int VEC, int PER, int TPR>
+__device__ __forceinline__ void ln_read(const T* row, int lane, int cols, float (&f)[PER][VEC]) {
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int c = (lane + k * TPR) * VEC;
+    if (c < cols) {
+      load_vec<T, VEC>(row + c, f[k]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f[k][j] = 0.f;
+    }
+  }
+}
+// One access of w or b, or what stands for it where there is none.
+template <typename W, int VEC>
+__device__ __forceinline__ void ln_weight(const W* w, int c, int cols, float dflt, float (&f)[VEC]) {
+  if (w != nullptr && c < cols) {
+    load_vec<W, VEC>(w + c, f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) f[j] = dflt;
+  }
+}
+template <typename T, int VEC, int PER, int TPR>
+__device__ __forceinline__ void ln_write(T* row, int lane, int cols, const float (&f)[PER][VEC]) {
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int c = (lane + k * TPR) * VEC;
+    if (c < cols) store_vec<T, VEC>(row + c, f[k]);
+  }
+}
+
+// BATCH rows are worked on at a time (1 or 2): with one CTA on an SM a second row fills the waits of the first.
+template <typename T, typename W, int VEC, int PER, int TPR, int BATCH>
+__global__ void __launch_bounds__(ln_threads<TPR>(), ln_per_sm<TPR, false>())
+ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ b, T* __restrict__ y, float* __restrict__ mean,
+              float* __restrict__ rstd, int rows, int cols, int64_t ldy, float eps, const LnRing ring, uint32_t* status) {
+  constexpr int GROUPS = ln_groups<TPR>();
+  constexpr bool HOLD = PER * VEC <= 16;      // w and b stay in registers
+  extern __shared__ __align__(16) char ring_mem[];
+  __shared__ uint64_t full[LN_MAX_STAGES], empty[LN_MAX_STAGES];
+  __shared__ __align__(16) float2 scratch[2][32];
+  __shared__ uint32_t abort_flag;
+  if (threadIdx.x < LN_MAX_STAGES) {
+    mbar_init(&full[threadIdx.x], 1);
+    mbar_init(&empty[threadIdx.x], GROUPS);
+  }
+  if (threadIdx.x == 0) abort_flag = 0;
+  fence_mbar_init();
+  __syncthreads();
+  const WaitCtx ctx{&abort_flag, status};
+  const int group = threadIdx.x / TPR;
+  if (group == GROUPS) {
+    const LnSource src[1] = {sx};
+    ln_fetch_all<T, 1>(src, ring, rows, cols * static_cast<int>(sizeof(T)), ring_mem, full, empty, ctx);
+  } else {
+    const int lane = threadIdx.x % TPR;
+    float fw[HOLD ? PER : 1][VEC], fb[HOLD ? PER : 1][VEC];
+    if constexpr (HOLD) {
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        ln_weight<W, VEC>(w, (lane + k * TPR) * VEC, cols, 1.f, fw[k]);
+        ln_weight<W, VEC>(b, (lane + k * TPR) * VEC, cols, 0.f, fb[k]);
+      }
+    }
+    const float inv_n = 1.f / static_cast<float>(cols);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int top = blockIdx.x * ring.stage_rows; top < rows; top += gridDim.x * ring.stage_rows) {
+      // a wait that gives up is on record; the rows are then worked through all the same, so that every barrier below is met
+      mbar_wait(&full[stage], phase, ctx, 71);
+      for (int i = group * BATCH; i < ring.stage_rows; i += GROUPS * BATCH) {
+        const int r = top + i;
+        if (r >= rows) break;
+        const bool two = BATCH == 2 && r + 1 < rows;
+        float f[BATCH][PER][VEC];
+        float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int h = 0; h < BATCH; ++h) {
+          const int at = h == 1 && two ? 1 : 0;      // without a second row the first one is read again: its results are dropped
+          const char* row = ring_mem + (stage * ring.stage_rows + i + at) * ring.row_bytes + (VEC * sizeof(T) == 16 ? 0 : ln_offset(sx, r + at));
+          ln_read<T, VEC, PER, TPR>(reinterpret_cast<const T*>(row), lane, cols, f[h]);
+          float t = 0.f;
+#pragma unroll
+          for (int k = 0; k < PER; ++k)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) t += f[h][k][j];
+          (h == 0 ? s.x : s.y) = t;
+        }
+        s = row_sum2<TPR>(s, scratch, 0);
+        if (TPR > 32 && lane == 0) mbar_arrive(&empty[stage]);       // every thread holds its part of the stage's rows in registers
+        const float mu[2] = {s.x * inv_n, s.y * inv_n};
+        s = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int h = 0; h < BATCH; ++h) {
+          float t = 0.f;
+#pragma unroll
+          for (int k = 0; k < PER; ++k) {
+            if ((lane + k * TPR) * VEC < cols) {                      // what lies behind the row's end stays out of the sum
+#pragma unroll
+              for (int j = 0; j < VEC; ++j) {
+                f[h][k][j] -= mu[h];
+                t += f[h][k][j] * f[h][k][j];
+              }
+            }
+          }
+          (h == 0 ? s.x : s.y) = t;
+        }
+        s = row_sum2<TPR>(s, scratch, 1);
+        const float rs[2] = {rsqrtf(s.x * inv_n + eps), rsqrtf(s.y * inv_n + eps)};
+#pragma unroll
+        for (int h = 0; h < BATCH; ++h) {
+          if (h == 0 || two) {
+            T* out = y + (r + h) * ldy;
+#pragma unroll
+            for (int k = 0; k < PER; ++k) {
+              const int c = (lane + k * TPR) * VEC;
+              if constexpr (!HOLD) {
+                ln_weight<W, VEC>(w, c, cols, 1.f, fw[0]);
+                ln_weight<W, VEC>(b, c, cols, 0.f, fb[0]);
+              }
+#pragma unroll
+              for (int j = 0; j < VEC; ++j) f[h][k][j] = f[h][k][j] * rs[h] * fw[HOLD ? k : 0][j] + fb[HOLD ? k : 0][j];
+              if (c < cols) store_vec<T, VEC>(out + c, f[h][k]);
+            }
+            if (lane == 0) {
+              if (mean != nullptr) mean[r + h] = mu[h];
+              if (rstd != nullptr) rstd[r + h] = rs[h];
+            }
+          }
+        }
+      }
+      if (TPR == 32) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[stage]);
+      }
+      if (++stage == ring.stages) { stage = 0; phase ^= 1u; }
+    }
+  }
+  drain_after_abort(&abort_flag);
+}
+
+// Backward.  The columns' sums of dy h and dy stay in registers until the end: one partial sum per CTA (part[2][gridDim.x][cols], first dw's).
+template <typename T, typename W, int VEC, int PER, int TPR>
+__global__ void __launch_bounds__(ln_threads<TPR>(), ln_per_sm<TPR, true>())
+ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, const float* __restrict__ mean, const float* __restrict__ rstd,
+              T* __restrict__ dx, float* __restrict__ part, int rows, int cols, int64_t lddx, const LnRing ring, uint32_t* status) {
+  constexpr int GROUPS = ln_groups<TPR>();
+  constexpr bool HOLD = PER * VEC <= 16;       // w stays in registers, and u and h do between the row sum and dx
+  extern __shared__ __align__(16) char ring_mem[];
+  __shared__ uint64_t full[LN_MAX_STAGES], empty[LN_MAX_STAGES];
+  __shared__ __align__(16) float2 scratch[2][32];
+  __shared__ uint32_t abort_flag;
+  if (threadIdx.x < LN_MAX_STAGES) {
+    mbar_init(&full[threadIdx.x], 1);
+    mbar_init(&empty[threadIdx.x], TPR == 32 ? GROUPS : TPR / 32);
+  }
+  if (threadIdx.x == 0) abort_flag = 0;
+  fence_mbar_init();
+  __syncthreads();
+  const WaitCtx ctx{&abort_flag, status};
+  const int group = threadIdx.x / TPR;
+  if (group == GROUPS) {
+    const LnSource src[2] = {sg, sx};
+    ln_fetch_all<T, 2>(src, ring, rows, cols * static_cast<int>(sizeof(T)), ring_mem, full, empty, ctx);
+  } else {
+    const int lane = threadIdx.x % TPR;
+    float fw[HOLD ? PER : 1][VEC], aw[PER][VEC], ab[PER][VEC];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      if constexpr (HOLD) ln_weight<W, VEC>(w, (lane + k * TPR) * VEC, cols, 1.f, fw[k]);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) aw[k][j] = ab[k][j] = 0.f;
+    }
+    const float inv_n = 1.f / static_cast<float>(cols);
+    int stage = 0, slot = 0;
+    uint32_t phase = 0;
+    int r = blockIdx.x * ring.stage_rows + group;
+    float mu = r < rows ? mean[r] : 0.f, rs = r < rows ? rstd[r] : 0.f;
+    for (int top = blockIdx.x * ring.stage_rows; top < rows; top += gridDim.x * ring.stage_rows) {
+      mbar_wait(&full[stage], phase, ctx, 72);
+      for (int i = group; i < ring.stage_rows; i += GROUPS) {
+        r = top + i;
+        if (r >= rows) break;
+        const float m = mu, q = rs;
+        {                                                       // the next row's statistics
+          const int n = i + GROUPS < ring.stage_rows ? r + GROUPS : top + gridDim.x * ring.stage_rows + group;
+          if (n < rows) {
+            mu = mean[n];
+            rs = rstd[n];
+          }
+        }
+        const char* row = ring_mem + 2 * (stage * ring.stage_rows + i) * ring.row_bytes;
+        const T* row_g = reinterpret_cast<const T*>(row + (VEC * sizeof(T) == 16 ? 0 : ln_offset(sg, r)));
+        const T* row_x = reinterpret_cast<const T*>(row + ring.row_bytes + (VEC * sizeof(T) == 16 ? 0 : ln_offset(sx, r)));
+        // u = dy w and h of one access; zero dy behind the row's end, so that nothing there enters a sum
+        auto terms = [&](int k, float (&g)[VEC], float (&h)[VEC], auto&& use) {
+          const int c = (lane + k * TPR) * VEC;
+          if (c < cols) {
+            load_vec<T, VEC>(row_g + c, g);
+            load_vec<T, VEC>(row_x + c, h);
+          } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) g[j] = h[j] = 0.f;
+          }
+          if constexpr (!HOLD) ln_weight<W, VEC>(w, c, cols, 1.f, fw[0]);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            h[j] = (h[j] - m) * q;
+            use(j, g[j], h[j]);
+            g[j] *= fw[HOLD ? k : 0][j];
+          }
+        };
+        float g[HOLD ? PER : 1][VEC], h[HOLD ? PER : 1][VEC];
+        float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          constexpr int ONE = HOLD ? 1 : 0;
+          terms(k, g[ONE * k], h[ONE * k], [&](int j, float dyj, float hj) {
+            aw[k][j] += dyj * hj;
+            ab[k][j] += dyj;
+          });
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            s.x += g[ONE * k][j];
+            s.y += g[ONE * k][j] * h[ONE * k][j];
+          }
+        }
+        if (TPR > 32 && HOLD) {                                 // the stage's only row is in registers
+          __syncwarp();
+          if ((lane & 31) == 0) mbar_arrive(&empty[stage]);
+        }
+        s = row_sum2<TPR>(s, scratch, slot);
+        slot ^= 1;
+        if (dx != nullptr) {
+          const float c1 = s.x * inv_n, c2 = s.y * inv_n;
+          T* out = dx + r * lddx;
+#pragma unroll
+          for (int k = 0; k < PER; ++k) {
+            constexpr int ONE = HOLD ? 1 : 0;
+            const int c = (lane + k * TPR) * VEC;
+            if constexpr (!HOLD) terms(k, g[0], h[0], [](int, float, float) {});   // read once more instead of held
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) g[ONE * k][j] = q * (g[ONE * k][j] - c1 - h[ONE * k][j] * c2);
+            if (c < cols) store_vec<T, VEC>(out + c, g[ONE * k]);
+          }
+        }
+      }
+      if (TPR == 32 || !HOLD) {
+        __syncwarp();
+        if ((lane & 31) == 0) mbar_arrive(&empty[stage]);
+      }
+      if (++stage == ring.stages) { stage = 0; phase ^= 1u; }
+    }
+    if (part != nullptr) {
+      float* out_w = part + static_cast<int64_t>(blockIdx.x) * cols;
+      float* out_b = part + static_cast<int64_t>(gridDim.x + blockIdx.x) * cols;
+      if constexpr (GROUPS == 1) {
+        ln_write<float, VEC, PER, TPR>(out_w, lane, cols, aw);
+        ln_write<float, VEC, PER, TPR>(out_b, lane, cols, ab);
+      } else {
+        // the warps' sums one after the other, in a fixed order
+        __shared__ float2 sums[TPR * PER * VEC];
+        for (int g = 0; g < GROUPS; ++g) {
+          if (group == g) {
+#pragma unroll
+            for (int k = 0; k < PER; ++k)
+#pragma unroll
+              for (int j = 0; j < VEC; ++j) {
+                const int c = (lane + k * TPR) * VEC + j;
+                float2 v = g > 0 ? sums[c] : make_float2(0.f, 0.f);
+                v.x += aw[k][j];
+                v.y += ab[k][j];
+                sums[c] = v;
+              }
+          }
+          named_bar_sync(1, GROUPS * TPR);
+        }
+        for (int c = threadIdx.x; c < cols; c += GROUPS * TPR) {
+          out_w[c] = sums[c].x;
+          out_b[c] = sums[c].y;
+        }
+      }
+    }
+  }
+  drain_after_abort(&abort_flag);
+}
+
 // dw[c] and db[c]: the sums over the parts, in a fixed order.
 template <typename W>
-__global__ void __launch_bounds__(256) ln_dw_join_kernel(const float* __restrict__ part, W* __restrict__ dw, W* __restrict__ db, int parts,
-                                                         int64_t cols) {
-  __shared__ float sums[8][33];
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x & 31);
-  const int slice = threadIdx.x >> 5;
+__global__ void __launch_bounds__(1024) ln_dw_join_kernel(const float* __restrict__ part, W* __restrict__ dw, W* __restrict__ db, int parts,
+                                                          int64_t cols) {
+  __shared__ float sums[32][33];
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   const float* p = part + static_cast<int64_t>(blockIdx.y) * parts * cols;
   float s = 0.f;
-  if (c < cols)
-    for (int i = slice; i < parts; i += 8) s += p[static_cast<int64_t>(i) * cols + c];
-  sums[slice][threadIdx.x & 31] = s;
-  __syncthreads();
-  if (slice == 0 && c < cols) {
-    for (int i = 1; i < 8; ++i) s += sums[i][threadIdx.x];
-    W* out = blockIdx.y == 0 ? dw : db;
-    if (out != nullptr) out[c] = from_f32<W>(s);
+  if (c < cols) {
+#pragma unroll 4
+    for (int i = slice; i < parts; i += 32) s += p[static_cast<int64_t>(i) * cols + c];
   }
+  sums[slice][lane] = s;
+  __syncthreads();
+  // warp i now adds the 32 slices of column i
+  s = warp_sum(sums[lane][slice]);
+  W* out = blockIdx.y == 0 ? dw : db;
+  const int64_t mine = static_cast<int64_t>(blockIdx.x) * 32 + slice;
+  if (lane == 0 && mine < cols && out != nullptr) out[mine] = from_f32<W>(s);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -135,39 +554,167 @@ static int ln_parts(int64_t rows) { return static_cast<int>(rows < LN_MAX_PARTS 
 
 int64_t layer_norm_bwd_workspace(int64_t rows, int64_t cols) { return 2 * ln_parts(rows) * cols; }
 
+// Largest power of two (at most 16) that divides every byte address and pitch given.
+static int ln_alignment(std::initializer_list<uintptr_t> v) {
+  uintptr_t all = 16;
+  for (uintptr_t x : v) all |= x;
+  return static_cast<int>(all & (~all + 1));
+}
+static LnSource ln_source(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t size) {
+  const char* base = static_cast<const char*>(p);
+  return LnSource{base, ld * size, base + ((rows - 1) * ld + cols) * size};
+}
+// The ring of a CTA: a few KB per stage (a row or a batch of them for a CTA-wide row, some for every warp otherwise) and as many stages as the CTA's
+// share of the shared memory holds.  stages < 2: the rows are too long.
+static LnRing ln_ring(int64_t cols, int size, int align, int operands, int groups, int per_sm, int batch) {
+  LnRing r;
+  r.row_bytes = static_cast<int>((cols * size + 15) / 16 * 16) + (align == 16 ? 0 : 16);
+  r.stage_rows = groups == 1 ? batch : r.row_bytes * operands <= 256 ? 4 * groups : r.row_bytes * operands <= 1024 ? 2 * groups : groups;
+  const int64_t stages = static_cast<int64_t>(208 * 1024) / per_sm / (static_cast<int64_t>(r.stage_rows) * r.row_bytes * operands);
+  r.stages = static_cast<int>(stages > LN_MAX_STAGES ? LN_MAX_STAGES : stages);
+  return r;
+}
+
+template <typename T, typename W, int VEC, int PER, int TPR>
+static int ln_fwd_rows(const LayerNormArgs& a, int align, const DeviceInfo* dev, cudaStream_t stream, bool* done) {
+  constexpr int GROUPS = ln_groups<TPR>(), PER_SM = ln_per_sm<TPR, false>(), BATCH = TPR == 512 && PER * VEC <= 16 ? 2 : 1;
+  const LnRing ring = ln_ring(a.cols, sizeof(T), align, 1, GROUPS, PER_SM, BATCH);
+  if (ring.stages < 2) return B200K_OK;
+  auto kernel = ln_fwd_kernel<T, W, VEC, PER, TPR, BATCH>;
+  const int smem = ring.stages * ring.stage_rows * ring.row_bytes;
+  B200K_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 208 * 1024));
+  const int64_t most = (a.rows + ring.stage_rows - 1) / ring.stage_rows, grid = static_cast<int64_t>(dev->sm_count) * PER_SM;
+  kernel<<<static_cast<unsigned>(most < grid ? most : grid), ln_threads<TPR>(), smem, stream>>>(
+      ln_source(a.x, a.rows, a.cols, a.ldx, sizeof(T)), static_cast<const W*>(a.w), static_cast<const W*>(a.b), static_cast<T*>(a.y), a.mean, a.rstd,
+      static_cast<int>(a.rows), static_cast<int>(a.cols), a.ldy, a.eps, ring, dev->status_word);
+  count_launch();
+  B200K_CHECK_LAUNCH("ln_fwd_kernel");
+  *done = true;
+  return B200K_OK;
+}
+
+template <typename T, typename W, int VEC, int PER, int TPR>
+static int ln_bwd_rows(const LayerNormArgs& a, int align, const DeviceInfo* dev, float* part, int* parts, cudaStream_t stream, bool* done) {
+  constexpr int GROUPS = ln_groups<TPR>(), PER_SM = ln_per_sm<TPR, true>();
+  const LnRing ring = ln_ring(a.cols, sizeof(T), align, 2, GROUPS, PER_SM, 1);
+  if (ring.stages < 2) return B200K_OK;
+  auto kernel = ln_bwd_kernel<T, W, VEC, PER, TPR>;
+  const int smem = 2 * ring.stages * ring.stage_rows * ring.row_bytes;
+  B200K_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 208 * 1024));
+  int64_t grid = (a.rows + ring.stage_rows - 1) / ring.stage_rows;
+  if (grid > static_cast<int64_t>(dev->sm_count) * PER_SM) grid = static_cast<int64_t>(dev->sm_count) * PER_SM;
+  if (grid > LN_MAX_PARTS) grid = LN_MAX_PARTS;
+  *parts = static_cast<int>(grid);
+  kernel<<<static_cast<unsigned>(grid), ln_threads<TPR>(), smem, stream>>>(
+      ln_source(a.dy, a.rows, a.cols, a.lddy, sizeof(T)), ln_source(a.x, a.rows, a.cols, a.ldx, sizeof(T)), static_cast<const W*>(a.w), a.mean,
+      a.rstd, static_cast<T*>(a.dx), part, static_cast<int>(a.rows), static_cast<int>(a.cols), a.lddx, ring, dev->status_word);
+  count_launch();
+  B200K_CHECK_LAUNCH("ln_bwd_kernel");
+  *done = true;
+  return B200K_OK;
+}
+
+// Calls f with the kernel shape for rows of `cols` elements of `size` bytes whose operands share `align`: (VEC, PER, TPR) as integral constants.
+// 16 elements a thread or less, 32 beyond 8192; false beyond 16384 elements.
+template <int N>
+using Int = std::integral_constant<int, N>;
+template <int SIZE, typename F>
+static bool ln_shape(int64_t cols, int align, F&& f) {
+  constexpr int V = 16 / SIZE;
+  if (align == 16) {
+    const int64_t u = cols / V;
+    if (u <= 32) f(Int<V>(), Int<1>(), Int<32>());
+    else if (u <= 64) f(Int<V>(), Int<2>(), Int<32>());
+    else if (u <= 2 * 1024 / V) f(Int<V>(), Int<16 / V>(), Int<128>());
+    else if (u <= 4 * 1024 / V) f(Int<V>(), Int<16 / V>(), Int<256>());
+    else if (u <= 8 * 1024 / V) f(Int<V>(), Int<16 / V>(), Int<512>());
+    else if (u <= 16 * 1024 / V) f(Int<V>(), Int<32 / V>(), Int<512>());
+    else return false;
+    return true;
+  }
+  if constexpr (SIZE == 2) if (align >= 4) {
+    if (cols <= 256) f(Int<2>(), Int<4>(), Int<32>());
+    else if (cols <= 512) f(Int<2>(), Int<8>(), Int<32>());
+    else if (cols <= 2048) f(Int<2>(), Int<8>(), Int<128>());
+    else if (cols <= 4096) f(Int<2>(), Int<8>(), Int<256>());
+    else if (cols <= 8192) f(Int<2>(), Int<8>(), Int<512>());
+    else if (cols <= 16384) f(Int<2>(), Int<16>(), Int<512>());
+    else return false;
+    return true;
+  }
+  if (cols <= 256) f(Int<1>(), Int<8>(), Int<32>());
+  else if (cols <= 512) f(Int<1>(), Int<16>(), Int<32>());
+  else if (cols <= 2048) f(Int<1>(), Int<16>(), Int<128>());
+  else if (cols <= 4096) f(Int<1>(), Int<16>(), Int<256>());
+  else if (cols <= 8192) f(Int<1>(), Int<16>(), Int<512>());
+  else if (cols <= 16384) f(Int<1>(), Int<32>(), Int<512>());
+  else return false;
+  return true;
+}
+
+// The alignment of x's accesses that the weights allow too: VEC elements of x go with VEC elements of w.
 template <typename T, typename W>
-static int ln_fwd(const LayerNormArgs& a, cudaStream_t stream) {
+static int ln_common_alignment(int rows_align, const void* w, const void* b) {
+  const int weights = ln_alignment({reinterpret_cast<uintptr_t>(w), reinterpret_cast<uintptr_t>(b)});
+  const int allowed = weights == 16 ? 16 : weights * static_cast<int>(sizeof(T)) / static_cast<int>(sizeof(W));
+  return rows_align < allowed ? rows_align : allowed;
+}
+
+template <typename T, typename W>
+static int ln_fwd(const LayerNormArgs& a, const DeviceInfo* dev, cudaStream_t stream) {
+  constexpr uintptr_t S = sizeof(T);
+  const int align = ln_common_alignment<T, W>(ln_alignment({reinterpret_cast<uintptr_t>(a.x), reinterpret_cast<uintptr_t>(a.y), a.cols * S, a.ldx * S, a.ldy * S}), a.w, a.b);
+  int rc = B200K_OK;
+  bool done = false;
+  if (a.rows < (int64_t(1) << 30)) ln_shape<S>(a.cols, align, [&](auto vec, auto per, auto tpr) { rc = ln_fwd_rows<T, W, vec(), per(), tpr()>(a, align, dev, stream, &done); });
+  if (rc != B200K_OK || done) return rc;
   const unsigned grid = static_cast<unsigned>(a.rows < (1 << 30) ? a.rows : (1 << 30));
-  const int threads = a.cols >= 2048 ? 512 : 128;
-  ln_fwd_loop_kernel<T, W><<<grid, threads, 0, stream>>>(static_cast<const T*>(a.x), static_cast<const W*>(a.w), static_cast<const W*>(a.b),
-                                                         static_cast<T*>(a.y), a.mean, a.rstd, a.rows, a.cols, a.ldx, a.ldy, a.eps);
+  ln_fwd_loop_kernel<T, W><<<grid, 512, 0, stream>>>(static_cast<const T*>(a.x), static_cast<const W*>(a.w), static_cast<const W*>(a.b),
+                                                     static_cast<T*>(a.y), a.mean, a.rstd, a.rows, a.cols, a.ldx, a.ldy, a.eps);
   count_launch();
   B200K_CHECK_LAUNCH("ln_fwd_loop_kernel");
   return B200K_OK;
 }
 
 template <typename T, typename W>
-static int ln_bwd(const LayerNormArgs& a, cudaStream_t stream) {
+static int ln_bwd_main(const LayerNormArgs& a, const DeviceInfo* dev, float* part, int* parts, cudaStream_t stream) {
+  constexpr uintptr_t S = sizeof(T);
+  const int align = ln_common_alignment<T, W>(ln_alignment({reinterpret_cast<uintptr_t>(a.x), reinterpret_cast<uintptr_t>(a.dy), reinterpret_cast<uintptr_t>(a.dx),
+                                                            a.cols * S, a.ldx * S, a.lddy * S, a.dx == nullptr ? 0 : a.lddx * S}), a.w, nullptr);
+  int rc = B200K_OK;
+  bool done = false;
+  if (a.rows < (int64_t(1) << 30)) ln_shape<S>(a.cols, align, [&](auto vec, auto per, auto tpr) { rc = ln_bwd_rows<T, W, vec(), per(), tpr()>(a, align, dev, part, parts, stream, &done); });
+  if (rc != B200K_OK || done) return rc;
   const T* dy = static_cast<const T*>(a.dy);
   const T* x = static_cast<const T*>(a.x);
-  if (a.dx != nullptr && a.rows > 0) {
+  if (a.dx != nullptr) {
     const unsigned grid = static_cast<unsigned>(a.rows < (1 << 30) ? a.rows : (1 << 30));
-    const int threads = a.cols >= 2048 ? 512 : 128;
-    ln_dx_loop_kernel<T, W><<<grid, threads, 0, stream>>>(dy, x, static_cast<const W*>(a.w), a.mean, a.rstd, static_cast<T*>(a.dx), a.rows,
-                                                          a.cols, a.lddy, a.ldx, a.lddx);
+    ln_dx_loop_kernel<T, W><<<grid, 512, 0, stream>>>(dy, x, static_cast<const W*>(a.w), a.mean, a.rstd, static_cast<T*>(a.dx), a.rows, a.cols,
+                                                      a.lddy, a.ldx, a.lddx);
     count_launch();
     B200K_CHECK_LAUNCH("ln_dx_loop_kernel");
   }
-  if (a.dw != nullptr || a.db != nullptr) {
-    const int parts = ln_parts(a.rows);
-    if (parts > 0) {
-      ln_dw_loop_kernel<T><<<dim3(static_cast<unsigned>((a.cols + 255) / 256), parts), 256, 0, stream>>>(dy, x, a.mean, a.rstd, a.workspace,
-                                                                                                       a.rows, a.cols, a.lddy, a.ldx);
-      count_launch();
-      B200K_CHECK_LAUNCH("ln_dw_loop_kernel");
-    }
-    ln_dw_join_kernel<W><<<dim3(static_cast<unsigned>((a.cols + 31) / 32), 2), 256, 0, stream>>>(a.workspace, static_cast<W*>(a.dw),
-                                                                                                static_cast<W*>(a.db), parts, a.cols);
+  if (part != nullptr) {
+    *parts = ln_parts(a.rows);
+    ln_dw_loop_kernel<T><<<dim3(static_cast<unsigned>((a.cols + 255) / 256), *parts), 256, 0, stream>>>(dy, x, a.mean, a.rstd, part, a.rows, a.cols,
+                                                                                                      a.lddy, a.ldx);
+    count_launch();
+    B200K_CHECK_LAUNCH("ln_dw_loop_kernel");
+  }
+  return B200K_OK;
+}
+
+template <typename T, typename W>
+static int ln_bwd(const LayerNormArgs& a, const DeviceInfo* dev, cudaStream_t stream) {
+  const bool sums = a.dw != nullptr || a.db != nullptr;
+  int parts = 0;
+  if (a.rows > 0 && (sums || a.dx != nullptr)) {
+    const int rc = ln_bwd_main<T, W>(a, dev, sums ? a.workspace : nullptr, &parts, stream);
+    if (rc != B200K_OK) return rc;
+  }
+  if (sums) {
+    ln_dw_join_kernel<W><<<dim3(static_cast<unsigned>((a.cols + 31) / 32), 2), 1024, 0, stream>>>(a.workspace, static_cast<W*>(a.dw),
+                                                                                                 static_cast<W*>(a.db), parts, a.cols);
     count_launch();
     B200K_CHECK_LAUNCH("ln_dw_join_kernel");
   }
@@ -190,6 +737,11 @@ static int ln_check(const LayerNormArgs& a, const char* what) {
     return set_error(B200K_ERR_INVALID_ARG, "%s: weight and bias have the type of x or fp32 (got %d for x of type %d)", what, a.wdtype, a.dtype);
   if (a.rows < 0 || a.cols < 1 || a.cols > (int64_t(1) << 31) - 512)
     return set_error(B200K_ERR_INVALID_ARG, "%s: rows >= 0 and 1 <= cols < 2^31 - 512 expected (got %lld x %lld)", what, (long long)a.rows, (long long)a.cols);
+  const uintptr_t size = a.dtype == B200K_DTYPE_F32 ? 4 : 2, wsize = a.wdtype == B200K_DTYPE_F32 ? 4 : 2;
+  if ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.dy) | reinterpret_cast<uintptr_t>(a.dx)) & (size - 1) ||
+      (reinterpret_cast<uintptr_t>(a.w) | reinterpret_cast<uintptr_t>(a.b) | reinterpret_cast<uintptr_t>(a.dw) | reinterpret_cast<uintptr_t>(a.db)) & (wsize - 1) ||
+      (reinterpret_cast<uintptr_t>(a.mean) | reinterpret_cast<uintptr_t>(a.rstd)) & 3u || reinterpret_cast<uintptr_t>(a.workspace) & 15u)
+    return set_error(B200K_ERR_INVALID_ARG, "%s: a pointer is not aligned to its element size, or the workspace not to 16 bytes", what);
   if (a.rows > 0 && a.cols > (int64_t(1) << 62) / a.rows) return set_error(B200K_ERR_INVALID_ARG, "%s: too many elements", what);
   return B200K_OK;
 }
@@ -203,7 +755,7 @@ int layer_norm_fwd(const LayerNormArgs& a, cudaStream_t stream) {
   if (a.ldx < 0 || a.ldy < a.cols) return set_error(B200K_ERR_INVALID_ARG, "layer_norm: bad row stride");
   const DeviceInfo* dev = current_device_info();
   if (dev == nullptr) return B200K_ERR_NO_DEVICE;
-  return ln_dispatch(a, [&](auto t, auto w) { return ln_fwd<decltype(t), decltype(w)>(a, stream); });
+  return ln_dispatch(a, [&](auto t, auto w) { return ln_fwd<decltype(t), decltype(w)>(a, dev, stream); });
 }
 
 int layer_norm_bwd(const LayerNormArgs& a, cudaStream_t stream) {
@@ -220,7 +772,7 @@ int layer_norm_bwd(const LayerNormArgs& a, cudaStream_t stream) {
   }
   const DeviceInfo* dev = current_device_info();
   if (dev == nullptr) return B200K_ERR_NO_DEVICE;
-  return ln_dispatch(a, [&](auto t, auto w) { return ln_bwd<decltype(t), decltype(w)>(a, stream); });
+  return ln_dispatch(a, [&](auto t, auto w) { return ln_bwd<decltype(t), decltype(w)>(a, dev, stream); });
 }
 
 }  // namespace b200k
