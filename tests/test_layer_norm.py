@@ -274,3 +274,36 @@ def test_entry_point_refusals():
     for bad in [dict(dy=None), dict(work=None), dict(floats=floats - 1), dict(lddx=63)]:
         assert bwd(**bad) == _lib.ERR_INVALID_ARG, bad
     assert "workspace" in _lib.last_error() or "stride" in _lib.last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols,pad", [(1, 7), (40, 8), (200, 24), (257, 3), (384, 16), (513, 1), (520, 8), (1000, 24), (1026, 2), (2051, 5), (2056, 8), (4104, 8), (5000, 8), (8200, 56),
+                                      (9001, 2), (16384, 8)])
+def test_nothing_outside_the_rows_is_written(cols, pad, dtype):
+    rows, ld = 5, cols + pad
+    x, w, b, dy = make(rows, cols, dtype, dtype)
+    lib, code = _lib.load(), ops._DTYPES[dtype]
+    y, dx = (torch.full((rows + 2, ld), 777.0, device="cuda", dtype=dtype) for _ in range(2))
+    stats = torch.full((2, rows + 8), 777.0, device="cuda")
+    grads = torch.full((2, cols + 32), 777.0, device="cuda", dtype=dtype)
+    floats = lib.b200k_layer_norm_bwd_workspace(rows, cols)
+    work = torch.full((floats + 64,), 777.0, device="cuda")
+    size = x.element_size()
+    stream = ops._stream()
+    _lib.check(lib.b200k_layer_norm_fwd(x.data_ptr(), w.data_ptr(), b.data_ptr(), y.data_ptr() + ld * size, stats.data_ptr(), stats[1].data_ptr(), rows,
+                                        cols, cols, ld, code, code, 1e-5, stream))
+    _lib.check(lib.b200k_layer_norm_bwd(dy.data_ptr(), x.data_ptr(), w.data_ptr(), stats.data_ptr(), stats[1].data_ptr(), dx.data_ptr() + ld * size,
+                                        grads.data_ptr(), grads[1].data_ptr(), work.data_ptr(), floats, rows, cols, cols, cols, ld, code, code, stream))
+    want = tt.layer_norm_with_stats(x, w, b)
+    want_grads = tt.layer_norm_backward(dy, x, w, *want[1:])
+    half_of.update(y=half(dtype), dx=half(dtype), dw=half(dtype), db=half(dtype), mean=U, rstd=U)
+    ref = reference(x, w, b, dy, 1e-5)
+    for buf, name in ((y, "y"), (dx, "dx")):
+        check(name, buf[1:rows + 1, :cols], ref[name])
+        assert bool((buf[0] == 777).all()) and bool((buf[rows + 1] == 777).all()) and bool((buf[1:rows + 1, cols:] == 777).all())
+    for buf, names, n in ((stats, ("mean", "rstd"), rows), (grads, ("dw", "db"), cols)):
+        for i, name in enumerate(names):
+            check(name, buf[i, :n], ref[name])
+            assert bool((buf[i, n:] == 777).all())
+    assert bool((work[floats:] == 777).all()) and want_grads[0].shape == x.shape

@@ -111,4 +111,58 @@ __device__ __forceinline__ void store_vec(T* p, const float (&f)[N]) {
   }
 }
 
+// VEC consecutive elements as N numbers of type V: pairs of fp32 (two of them go through one packed instruction, which halves the issue slots of
+// kernels with a dozen operations per 16-bit element), or one fp32 when VEC is 1.
+template <int VEC>
+struct Lanes {
+  using V = uint64_t;
+  static constexpr int N = VEC / 2;
+};
+template <>
+struct Lanes<1> {
+  using V = float;
+  static constexpr int N = 1;
+};
+__device__ __forceinline__ float vadd(float a, float b) { return a + b; }
+__device__ __forceinline__ float vmul(float a, float b) { return a * b; }
+__device__ __forceinline__ float vfma(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ uint64_t vadd(uint64_t a, uint64_t b) { return add_f32x2(a, b); }
+__device__ __forceinline__ uint64_t vmul(uint64_t a, uint64_t b) { return mul_f32x2(a, b); }
+__device__ __forceinline__ uint64_t vfma(uint64_t a, uint64_t b, uint64_t c) { return fma_f32x2(a, b, c); }
+__device__ __forceinline__ float vsum(float a) { return a; }
+__device__ __forceinline__ float vsum(uint64_t a) {
+  float lo, hi;
+  unpack_f32x2(a, lo, hi);
+  return lo + hi;
+}
+template <typename V>
+__device__ __forceinline__ V vsplat(float a);
+template <>
+__device__ __forceinline__ float vsplat<float>(float a) { return a; }
+template <>
+__device__ __forceinline__ uint64_t vsplat<uint64_t>(float a) { return pack_f32x2(a, a); }
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_lanes(const T* p, typename Lanes<VEC>::V (&v)[Lanes<VEC>::N]) {
+  float f[VEC];
+  load_vec<T, VEC>(p, f);
+  if constexpr (VEC == 1) {
+    v[0] = f[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) v[i] = pack_f32x2(f[2 * i], f[2 * i + 1]);
+  }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_lanes(T* p, const typename Lanes<VEC>::V (&v)[Lanes<VEC>::N]) {
+  float f[VEC];
+  if constexpr (VEC == 1) {
+    f[0] = v[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) unpack_f32x2(v[i], f[2 * i], f[2 * i + 1]);
+  }
+  store_vec<T, VEC>(p, f);
+}
+
 }  // namespace b200k

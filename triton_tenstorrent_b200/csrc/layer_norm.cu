@@ -133,6 +133,11 @@ __host__ __device__ constexpr int ln_per_sm() {
   return TPR == 32 ? (BWD ? 2 : 3) : TPR == 128 ? (BWD ? 4 : 5) : TPR == 256 ? (BWD ? 2 : 3) : 1;
 }
 
+// Whether access k of a thread can lie behind the row's end.  A CTA-wide row fills more than half of its shape (ln_shape), so the first half of the
+// accesses cannot.
+template <int TPR, int PER>
+__device__ __forceinline__ bool ln_inside(int k, int c, int cols) { return (TPR > 32 && k < PER / 2) || c < cols; }
+
 struct LnRing {
   int stage_rows, stages, row_bytes;   // rows of a stage; row_bytes: a row's place in it, a multiple of 16
 };
@@ -236,36 +241,14 @@ __device__ __forceinline__ float2 row_sum2(float2 v, float2 (*scratch)[32], int 
   }
 }
 
-// A thread's elements of a row: PER accesses of VEC elements, TPR accesses apart; zeros behind the row's end.
-template <typename T, int VEC, int PER, int TPR>
-__device__ __forceinline__ void ln_read(const T* row, int lane, int cols, float (&f)[PER][VEC]) {
-#pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const int c = (lane + k * TPR) * VEC;
-    if (c < cols) {
-      load_vec<T, VEC>(row + c, f[k]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) f[k][j] = 0.f;
-    }
-  }
-}
 // One access of w or b, or what stands for it where there is none.
 template <typename W, int VEC>
-__device__ __forceinline__ void ln_weight(const W* w, int c, int cols, float dflt, float (&f)[VEC]) {
+__device__ __forceinline__ void ln_weight(const W* w, int c, int cols, float dflt, typename Lanes<VEC>::V (&f)[Lanes<VEC>::N]) {
   if (w != nullptr && c < cols) {
-    load_vec<W, VEC>(w + c, f);
+    load_lanes<W, VEC>(w + c, f);
   } else {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) f[j] = dflt;
-  }
-}
-template <typename T, int VEC, int PER, int TPR>
-__device__ __forceinline__ void ln_write(T* row, int lane, int cols, const float (&f)[PER][VEC]) {
-#pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const int c = (lane + k * TPR) * VEC;
-    if (c < cols) store_vec<T, VEC>(row + c, f[k]);
+    for (int j = 0; j < Lanes<VEC>::N; ++j) f[j] = vsplat<typename Lanes<VEC>::V>(dflt);
   }
 }
 
@@ -276,6 +259,8 @@ ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ 
               float* __restrict__ rstd, int rows, int cols, int64_t ldy, float eps, const LnRing ring, uint32_t* status) {
   constexpr int GROUPS = ln_groups<TPR>();
   constexpr bool HOLD = PER * VEC <= 16;      // w and b stay in registers
+  using V = typename Lanes<VEC>::V;
+  constexpr int N = Lanes<VEC>::N;
   extern __shared__ __align__(16) char ring_mem[];
   __shared__ uint64_t full[LN_MAX_STAGES], empty[LN_MAX_STAGES];
   __shared__ __align__(16) float2 scratch[2][32];
@@ -294,7 +279,7 @@ ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ 
     ln_fetch_all<T, 1>(src, ring, rows, cols * static_cast<int>(sizeof(T)), ring_mem, full, empty, ctx);
   } else {
     const int lane = threadIdx.x % TPR;
-    float fw[HOLD ? PER : 1][VEC], fb[HOLD ? PER : 1][VEC];
+    V fw[HOLD ? PER : 1][N], fb[HOLD ? PER : 1][N];
     if constexpr (HOLD) {
 #pragma unroll
       for (int k = 0; k < PER; ++k) {
@@ -303,28 +288,34 @@ ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ 
       }
     }
     const float inv_n = 1.f / static_cast<float>(cols);
-    int stage = 0;
+    const int stage_rows = TPR == 32 ? ring.stage_rows : BATCH;
+    const char* const my_ring = ring_mem + lane * VEC * static_cast<int>(sizeof(T));
+    T* const my_y = y + lane * VEC;
+    int stage = 0, stage_at = 0;
     uint32_t phase = 0;
-    for (int top = blockIdx.x * ring.stage_rows; top < rows; top += gridDim.x * ring.stage_rows) {
+    for (int top = blockIdx.x * stage_rows; top < rows; top += gridDim.x * stage_rows) {
       // a wait that gives up is on record; the rows are then worked through all the same, so that every barrier below is met
       mbar_wait(&full[stage], phase, ctx, 71);
-      for (int i = group * BATCH; i < ring.stage_rows; i += GROUPS * BATCH) {
+      for (int i = group * BATCH; i < stage_rows; i += GROUPS * BATCH) {
         const int r = top + i;
-        if (r >= rows) break;
+        if (TPR == 32 && r >= rows) break;
         const bool two = BATCH == 2 && r + 1 < rows;
-        float f[BATCH][PER][VEC];
+        V f[BATCH][PER][N];
         float2 s = make_float2(0.f, 0.f);
 #pragma unroll
         for (int h = 0; h < BATCH; ++h) {
           const int at = h == 1 && two ? 1 : 0;      // without a second row the first one is read again: its results are dropped
-          const char* row = ring_mem + (stage * ring.stage_rows + i + at) * ring.row_bytes + (VEC * sizeof(T) == 16 ? 0 : ln_offset(sx, r + at));
-          ln_read<T, VEC, PER, TPR>(reinterpret_cast<const T*>(row), lane, cols, f[h]);
-          float t = 0.f;
+          const char* row = my_ring + stage_at + (i + at) * ring.row_bytes + (VEC * sizeof(T) == 16 ? 0 : ln_offset(sx, r + at));
+          V t = vsplat<V>(0.f);
 #pragma unroll
-          for (int k = 0; k < PER; ++k)
+          for (int k = 0; k < PER; ++k) {
+            if (ln_inside<TPR, PER>(k, (lane + k * TPR) * VEC, cols)) {
+              load_lanes<T, VEC>(reinterpret_cast<const T*>(row) + k * TPR * VEC, f[h][k]);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) t += f[h][k][j];
-          (h == 0 ? s.x : s.y) = t;
+              for (int j = 0; j < N; ++j) t = vadd(t, f[h][k][j]);
+            }
+          }
+          (h == 0 ? s.x : s.y) = vsum(t);
         }
         s = row_sum2<TPR>(s, scratch, 0);
         if (TPR > 32 && lane == 0) mbar_arrive(&empty[stage]);       // every thread holds its part of the stage's rows in registers
@@ -332,35 +323,38 @@ ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ 
         s = make_float2(0.f, 0.f);
 #pragma unroll
         for (int h = 0; h < BATCH; ++h) {
-          float t = 0.f;
+          V t = vsplat<V>(0.f);
+          const V minus = vsplat<V>(-mu[h]);
 #pragma unroll
           for (int k = 0; k < PER; ++k) {
-            if ((lane + k * TPR) * VEC < cols) {                      // what lies behind the row's end stays out of the sum
+            if (ln_inside<TPR, PER>(k, (lane + k * TPR) * VEC, cols)) {
 #pragma unroll
-              for (int j = 0; j < VEC; ++j) {
-                f[h][k][j] -= mu[h];
-                t += f[h][k][j] * f[h][k][j];
+              for (int j = 0; j < N; ++j) {
+                f[h][k][j] = vadd(f[h][k][j], minus);
+                t = vfma(f[h][k][j], f[h][k][j], t);
               }
             }
           }
-          (h == 0 ? s.x : s.y) = t;
+          (h == 0 ? s.x : s.y) = vsum(t);
         }
         s = row_sum2<TPR>(s, scratch, 1);
         const float rs[2] = {rsqrtf(s.x * inv_n + eps), rsqrtf(s.y * inv_n + eps)};
 #pragma unroll
         for (int h = 0; h < BATCH; ++h) {
           if (h == 0 || two) {
-            T* out = y + (r + h) * ldy;
+            T* out = my_y + (r + h) * ldy;
+            const V scale = vsplat<V>(rs[h]);
 #pragma unroll
             for (int k = 0; k < PER; ++k) {
               const int c = (lane + k * TPR) * VEC;
+              if (!ln_inside<TPR, PER>(k, c, cols)) continue;
               if constexpr (!HOLD) {
                 ln_weight<W, VEC>(w, c, cols, 1.f, fw[0]);
                 ln_weight<W, VEC>(b, c, cols, 0.f, fb[0]);
               }
 #pragma unroll
-              for (int j = 0; j < VEC; ++j) f[h][k][j] = f[h][k][j] * rs[h] * fw[HOLD ? k : 0][j] + fb[HOLD ? k : 0][j];
-              if (c < cols) store_vec<T, VEC>(out + c, f[h][k]);
+              for (int j = 0; j < N; ++j) f[h][k][j] = vfma(vmul(f[h][k][j], scale), fw[HOLD ? k : 0][j], fb[HOLD ? k : 0][j]);
+              store_lanes<T, VEC>(out + k * TPR * VEC, f[h][k]);
             }
             if (lane == 0) {
               if (mean != nullptr) mean[r + h] = mu[h];
@@ -373,7 +367,8 @@ ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ 
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[stage]);
       }
-      if (++stage == ring.stages) { stage = 0; phase ^= 1u; }
+      stage_at += stage_rows * ring.row_bytes;
+      if (++stage == ring.stages) { stage = stage_at = 0; phase ^= 1u; }
     }
   }
   drain_after_abort(&abort_flag);
@@ -386,6 +381,8 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
               T* __restrict__ dx, float* __restrict__ part, int rows, int cols, int64_t lddx, const LnRing ring, uint32_t* status) {
   constexpr int GROUPS = ln_groups<TPR>();
   constexpr bool HOLD = PER * VEC <= 16;       // w stays in registers, and u and h do between the row sum and dx
+  using V = typename Lanes<VEC>::V;
+  constexpr int N = Lanes<VEC>::N;
   extern __shared__ __align__(16) char ring_mem[];
   __shared__ uint64_t full[LN_MAX_STAGES], empty[LN_MAX_STAGES];
   __shared__ __align__(16) float2 scratch[2][32];
@@ -404,67 +401,68 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
     ln_fetch_all<T, 2>(src, ring, rows, cols * static_cast<int>(sizeof(T)), ring_mem, full, empty, ctx);
   } else {
     const int lane = threadIdx.x % TPR;
-    float fw[HOLD ? PER : 1][VEC], aw[PER][VEC], ab[PER][VEC];
+    V fw[HOLD ? PER : 1][N], aw[PER][N], ab[PER][N];
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
       if constexpr (HOLD) ln_weight<W, VEC>(w, (lane + k * TPR) * VEC, cols, 1.f, fw[k]);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) aw[k][j] = ab[k][j] = 0.f;
+      for (int j = 0; j < N; ++j) aw[k][j] = ab[k][j] = vsplat<V>(0.f);
     }
     const float inv_n = 1.f / static_cast<float>(cols);
-    int stage = 0, slot = 0;
+    const int stage_rows = TPR == 32 ? ring.stage_rows : 1;
+    const char* const my_ring = ring_mem + lane * VEC * static_cast<int>(sizeof(T));
+    T* const my_dx = dx + lane * VEC;
+    int stage = 0, stage_at = 0, slot = 0;
     uint32_t phase = 0;
-    int r = blockIdx.x * ring.stage_rows + group;
+    int r = blockIdx.x * stage_rows + group;
     float mu = r < rows ? mean[r] : 0.f, rs = r < rows ? rstd[r] : 0.f;
-    for (int top = blockIdx.x * ring.stage_rows; top < rows; top += gridDim.x * ring.stage_rows) {
+    for (int top = blockIdx.x * stage_rows; top < rows; top += gridDim.x * stage_rows) {
       mbar_wait(&full[stage], phase, ctx, 72);
-      for (int i = group; i < ring.stage_rows; i += GROUPS) {
+      for (int i = group; i < stage_rows; i += GROUPS) {
         r = top + i;
-        if (r >= rows) break;
-        const float m = mu, q = rs;
+        if (TPR == 32 && r >= rows) break;
+        const V minus = vsplat<V>(-mu), q = vsplat<V>(rs);
         {                                                       // the next row's statistics
-          const int n = i + GROUPS < ring.stage_rows ? r + GROUPS : top + gridDim.x * ring.stage_rows + group;
+          const int n = i + GROUPS < stage_rows ? r + GROUPS : top + gridDim.x * stage_rows + group;
           if (n < rows) {
             mu = mean[n];
             rs = rstd[n];
           }
         }
-        const char* row = ring_mem + 2 * (stage * ring.stage_rows + i) * ring.row_bytes;
+        const char* row = my_ring + stage_at + 2 * i * ring.row_bytes;
         const T* row_g = reinterpret_cast<const T*>(row + (VEC * sizeof(T) == 16 ? 0 : ln_offset(sg, r)));
         const T* row_x = reinterpret_cast<const T*>(row + ring.row_bytes + (VEC * sizeof(T) == 16 ? 0 : ln_offset(sx, r)));
-        // u = dy w and h of one access; zero dy behind the row's end, so that nothing there enters a sum
-        auto terms = [&](int k, float (&g)[VEC], float (&h)[VEC], auto&& use) {
+        // dy and h of one access; zeros behind the row's end, so that nothing there enters a sum
+        auto terms = [&](int k, V (&g)[N], V (&h)[N]) {
           const int c = (lane + k * TPR) * VEC;
-          if (c < cols) {
-            load_vec<T, VEC>(row_g + c, g);
-            load_vec<T, VEC>(row_x + c, h);
+          if (ln_inside<TPR, PER>(k, c, cols)) {
+            load_lanes<T, VEC>(row_g + k * TPR * VEC, g);
+            load_lanes<T, VEC>(row_x + k * TPR * VEC, h);
           } else {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) g[j] = h[j] = 0.f;
+            for (int j = 0; j < N; ++j) g[j] = h[j] = vsplat<V>(0.f);
           }
           if constexpr (!HOLD) ln_weight<W, VEC>(w, c, cols, 1.f, fw[0]);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            h[j] = (h[j] - m) * q;
-            use(j, g[j], h[j]);
-            g[j] *= fw[HOLD ? k : 0][j];
-          }
+          for (int j = 0; j < N; ++j) h[j] = vmul(vadd(h[j], minus), q);
         };
-        float g[HOLD ? PER : 1][VEC], h[HOLD ? PER : 1][VEC];
-        float2 s = make_float2(0.f, 0.f);
+        V g[HOLD ? PER : 1][N], h[HOLD ? PER : 1][N];
+        V s1 = vsplat<V>(0.f), s2 = vsplat<V>(0.f);
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-          constexpr int ONE = HOLD ? 1 : 0;
-          terms(k, g[ONE * k], h[ONE * k], [&](int j, float dyj, float hj) {
-            aw[k][j] += dyj * hj;
-            ab[k][j] += dyj;
-          });
+          V (&gk)[N] = g[HOLD ? k : 0];
+          V (&hk)[N] = h[HOLD ? k : 0];
+          terms(k, gk, hk);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            s.x += g[ONE * k][j];
-            s.y += g[ONE * k][j] * h[ONE * k][j];
+          for (int j = 0; j < N; ++j) {
+            aw[k][j] = vfma(gk[j], hk[j], aw[k][j]);
+            ab[k][j] = vadd(ab[k][j], gk[j]);
+            gk[j] = vmul(gk[j], fw[HOLD ? k : 0][j]);            // u
+            s1 = vadd(s1, gk[j]);
+            s2 = vfma(gk[j], hk[j], s2);
           }
         }
+        float2 s = make_float2(vsum(s1), vsum(s2));
         if (TPR > 32 && HOLD) {                                 // the stage's only row is in registers
           __syncwarp();
           if ((lane & 31) == 0) mbar_arrive(&empty[stage]);
@@ -472,16 +470,21 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
         s = row_sum2<TPR>(s, scratch, slot);
         slot ^= 1;
         if (dx != nullptr) {
-          const float c1 = s.x * inv_n, c2 = s.y * inv_n;
-          T* out = dx + r * lddx;
+          const V c1 = vsplat<V>(-s.x * inv_n), c2 = vsplat<V>(-s.y * inv_n);
+          T* out = my_dx + r * lddx;
 #pragma unroll
           for (int k = 0; k < PER; ++k) {
-            constexpr int ONE = HOLD ? 1 : 0;
             const int c = (lane + k * TPR) * VEC;
-            if constexpr (!HOLD) terms(k, g[0], h[0], [](int, float, float) {});   // read once more instead of held
+            V (&gk)[N] = g[HOLD ? k : 0];
+            V (&hk)[N] = h[HOLD ? k : 0];
+            if constexpr (!HOLD) {                                // read once more instead of held
+              terms(k, gk, hk);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) g[ONE * k][j] = q * (g[ONE * k][j] - c1 - h[ONE * k][j] * c2);
-            if (c < cols) store_vec<T, VEC>(out + c, g[ONE * k]);
+              for (int j = 0; j < N; ++j) gk[j] = vmul(gk[j], fw[0][j]);
+            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) gk[j] = vmul(vfma(hk[j], c2, vadd(gk[j], c1)), q);
+            if (ln_inside<TPR, PER>(k, c, cols)) store_lanes<T, VEC>(out + k * TPR * VEC, gk);
           }
         }
       }
@@ -489,35 +492,46 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
         __syncwarp();
         if ((lane & 31) == 0) mbar_arrive(&empty[stage]);
       }
-      if (++stage == ring.stages) { stage = 0; phase ^= 1u; }
+      stage_at += 2 * stage_rows * ring.row_bytes;
+      if (++stage == ring.stages) { stage = stage_at = 0; phase ^= 1u; }
     }
     if (part != nullptr) {
       float* out_w = part + static_cast<int64_t>(blockIdx.x) * cols;
       float* out_b = part + static_cast<int64_t>(gridDim.x + blockIdx.x) * cols;
       if constexpr (GROUPS == 1) {
-        ln_write<float, VEC, PER, TPR>(out_w, lane, cols, aw);
-        ln_write<float, VEC, PER, TPR>(out_b, lane, cols, ab);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          const int c = (lane + k * TPR) * VEC;
+          if (c < cols) {
+            store_lanes<float, VEC>(out_w + c, aw[k]);
+            store_lanes<float, VEC>(out_b + c, ab[k]);
+          }
+        }
       } else {
         // the warps' sums one after the other, in a fixed order
-        __shared__ float2 sums[TPR * PER * VEC];
+        __shared__ __align__(16) float sums_w[TPR * PER * VEC], sums_b[TPR * PER * VEC];
         for (int g = 0; g < GROUPS; ++g) {
           if (group == g) {
 #pragma unroll
-            for (int k = 0; k < PER; ++k)
+            for (int k = 0; k < PER; ++k) {
+              const int c = (lane + k * TPR) * VEC;
+              V tw[N], tb[N];
+              load_lanes<float, VEC>(sums_w + c, tw);
+              load_lanes<float, VEC>(sums_b + c, tb);
 #pragma unroll
-              for (int j = 0; j < VEC; ++j) {
-                const int c = (lane + k * TPR) * VEC + j;
-                float2 v = g > 0 ? sums[c] : make_float2(0.f, 0.f);
-                v.x += aw[k][j];
-                v.y += ab[k][j];
-                sums[c] = v;
+              for (int j = 0; j < N; ++j) {
+                tw[j] = g > 0 ? vadd(tw[j], aw[k][j]) : aw[k][j];
+                tb[j] = g > 0 ? vadd(tb[j], ab[k][j]) : ab[k][j];
               }
+              store_lanes<float, VEC>(sums_w + c, tw);
+              store_lanes<float, VEC>(sums_b + c, tb);
+            }
           }
           named_bar_sync(1, GROUPS * TPR);
         }
         for (int c = threadIdx.x; c < cols; c += GROUPS * TPR) {
-          out_w[c] = sums[c].x;
-          out_b[c] = sums[c].y;
+          out_w[c] = sums_w[c];
+          out_b[c] = sums_b[c];
         }
       }
     }
@@ -579,7 +593,7 @@ template <typename T, typename W, int VEC, int PER, int TPR>
 static int ln_fwd_rows(const LayerNormArgs& a, int align, const DeviceInfo* dev, cudaStream_t stream, bool* done) {
   constexpr int GROUPS = ln_groups<TPR>(), PER_SM = ln_per_sm<TPR, false>(), BATCH = TPR == 512 && PER * VEC <= 16 ? 2 : 1;
   const LnRing ring = ln_ring(a.cols, sizeof(T), align, 1, GROUPS, PER_SM, BATCH);
-  if (ring.stages < 2) return B200K_OK;
+  if (ring.stages < 2 || (TPR > 32 && a.cols <= TPR * VEC * (PER / 2))) return B200K_OK;   // the second is what ln_inside relies on
   auto kernel = ln_fwd_kernel<T, W, VEC, PER, TPR, BATCH>;
   const int smem = ring.stages * ring.stage_rows * ring.row_bytes;
   B200K_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 208 * 1024));
@@ -597,7 +611,7 @@ template <typename T, typename W, int VEC, int PER, int TPR>
 static int ln_bwd_rows(const LayerNormArgs& a, int align, const DeviceInfo* dev, float* part, int* parts, cudaStream_t stream, bool* done) {
   constexpr int GROUPS = ln_groups<TPR>(), PER_SM = ln_per_sm<TPR, true>();
   const LnRing ring = ln_ring(a.cols, sizeof(T), align, 2, GROUPS, PER_SM, 1);
-  if (ring.stages < 2) return B200K_OK;
+  if (ring.stages < 2 || (TPR > 32 && a.cols <= TPR * VEC * (PER / 2))) return B200K_OK;   // the second is what ln_inside relies on
   auto kernel = ln_bwd_kernel<T, W, VEC, PER, TPR>;
   const int smem = 2 * ring.stages * ring.stage_rows * ring.row_bytes;
   B200K_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 208 * 1024));
@@ -615,7 +629,8 @@ static int ln_bwd_rows(const LayerNormArgs& a, int align, const DeviceInfo* dev,
 }
 
 // Calls f with the kernel shape for rows of `cols` elements of `size` bytes whose operands share `align`: (VEC, PER, TPR) as integral constants.
-// 16 elements a thread or less, 32 beyond 8192; false beyond 16384 elements.
+// 16 elements a thread or less, 32 beyond 8192; false beyond 16384 elements.  A warp takes a row of up to 512; a CTA-wide shape is the smallest one
+// that holds the row, so that more than half of it is filled.
 template <int N>
 using Int = std::integral_constant<int, N>;
 template <int SIZE, typename F>
@@ -625,6 +640,8 @@ static bool ln_shape(int64_t cols, int align, F&& f) {
     const int64_t u = cols / V;
     if (u <= 32) f(Int<V>(), Int<1>(), Int<32>());
     else if (u <= 64) f(Int<V>(), Int<2>(), Int<32>());
+    else if (u <= 512 / V) f(Int<V>(), Int<4>(), Int<32>());
+    else if (u <= 1024 / V) f(Int<V>(), Int<8 / V>(), Int<128>());
     else if (u <= 2 * 1024 / V) f(Int<V>(), Int<16 / V>(), Int<128>());
     else if (u <= 4 * 1024 / V) f(Int<V>(), Int<16 / V>(), Int<256>());
     else if (u <= 8 * 1024 / V) f(Int<V>(), Int<16 / V>(), Int<512>());
@@ -635,6 +652,7 @@ static bool ln_shape(int64_t cols, int align, F&& f) {
   if constexpr (SIZE == 2) if (align >= 4) {
     if (cols <= 256) f(Int<2>(), Int<4>(), Int<32>());
     else if (cols <= 512) f(Int<2>(), Int<8>(), Int<32>());
+    else if (cols <= 1024) f(Int<2>(), Int<4>(), Int<128>());
     else if (cols <= 2048) f(Int<2>(), Int<8>(), Int<128>());
     else if (cols <= 4096) f(Int<2>(), Int<8>(), Int<256>());
     else if (cols <= 8192) f(Int<2>(), Int<8>(), Int<512>());
@@ -644,6 +662,7 @@ static bool ln_shape(int64_t cols, int align, F&& f) {
   }
   if (cols <= 256) f(Int<1>(), Int<8>(), Int<32>());
   else if (cols <= 512) f(Int<1>(), Int<16>(), Int<32>());
+  else if (cols <= 1024) f(Int<1>(), Int<8>(), Int<128>());
   else if (cols <= 2048) f(Int<1>(), Int<16>(), Int<128>());
   else if (cols <= 4096) f(Int<1>(), Int<16>(), Int<256>());
   else if (cols <= 8192) f(Int<1>(), Int<16>(), Int<512>());
