@@ -79,48 +79,120 @@ __device__ __forceinline__ uint32_t scale_exponent(float peak) {
 __device__ __forceinline__ float scale_of(uint32_t e) { return __uint_as_float((e - 15) << 23); }
 __device__ __forceinline__ float inverse_scale_of(uint32_t e) { return __uint_as_float((269 - e) << 23); }
 
-template <int MB>
-__device__ __forceinline__ float code_value(uint32_t c) {
-  constexpr uint32_t MASK = (1u << (4 + MB)) - 1;
-  const uint32_t mag = c & MASK;
-  float v = __uint_as_float((mag << (23 - MB)) + (127u << 23));
-  v = mag == 0 ? 0.f : v;
-  v = mag == MASK ? __int_as_float(0x7FC00000) : v;
-  return (MB == 3 && (c & 0x80u)) ? -v : v;
+// prmt with the top bit of the selected bytes spread over them (selector nibbles 8..15, which __byte_perm does not pass on).
+__device__ __forceinline__ uint32_t spread_top(uint32_t x, uint32_t selector) {
+  uint32_t d;
+  asm("prmt.b32 %0, %1, %1, %2;" : "=r"(d) : "r"(x), "r"(selector));
+  return d;
 }
 
-// |x| * inverse scale -> code, given 16 random bits.
+// The four elements of a word of codes.
 template <int MB>
-__device__ __forceinline__ uint32_t code_of(float x, float inverse, uint32_t random16) {
+__device__ __forceinline__ void decode4(uint32_t word, float scale, float (&f)[4]) {
+  constexpr uint32_t MASK = MB == 3 ? 0x7F7F7F7Fu : 0xFFFFFFFFu;
+  const uint32_t mag = word & MASK;
+  uint32_t bits[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) bits[j] = __byte_perm(mag, 0, 0x4440 + j) * (1u << (23 - MB)) + (127u << 23);
+  if (MB == 3) {
+    // zeros are common among first moments: a mask per element, and the sign with the same instruction
+    const uint32_t some = mag + 0x7F7F7F7Fu, sign = word & 0x80808080u;      // some: top bit of each byte that is not 0
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bits[j] = (bits[j] & spread_top(some, 0x8888 + 0x1111 * j)) | __byte_perm(sign, 0, (j << 12) | 0x0444);
+  }
+  // rare: the NaN code, and a zero root.  All four bytes at once, by carries; a false alarm only costs time.
+  const uint32_t rare = MB == 3 ? (mag + 0x01010101u) & 0x80808080u : ((mag - 0x01010101u) & ~mag & 0x80808080u) | ((~mag - 0x01010101u) & mag & 0x80808080u);
+  if (rare != 0) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t c = (mag >> (8 * j)) & 0xFFu;
+      if (c == (1u << (4 + MB)) - 1) bits[j] = 0x7FC00000u;
+      if (MB == 4 && c == 0) bits[j] = 0;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[j] = __fmul_rn(__uint_as_float(bits[j]), scale);
+}
+
+__device__ __forceinline__ bool is_finite(float x) { return fabsf(x) <= 3.4028234663852886e38f; }
+
+// The codes of four elements, without signs, given 16 random bits of each hash.  `finite`: none of the block's elements is infinite or NaN.
+template <int MB>
+__device__ __forceinline__ uint32_t encode4(const float (&x)[4], float inverse, const uint32_t (&hash)[4], bool finite) {
   constexpr float LEAST = 1.f + 1.f / (1 << MB);       // value of code 1
-  const float a = fabsf(x);
-  const float y = __fmul_rn(a, inverse);
-  // normal codes: add random bits below the kept ones, then cut them off
-  const uint32_t raw = (__float_as_uint(y) - (127u << 23) + (random16 << (7 - MB))) >> (23 - MB);
-  // below code 1: an m up to it with probability y / value(1), an r always
-  const uint32_t small = (MB == 4 ? 0.f : static_cast<float>(2 * random16 + 1) * (LEAST * 0x1p-17f)) < y ? 1u : 0u;
-  uint32_t c = y < LEAST ? small : raw;
-  if (!(a <= 3.4028234663852886e38f)) c = (1u << (4 + MB)) - 1;
-  if (MB == 3 && x < 0.f) c |= 0x80u;
-  return c;
+  uint32_t c[4];
+  float y[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    y[j] = __fmul_rn(fabsf(x[j]), inverse);
+    // normal codes: add the random bits just below the kept ones, then cut them off
+    const uint32_t rnd = MB == 3 ? (hash[j] & 0xFFFFu) << 4 : (hash[j] >> 13) & ~7u;
+    c[j] = (__float_as_uint(y[j]) + rnd - (127u << 23)) >> (23 - MB);
+  }
+  if (fminf(fminf(y[0], y[1]), fminf(y[2], y[3])) < LEAST) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // below code 1: an m up to it with probability y / value(1), an r above zero always.  u = 1 + (2 r + 1) / 2^17 for the 16 bits r.
+      const float u = __uint_as_float(0x3F800040u | (hash[j] & 0xFFFFu) << 7);
+      const uint32_t small = (MB == 3 ? fmaf(u, LEAST, -LEAST) : 0.f) < y[j] ? 1u : 0u;
+      c[j] = y[j] < LEAST ? small : c[j];
+    }
+  }
+  if (!finite) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[j] = is_finite(x[j]) ? c[j] : (1u << (4 + MB)) - 1;
+  }
+  return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+}
+// The sign bits of four elements, at the top of their bytes.
+__device__ __forceinline__ uint32_t signs4(const float (&x)[4]) {
+  const uint32_t lo = __byte_perm(__float_as_uint(x[0]), __float_as_uint(x[1]), 0x0073);
+  const uint32_t hi = __byte_perm(__float_as_uint(x[2]), __float_as_uint(x[3]), 0x0073);
+  return __byte_perm(lo, hi, 0x5410) & 0x80808080u;
 }
 
-__device__ __forceinline__ float finite_abs(float x) {
-  const float a = fabsf(x);
-  return a <= 3.4028234663852886e38f ? a : 0.f;
+// Maximum that lets NaN through.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
-__device__ __forceinline__ float warp_max_nonneg(float v) {   // floats >= 0 order like their bits
+__device__ __forceinline__ float warp_max_nonneg(float v) {   // floats >= 0 order like their bits, infinity and NaN above them
   return __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v)));
 }
 
-// 4 consecutive elements at p[0..4) of which the first `left` exist.
+// 4 consecutive elements at p[0..4), of which the first `left` exist, as the words that they take in memory.
 template <typename T>
-__device__ __forceinline__ void load4(const T* p, bool vec, int left, float (&f)[4]) {
+struct Four {
+  uint32_t w[sizeof(T)];
+};
+template <typename T>
+__device__ __forceinline__ Four<T> fetch4(const T* p, bool vec, int left) {
+  Four<T> v;
   if (vec) {
-    load_vec<T, 4>(p, f);
+    if constexpr (sizeof(T) == 4) {
+      const uint4 u = *reinterpret_cast<const uint4*>(p);
+      v.w[0] = u.x; v.w[1] = u.y; v.w[2] = u.z; v.w[3] = u.w;
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      v.w[0] = u.x; v.w[1] = u.y;
+    }
   } else {
+    float f[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = i < left ? to_f32<T>(p[i]) : 0.f;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) {
+      if constexpr (sizeof(T) == 4) v.w[i] = __float_as_uint(f[i]); else v.w[i] = pack_word<T>(f[2 * i], f[2 * i + 1]);
+    }
+  }
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void values4(const Four<T>& v, float (&f)[4]) {
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) {
+    if constexpr (sizeof(T) == 4) f[i] = __uint_as_float(v.w[i]); else unpack_word<T>(v.w[i], f[2 * i], f[2 * i + 1]);
   }
 }
 template <typename T>
@@ -131,6 +203,68 @@ __device__ __forceinline__ void store4(T* p, bool vec, int left, const float (&f
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (i < left) p[i] = from_f32<T>(f[i]);
+  }
+}
+
+// sqrt(x), correctly rounded, of an x in [2^-60, 2^120]: Goldschmidt's iteration from an approximate 1 / sqrt(x), and a last step on the exact residual,
+// which by Markstein's theorem rounds correctly (P. Markstein, IA-64 and Elementary Functions, ch. 9).  Without the range test of the
+// general function it takes no branch.
+__device__ __forceinline__ float sqrt_in_range(float x) {
+  float y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  float g = __fmul_rn(x, y), h = __fmul_rn(0.5f, y);
+  const float r = __fmaf_rn(-g, h, 0.5f);
+  g = __fmaf_rn(g, r, g);
+  h = __fmaf_rn(h, r, h);
+  return __fmaf_rn(__fmaf_rn(-g, g, x), h, g);
+}
+__device__ __forceinline__ void sqrt4(const float (&x)[4], float (&root)[4]) {
+  const float lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3]));
+  const float hi = max_nan(max_nan(x[0], x[1], x[2]), x[3], x[3]);
+  if (lo >= 0x1p-60f && hi <= 0x1p120f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) root[j] = sqrt_in_range(x[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) root[j] = __fsqrt_rn(x[j]);
+  }
+}
+
+// What a lane reads of a block: twice four elements, 128 apart.
+template <typename P, typename G, bool MASTER, int BITS>
+struct AdamwBlock {
+  Four<P> p[MASTER ? 1 : 2];
+  Four<float> master[MASTER ? 2 : 1];
+  Four<G> g[2];
+  uint32_t cm[2], cr[2];                           // 8-bit moments
+  Four<float> m[BITS == 32 ? 2 : 1], v[BITS == 32 ? 2 : 1];
+  float scale_m, scale_r;
+};
+__device__ __forceinline__ int left_of(int64_t i, int64_t end) { return i >= end ? 0 : (end - i < 4 ? static_cast<int>(end - i) : 4); }
+
+// `full`: the block is whole and everything is aligned (the same for all lanes).
+template <typename P, typename G, bool MASTER, int BITS>
+__device__ __forceinline__ void adamw_read(AdamwBlock<P, G, MASTER, BITS>& k, const b200k_adamw_tensor& t, int64_t base, int64_t end, bool full) {
+  const int64_t i0 = base + (threadIdx.x & 31) * 4;
+  if constexpr (BITS == 8) {
+    k.scale_m = t.m_scale[base / ADAMW_BLOCK];
+    k.scale_r = t.v_scale[base / ADAMW_BLOCK];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {                  // the code buffers are padded to whole blocks
+      k.cm[h] = reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(t.m) + i0)[32 * h];
+      k.cr[h] = reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(t.v) + i0)[32 * h];
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int64_t i = i0 + h * 128;
+    const int left = full ? 4 : left_of(i, end);
+    if constexpr (MASTER) k.master[h] = fetch4<float>(t.master + i, full, left); else k.p[h] = fetch4<P>(static_cast<const P*>(t.p) + i, full, left);
+    k.g[h] = fetch4<G>(static_cast<const G*>(t.g) + i, full, left);
+    if constexpr (BITS == 32) {
+      k.m[h] = fetch4<float>(static_cast<const float*>(t.m) + i, full, left);
+      k.v[h] = fetch4<float>(static_cast<const float*>(t.v) + i, full, left);
+    }
   }
 }
 
@@ -156,79 +290,91 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const __grid_const
   const int64_t end = begin + ADAMW_CHUNK < t.n ? begin + ADAMW_CHUNK : t.n;
   const uint32_t salt = BITS == 8 ? mix32(mix32(q.seed + step * 0x9E3779B9u) + static_cast<uint32_t>(t.index)) : 0u;
   P* const tp = static_cast<P*>(t.p);
-  const G* const tg = static_cast<const G*>(t.g);
-  const uintptr_t odd = (reinterpret_cast<uintptr_t>(tp) & (4 * sizeof(P) - 1)) | (reinterpret_cast<uintptr_t>(tg) & (4 * sizeof(G) - 1));
+  const bool aligned = ((reinterpret_cast<uintptr_t>(tp) & (4 * sizeof(P) - 1)) | (reinterpret_cast<uintptr_t>(t.g) & (4 * sizeof(G) - 1))) == 0;
 
-  for (int64_t base = begin + warp * ADAMW_BLOCK; base < end; base += (ADAMW_THREADS / 32) * ADAMW_BLOCK) {
+  // the next block's loads are under way while this one is worked on
+  AdamwBlock<P, G, MASTER, BITS> next;
+  int64_t base = begin + warp * ADAMW_BLOCK;
+  if (base < end) adamw_read<P, G, MASTER, BITS>(next, t, base, end, aligned && base + ADAMW_BLOCK <= end);
+  for (; base < end; base += (ADAMW_THREADS / 32) * ADAMW_BLOCK) {
     const int64_t block = base / ADAMW_BLOCK;
+    const AdamwBlock<P, G, MASTER, BITS> now = next;
+    const int64_t following = base + (ADAMW_THREADS / 32) * ADAMW_BLOCK;
+    if (following < end) adamw_read<P, G, MASTER, BITS>(next, t, following, end, aligned && following + ADAMW_BLOCK <= end);
+    const bool full = aligned && base + ADAMW_BLOCK <= end;
     float m1[2][4], root[2][4];
     float peak_m = 0.f, peak_r = 0.f;
-    float scale_m = 0.f, scale_r = 0.f;
-    if (BITS == 8) {
-      scale_m = t.m_scale[block];
-      scale_r = t.v_scale[block];
-    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int64_t i = base + h * 128 + lane * 4;
-      const int left = i >= end ? 0 : (end - i < 4 ? static_cast<int>(end - i) : 4);
-      const bool vec = odd == 0 && left == 4;
+      const int left = full ? 4 : left_of(i, end);
       float p[4], g[4], m[4], v[4];
-      if (MASTER) load4<float>(t.master + i, left == 4, left, p); else load4<P>(tp + i, vec, left, p);
-      load4<G>(tg + i, vec, left, g);
-      if (BITS == 8) {
-        // the code buffers are padded to whole blocks
-        const uint32_t cm = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(t.m) + i);
-        const uint32_t cr = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(t.v) + i);
+      if constexpr (MASTER) values4<float>(now.master[h], p); else values4<P>(now.p[h], p);
+      values4<G>(now.g[h], g);
+      if constexpr (BITS == 8) {
+        decode4<3>(now.cm[h], now.scale_m, m);
+        decode4<4>(now.cr[h], now.scale_r, v);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          m[j] = __fmul_rn(code_value<3>((cm >> (8 * j)) & 0xFFu), scale_m);
-          const float r = __fmul_rn(code_value<4>((cr >> (8 * j)) & 0xFFu), scale_r);
-          v[j] = __fmul_rn(r, r);
-        }
+        for (int j = 0; j < 4; ++j) v[j] = __fmul_rn(v[j], v[j]);
       } else {
-        load4<float>(static_cast<const float*>(t.m) + i, left == 4, left, m);
-        load4<float>(static_cast<const float*>(t.v) + i, left == 4, left, v);
+        values4<float>(now.m[h], m);
+        values4<float>(now.v[h], v);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float gj = __fmul_rn(g[j], grad_scale);
-        m[j] = __fadd_rn(__fmul_rn(m[j], q.b1), __fmul_rn(gj, q.one_minus_b1));
-        v[j] = __fadd_rn(__fmul_rn(v[j], q.b2), __fmul_rn(__fmul_rn(gj, gj), q.one_minus_b2));
-        root[h][j] = __fsqrt_rn(v[j]);
+        g[j] = __fmul_rn(g[j], grad_scale);
+        m[j] = __fadd_rn(__fmul_rn(m[j], q.b1), __fmul_rn(g[j], q.one_minus_b1));
+        v[j] = __fadd_rn(__fmul_rn(v[j], q.b2), __fmul_rn(__fmul_rn(g[j], g[j]), q.one_minus_b2));
         m1[h][j] = m[j];
-        p[j] = p[j] * decay - (m[j] / (root[h][j] * inv_sqrt_bc2 + q.eps)) * step_size;
-        if (BITS == 8 && j < left) {
-          peak_m = fmaxf(peak_m, finite_abs(m[j]));
-          peak_r = fmaxf(peak_r, finite_abs(root[h][j]));
-        }
       }
-      if (MASTER) store4<float>(t.master + i, left == 4, left, p);
-      store4<P>(tp + i, vec, left, p);
+      sqrt4(v, root[h]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // p alone may round otherwise than the plain formula: the quotient takes an approximate reciprocal (1 unit in the last place), of an
+        // update that is itself a small part of p.  The divisor is zero or a normal number: sqrt of the smallest fp32 is 2^-74.5.
+        float inverse;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(fmaf(root[h][j], inv_sqrt_bc2, q.eps)));
+        p[j] = p[j] * decay - m[j] * inverse * step_size;
+      }
+      if (BITS == 8) {                     // behind the tensor's end all of it is zero
+        peak_m = max_nan(max_nan(peak_m, fabsf(m[0]), fabsf(m[1])), fabsf(m[2]), fabsf(m[3]));
+        peak_r = max_nan(max_nan(peak_r, root[h][0], root[h][1]), root[h][2], root[h][3]);
+      }
+      if (MASTER) store4<float>(t.master + i, full, left, p);
+      store4<P>(tp + i, full, left, p);
       if (BITS == 32) {
-        store4<float>(static_cast<float*>(t.m) + i, left == 4, left, m);
-        store4<float>(static_cast<float*>(t.v) + i, left == 4, left, v);
+        store4<float>(static_cast<float*>(t.m) + i, full, left, m);
+        store4<float>(static_cast<float*>(t.v) + i, full, left, v);
       }
     }
     if (BITS == 8) {
       peak_m = warp_max_nonneg(peak_m);
       peak_r = warp_max_nonneg(peak_r);
+      const bool finite_m = is_finite(peak_m), finite_r = is_finite(peak_r);
+      if (!(finite_m && finite_r)) {         // the largest finite magnitudes
+        peak_m = peak_r = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (is_finite(m1[h][j])) peak_m = fmaxf(peak_m, fabsf(m1[h][j]));
+            if (is_finite(root[h][j])) peak_r = fmaxf(peak_r, root[h][j]);
+          }
+        peak_m = warp_max_nonneg(peak_m);
+        peak_r = warp_max_nonneg(peak_r);
+      }
       const uint32_t exp_m = scale_exponent<3>(peak_m), exp_r = scale_exponent<4>(peak_r);
       const float inv_m = inverse_scale_of(exp_m), inv_r = inverse_scale_of(exp_r);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int64_t i = base + h * 128 + lane * 4;
-        uint32_t cm = 0, cr = 0;
+        uint32_t hash[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t rnd = mix32(static_cast<uint32_t>(i + j) + salt);
-          if (i + j < end) {
-            cm |= code_of<3>(m1[h][j], inv_m, rnd & 0xFFFFu) << (8 * j);
-            cr |= code_of<4>(root[h][j], inv_r, rnd >> 16) << (8 * j);
-          }
-        }
-        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.m) + i) = cm;
-        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.v) + i) = cr;
+        for (int j = 0; j < 4; ++j) hash[j] = mix32(static_cast<uint32_t>(i) + j + salt);
+        // behind the tensor's end the codes are those of zero
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.m) + i) =
+            peak_m == 0.f && finite_m ? 0u : encode4<3>(m1[h], inv_m, hash, finite_m) | signs4(m1[h]);
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.v) + i) = peak_r == 0.f && finite_r ? 0u : encode4<4>(root[h], inv_r, hash, finite_r);
       }
       if (lane == 0) {
         t.m_scale[block] = scale_of(exp_m);
@@ -263,17 +409,11 @@ __global__ void __launch_bounds__(256) adamw_moments_kernel(const uint8_t* __res
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= n4) return;
   const int64_t block = i / (ADAMW_BLOCK / 4);
-  const uint32_t cm = reinterpret_cast<const uint32_t*>(m)[i], cr = reinterpret_cast<const uint32_t*>(r)[i];
-  const float sm = m_scale[block], sr = r_scale[block];
-  float4 a, b;
-  float* fa = &a.x;
-  float* fb = &b.x;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    fa[j] = __fmul_rn(code_value<3>((cm >> (8 * j)) & 0xFFu), sm);
-    const float x = __fmul_rn(code_value<4>((cr >> (8 * j)) & 0xFFu), sr);
-    fb[j] = __fmul_rn(x, x);
-  }
+  float fm[4], fr[4];
+  decode4<3>(reinterpret_cast<const uint32_t*>(m)[i], m_scale[block], fm);
+  decode4<4>(reinterpret_cast<const uint32_t*>(r)[i], r_scale[block], fr);
+  const float4 a = make_float4(fm[0], fm[1], fm[2], fm[3]);
+  const float4 b = make_float4(__fmul_rn(fr[0], fr[0]), __fmul_rn(fr[1], fr[1]), __fmul_rn(fr[2], fr[2]), __fmul_rn(fr[3], fr[3]));
   reinterpret_cast<float4*>(m_out)[i] = a;
   reinterpret_cast<float4*>(v_out)[i] = b;
 }
