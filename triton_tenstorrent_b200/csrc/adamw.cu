@@ -56,17 +56,20 @@ struct AdamwParams {
   double b1d, b2d;
   float b1, one_minus_b1, b2, one_minus_b2, eps, grad_scale;
   uint32_t seed;
+  // Powers of two that come as parameters: a shift and add by a constant would run on the ALU pipe, which the byte and bit work of the 8-bit moments
+  // fills before anything else; a multiply-add by a number the compiler does not know runs on the FMA pipe.
+  uint32_t two4, two5, two16, two19, two20;
   int n;                         // tensors in the table
   int advance;                   // this launch ends the step
 };
 
 // 32-bit hash: two rounds of xor-shift and an odd multiplier (the leading bits of sqrt(3)/2 and sqrt(2)/2).
-__device__ __forceinline__ uint32_t mix32(uint32_t x) {
-  x ^= x >> 16;
+__device__ __forceinline__ uint32_t mix32(uint32_t x, uint32_t two16) {
+  x ^= __umulhi(x, two16);           // x >> 16
   x *= 0xDDB3D743u;
   x ^= x >> 15;
   x *= 0xB504F335u;
-  return x ^ (x >> 16);
+  return x ^ __umulhi(x, two16);
 }
 
 // Exponent field E of the block's scale 2^(E - 142): the largest finite code has the value (2 - 2^(1 - MB)) 2^15, and adding what a mantissa may
@@ -86,14 +89,14 @@ __device__ __forceinline__ uint32_t spread_top(uint32_t x, uint32_t selector) {
   return d;
 }
 
-// The four elements of a word of codes.
+// The values of a word's four codes (to be multiplied by their block's scale); up = 2^(23 - MB).
 template <int MB>
-__device__ __forceinline__ void decode4(uint32_t word, float scale, float (&f)[4]) {
+__device__ __forceinline__ void decode4(uint32_t word, uint32_t up, float (&f)[4]) {
   constexpr uint32_t MASK = MB == 3 ? 0x7F7F7F7Fu : 0xFFFFFFFFu;
   const uint32_t mag = word & MASK;
   uint32_t bits[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) bits[j] = __byte_perm(mag, 0, 0x4440 + j) * (1u << (23 - MB)) + (127u << 23);
+  for (int j = 0; j < 4; ++j) bits[j] = __byte_perm(mag, 0, 0x4440 + j) * up + (127u << 23);
   if (MB == 3) {
     // zeros are common among first moments: a mask per element, and the sign with the same instruction
     const uint32_t some = mag + 0x7F7F7F7Fu, sign = word & 0x80808080u;      // some: top bit of each byte that is not 0
@@ -111,44 +114,52 @@ __device__ __forceinline__ void decode4(uint32_t word, float scale, float (&f)[4
     }
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) f[j] = __fmul_rn(__uint_as_float(bits[j]), scale);
+  for (int j = 0; j < 4; ++j) f[j] = __uint_as_float(bits[j]);
 }
 
 __device__ __forceinline__ bool is_finite(float x) { return fabsf(x) <= 3.4028234663852886e38f; }
 
-// The codes of four elements, without signs, given 16 random bits of each hash.  `finite`: none of the block's elements is infinite or NaN.
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// The codes of four elements, m's with their signs, given 16 random bits of each hash.  up = 2^(1 + MB).  `finite`: none of the block's elements is infinite or NaN.
+//
+// A normal code is the exponent and the MB first mantissa bits of |x| * inverse (in [1, 2^16), so that exponent 127 is 0), after the random bits were
+// added just below them.  Multiplied by 2^(1 + MB) those 4 + MB bits are the top byte of the word (m's with a zero above them), the random bits
+// are bytes 1 and 2 of what is added, and the exponent's offset is a constant in byte 3: a byte permutation and a multiply-add.
 template <int MB>
-__device__ __forceinline__ uint32_t encode4(const float (&x)[4], float inverse, const uint32_t (&hash)[4], bool finite) {
+__device__ __forceinline__ uint32_t encode4(const float (&x)[4], float inverse, const uint32_t (&hash)[4], uint32_t up, bool finite) {
   constexpr float LEAST = 1.f + 1.f / (1 << MB);       // value of code 1
   uint32_t c[4];
   float y[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     y[j] = __fmul_rn(fabsf(x[j]), inverse);
-    // normal codes: add the random bits just below the kept ones, then cut them off
-    const uint32_t rnd = MB == 3 ? (hash[j] & 0xFFFFu) << 4 : (hash[j] >> 13) & ~7u;
-    c[j] = (__float_as_uint(y[j]) + rnd - (127u << 23)) >> (23 - MB);
+    // -(127 << 23) * up is 8 << 24 and 16 << 24 modulo 2^32
+    const uint32_t add = __byte_perm(hash[j], MB == 3 ? 0x08u : 0x10u, MB == 3 ? 0x4105 : 0x4325);
+    c[j] = __float_as_uint(y[j]) * up + add;
   }
-  if (fminf(fminf(y[0], y[1]), fminf(y[2], y[3])) < LEAST) {
+  if (min3(min3(y[0], y[1], y[2]), y[3], y[3]) < LEAST) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       // below code 1: an m up to it with probability y / value(1), an r above zero always.  u = 1 + (2 r + 1) / 2^17 for the 16 bits r.
-      const float u = __uint_as_float(0x3F800040u | (hash[j] & 0xFFFFu) << 7);
-      const uint32_t small = (MB == 3 ? fmaf(u, LEAST, -LEAST) : 0.f) < y[j] ? 1u : 0u;
+      const float u = __uint_as_float((hash[j] & 0xFFFFu) * 128u + 0x3F800040u);
+      const uint32_t small = (MB == 3 ? fmaf(u, LEAST, -LEAST) : 0.f) < y[j] ? 1u << 24 : 0u;
       c[j] = y[j] < LEAST ? small : c[j];
     }
   }
   if (!finite) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) c[j] = is_finite(x[j]) ? c[j] : (1u << (4 + MB)) - 1;
+    for (int j = 0; j < 4; ++j) c[j] = is_finite(x[j]) ? c[j] : MB == 3 ? 0x7F000000u : 0xFF000000u;
   }
-  return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
-}
-// The sign bits of four elements, at the top of their bytes.
-__device__ __forceinline__ uint32_t signs4(const float (&x)[4]) {
-  const uint32_t lo = __byte_perm(__float_as_uint(x[0]), __float_as_uint(x[1]), 0x0073);
-  const uint32_t hi = __byte_perm(__float_as_uint(x[2]), __float_as_uint(x[3]), 0x0073);
-  return __byte_perm(lo, hi, 0x5410) & 0x80808080u;
+  if (MB == 3) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[j] = (c[j] & 0x7FFFFFFFu) | (__float_as_uint(x[j]) & 0x80000000u);
+  }
+  return __byte_perm(__byte_perm(c[0], c[1], 0x0073), __byte_perm(c[2], c[3], 0x0073), 0x5410);
 }
 
 // Maximum that lets NaN through.
@@ -206,27 +217,33 @@ __device__ __forceinline__ void store4(T* p, bool vec, int left, const float (&f
   }
 }
 
-// sqrt(x), correctly rounded, of an x in [2^-60, 2^120]: Goldschmidt's iteration from an approximate 1 / sqrt(x), and a last step on the exact residual,
-// which by Markstein's theorem rounds correctly (P. Markstein, IA-64 and Elementary Functions, ch. 9).  Without the range test of the
-// general function it takes no branch.
-__device__ __forceinline__ float sqrt_in_range(float x) {
-  float y;
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  float g = __fmul_rn(x, y), h = __fmul_rn(0.5f, y);
-  const float r = __fmaf_rn(-g, h, 0.5f);
-  g = __fmaf_rn(g, r, g);
-  h = __fmaf_rn(h, r, h);
-  return __fmaf_rn(__fmaf_rn(-g, g, x), h, g);
+// sqrt(x), correctly rounded, of two numbers in [2^-60, 2^120]: Goldschmidt's iteration from an approximate 1 / sqrt(x), and a last step on the exact
+// residual, which by Markstein's theorem rounds correctly (P. Markstein, IA-64 and Elementary Functions, ch. 9).  Without the range test of
+// the general function it takes no branch and runs on packed numbers.  Half the reciprocal root and the residual are held negated.
+__device__ __forceinline__ uint64_t sqrt_in_range(uint64_t x) {
+  float x0, x1, y0, y1;
+  unpack_f32x2(x, x0, x1);
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y0) : "f"(x0));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y1) : "f"(x1));
+  const uint64_t y = pack_f32x2(y0, y1);
+  uint64_t g = mul_f32x2(x, y), h = mul_f32x2(pack_f32x2(-0.5f, -0.5f), y);
+  const uint64_t r = fma_f32x2(g, h, pack_f32x2(0.5f, 0.5f));
+  g = fma_f32x2(g, r, g);
+  h = fma_f32x2(h, r, h);
+  return fma_f32x2(fma_f32x2(g, g, mul_f32x2(x, pack_f32x2(-1.f, -1.f))), h, g);
 }
-__device__ __forceinline__ void sqrt4(const float (&x)[4], float (&root)[4]) {
-  const float lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3]));
-  const float hi = max_nan(max_nan(x[0], x[1], x[2]), x[3], x[3]);
+__device__ __forceinline__ void sqrt4(const uint64_t (&x)[2], float (&root)[4]) {
+  float f[4];
+  unpack_f32x2(x[0], f[0], f[1]);
+  unpack_f32x2(x[1], f[2], f[3]);
+  const float lo = min3(min3(f[0], f[1], f[2]), f[3], f[3]);
+  const float hi = max_nan(max_nan(f[0], f[1], f[2]), f[3], f[3]);
   if (lo >= 0x1p-60f && hi <= 0x1p120f) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) root[j] = sqrt_in_range(x[j]);
+    for (int j = 0; j < 2; ++j) unpack_f32x2(sqrt_in_range(x[j]), root[2 * j], root[2 * j + 1]);
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) root[j] = __fsqrt_rn(x[j]);
+    for (int j = 0; j < 4; ++j) root[j] = __fsqrt_rn(f[j]);
   }
 }
 
@@ -288,9 +305,13 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const __grid_const
   const b200k_adamw_tensor& t = table.t[lo];
   const int64_t begin = static_cast<int64_t>(chunk - table.first_chunk[lo]) * ADAMW_CHUNK;
   const int64_t end = begin + ADAMW_CHUNK < t.n ? begin + ADAMW_CHUNK : t.n;
-  const uint32_t salt = BITS == 8 ? mix32(mix32(q.seed + step * 0x9E3779B9u) + static_cast<uint32_t>(t.index)) : 0u;
+  const uint32_t salt = BITS == 8 ? mix32(mix32(q.seed + step * 0x9E3779B9u, q.two16) + static_cast<uint32_t>(t.index), q.two16) : 0u;
   P* const tp = static_cast<P*>(t.p);
   const bool aligned = ((reinterpret_cast<uintptr_t>(tp) & (4 * sizeof(P) - 1)) | (reinterpret_cast<uintptr_t>(t.g) & (4 * sizeof(G) - 1))) == 0;
+
+  auto twice = [](float x) { return pack_f32x2(x, x); };
+  const uint64_t k_scale = twice(grad_scale), k_b1 = twice(q.b1), k_c1 = twice(q.one_minus_b1), k_b2 = twice(q.b2), k_c2 = twice(q.one_minus_b2),
+                 k_bc2 = twice(inv_sqrt_bc2), k_eps = twice(q.eps), k_decay = twice(decay), k_step = twice(-step_size);
 
   // the next block's loads are under way while this one is worked on
   AdamwBlock<P, G, MASTER, BITS> next;
@@ -312,29 +333,42 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const __grid_const
       if constexpr (MASTER) values4<float>(now.master[h], p); else values4<P>(now.p[h], p);
       values4<G>(now.g[h], g);
       if constexpr (BITS == 8) {
-        decode4<3>(now.cm[h], now.scale_m, m);
-        decode4<4>(now.cr[h], now.scale_r, v);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = __fmul_rn(v[j], v[j]);
+        decode4<3>(now.cm[h], q.two20, m);
+        decode4<4>(now.cr[h], q.two19, v);
       } else {
         values4<float>(now.m[h], m);
         values4<float>(now.v[h], v);
       }
+      // two elements at a time: each product and sum is rounded as a scalar one
+      uint64_t m2[2], v2[2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        g[j] = __fmul_rn(g[j], grad_scale);
-        m[j] = __fadd_rn(__fmul_rn(m[j], q.b1), __fmul_rn(g[j], q.one_minus_b1));
-        v[j] = __fadd_rn(__fmul_rn(v[j], q.b2), __fmul_rn(__fmul_rn(g[j], g[j]), q.one_minus_b2));
-        m1[h][j] = m[j];
+      for (int j = 0; j < 2; ++j) {
+        m2[j] = pack_f32x2(m[2 * j], m[2 * j + 1]);
+        v2[j] = pack_f32x2(v[2 * j], v[2 * j + 1]);
+        if (BITS == 8) {
+          m2[j] = mul_f32x2(m2[j], pack_f32x2(now.scale_m, now.scale_m));
+          v2[j] = mul_f32x2(v2[j], pack_f32x2(now.scale_r, now.scale_r));
+          v2[j] = mul_f32x2(v2[j], v2[j]);
+        }
+        const uint64_t g2 = mul_f32x2(pack_f32x2(g[2 * j], g[2 * j + 1]), k_scale);
+        m2[j] = add_f32x2(mul_f32x2(m2[j], k_b1), mul_f32x2(g2, k_c1));
+        v2[j] = add_f32x2(mul_f32x2(v2[j], k_b2), mul_f32x2(mul_f32x2(g2, g2), k_c2));
       }
-      sqrt4(v, root[h]);
+      sqrt4(v2, root[h]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 2; ++j) {
         // p alone may round otherwise than the plain formula: the quotient takes an approximate reciprocal (1 unit in the last place), of an
         // update that is itself a small part of p.  The divisor is zero or a normal number: sqrt of the smallest fp32 is 2^-74.5.
-        float inverse;
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(fmaf(root[h][j], inv_sqrt_bc2, q.eps)));
-        p[j] = p[j] * decay - m[j] * inverse * step_size;
+        float d0, d1;
+        unpack_f32x2(fma_f32x2(pack_f32x2(root[h][2 * j], root[h][2 * j + 1]), k_bc2, k_eps), d0, d1);
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d0) : "f"(d0));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d1) : "f"(d1));
+        const uint64_t update = mul_f32x2(m2[j], pack_f32x2(d0, d1));
+        unpack_f32x2(fma_f32x2(update, k_step, mul_f32x2(pack_f32x2(p[2 * j], p[2 * j + 1]), k_decay)), p[2 * j], p[2 * j + 1]);
+        unpack_f32x2(m2[j], m[2 * j], m[2 * j + 1]);
+        unpack_f32x2(v2[j], v[2 * j], v[2 * j + 1]);
+        m1[h][2 * j] = m[2 * j];
+        m1[h][2 * j + 1] = m[2 * j + 1];
       }
       if (BITS == 8) {                     // behind the tensor's end all of it is zero
         peak_m = max_nan(max_nan(peak_m, fabsf(m[0]), fabsf(m[1])), fabsf(m[2]), fabsf(m[3]));
@@ -370,11 +404,11 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const __grid_const
         const int64_t i = base + h * 128 + lane * 4;
         uint32_t hash[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) hash[j] = mix32(static_cast<uint32_t>(i) + j + salt);
+        for (int j = 0; j < 4; ++j) hash[j] = mix32(static_cast<uint32_t>(i) + j + salt, q.two16);
         // behind the tensor's end the codes are those of zero
         *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.m) + i) =
-            peak_m == 0.f && finite_m ? 0u : encode4<3>(m1[h], inv_m, hash, finite_m) | signs4(m1[h]);
-        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.v) + i) = peak_r == 0.f && finite_r ? 0u : encode4<4>(root[h], inv_r, hash, finite_r);
+            peak_m == 0.f && finite_m ? 0u : encode4<3>(m1[h], inv_m, hash, q.two4, finite_m);
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.v) + i) = peak_r == 0.f && finite_r ? 0u : encode4<4>(root[h], inv_r, hash, q.two5, finite_r);
       }
       if (lane == 0) {
         t.m_scale[block] = scale_of(exp_m);
@@ -410,8 +444,14 @@ __global__ void __launch_bounds__(256) adamw_moments_kernel(const uint8_t* __res
   if (i >= n4) return;
   const int64_t block = i / (ADAMW_BLOCK / 4);
   float fm[4], fr[4];
-  decode4<3>(reinterpret_cast<const uint32_t*>(m)[i], m_scale[block], fm);
-  decode4<4>(reinterpret_cast<const uint32_t*>(r)[i], r_scale[block], fr);
+  decode4<3>(reinterpret_cast<const uint32_t*>(m)[i], 1u << 20, fm);
+  decode4<4>(reinterpret_cast<const uint32_t*>(r)[i], 1u << 19, fr);
+  const float sm = m_scale[block], sr = r_scale[block];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    fm[j] = __fmul_rn(fm[j], sm);
+    fr[j] = __fmul_rn(fr[j], sr);
+  }
   const float4 a = make_float4(fm[0], fm[1], fm[2], fm[3]);
   const float4 b = make_float4(__fmul_rn(fr[0], fr[0]), __fmul_rn(fr[1], fr[1]), __fmul_rn(fr[2], fr[2]), __fmul_rn(fr[3], fr[3]));
   reinterpret_cast<float4*>(m_out)[i] = a;
@@ -505,6 +545,11 @@ int adamw(const AdamwArgs& a, cudaStream_t stream) {
   q.eps = static_cast<float>(a.eps);
   q.grad_scale = a.grad_scale;
   q.seed = a.seed;
+  q.two4 = 1u << 4;
+  q.two5 = 1u << 5;
+  q.two16 = 1u << 16;
+  q.two19 = 1u << 19;
+  q.two20 = 1u << 20;
   q.advance = a.advance;
   if (a.dtype == B200K_DTYPE_F32) return adamw_bits<float, float, false>(a.tensors, a.n, a.state_bits, q, stream);
   if (a.dtype == B200K_DTYPE_BF16) return adamw_16bit<__nv_bfloat16>(a.tensors, a.n, a.gdtype, master, a.state_bits, q, stream);
