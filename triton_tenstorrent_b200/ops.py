@@ -539,6 +539,8 @@ _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch
 def _rows_of(t: torch.Tensor) -> torch.Tensor:
     """The [rows, last dimension] view of t with unit inner stride; a copy where t's strides have no such view."""
     n = t.shape[-1]
+    if t.dim() == 2 and (n < 2 or t.stride(1) == 1):
+        return t
     if t.dim() == 1:
         t = t.unsqueeze(0)
     if t.numel() == 0:
@@ -577,26 +579,43 @@ def _norm_input(name, x):
         raise ValueError(f"{name}: the last dimension must have at least one element, got shape {tuple(x.shape)}")
 
 
-def layer_norm_with_stats(x, weight=None, bias=None, eps: float = 1e-5):
-    """Returns (y, mean, rstd): the layer norm of x over its last dimension and the fp32 row statistics (x's shape without its last
-    dimension) that layer_norm_backward takes."""
+def _layer_norm_call(x, weight, bias, eps, stats):
+    """y of layer_norm; `stats` (fp32 [2, rows] on the device, or None) receives the row statistics."""
+    w, b = weight, bias
+    if not x.is_cuda:
+        w, b = (None if t is None else _to_device(t) for t in (w, b))
+    xd = _rows_of(_to_device(x))
+    rows, cols = xd.shape
+    y = torch.empty(x.shape, device=xd.device, dtype=x.dtype)
+    w = None if w is None else w if w.is_contiguous() else w.contiguous()
+    b = None if b is None else b if b.is_contiguous() else b.contiguous()
+    wdtype = _DTYPES[(w if w is not None else b if b is not None else xd).dtype]
+    mean = 0 if stats is None else stats.data_ptr()
+    with _on(xd.device):
+        _lib.check(_lib.load().b200k_layer_norm_fwd(xd.data_ptr(), 0 if w is None else w.data_ptr(), 0 if b is None else b.data_ptr(), y.data_ptr(),
+                                                    mean, mean and mean + 4 * rows, rows, cols, _pitch(xd), cols, _DTYPES[x.dtype], wdtype, eps,
+                                                    _stream()))
+    return y
+
+
+def _layer_norm_check(x, weight, bias, eps):
     _norm_input("layer_norm", x)
     if not eps >= 0:
         raise ValueError(f"layer_norm: eps must be >= 0, got {eps}")
-    w = _norm_weight("weight", x, weight)
-    b = _norm_weight("bias", x, bias, weight)
-    lib = _lib.load()
-    w, b = (None if t is None else _to_device(t).contiguous() for t in (w, b))
-    xd = _rows_of(_to_device(x))
-    rows, cols = xd.shape
-    y = torch.empty((rows, cols), device=xd.device, dtype=x.dtype)
-    stats = torch.empty((2, rows), device=xd.device, dtype=torch.float32)
-    wdtype = _DTYPES[(w if w is not None else b if b is not None else xd).dtype]
-    with _on(xd.device):
-        _lib.check(lib.b200k_layer_norm_fwd(xd.data_ptr(), 0 if w is None else w.data_ptr(), 0 if b is None else b.data_ptr(), y.data_ptr(),
-                                            stats.data_ptr(), stats.data_ptr() + 4 * rows, rows, cols, _pitch(xd), cols, _DTYPES[x.dtype],
-                                            wdtype, float(eps), _stream()))
-    return (_like_input(y.view(x.shape), x), _like_input(stats[0].view(x.shape[:-1]), x), _like_input(stats[1].view(x.shape[:-1]), x))
+    _norm_weight("weight", x, weight)
+    _norm_weight("bias", x, bias, weight)
+
+
+def layer_norm_with_stats(x, weight=None, bias=None, eps: float = 1e-5):
+    """Returns (y, mean, rstd): the layer norm of x over its last dimension and the fp32 row statistics (x's shape without its last
+    dimension) that layer_norm_backward takes."""
+    _layer_norm_check(x, weight, bias, eps)
+    if not x.is_cuda:
+        _require_cuda()
+    stats = torch.empty((2, *x.shape[:-1]), device=x.device if x.is_cuda else "cuda", dtype=torch.float32)
+    y = _layer_norm_call(x, weight, bias, eps, stats)
+    mean, rstd = stats.unbind(0)
+    return _like_input(y, x), _like_input(mean, x), _like_input(rstd, x)
 
 
 def layer_norm_backward(dy, x, weight, mean, rstd, need_dx: bool = True, need_dw: bool = True, need_db: bool = True):
@@ -653,9 +672,10 @@ class _layer_norm(torch.autograd.Function):
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5) -> torch.Tensor:
     """y = (x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x (fp32, bf16 or fp16; weight and bias in x's type or in
     fp32, either may be None).  fp32 arithmetic, one rounding; differentiable in x, weight and bias."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         return _layer_norm.apply(x, weight, bias, eps)
-    return layer_norm_with_stats(x, weight, bias, eps)[0]
+    _layer_norm_check(x, weight, bias, eps)
+    return _like_input(_layer_norm_call(x, weight, bias, eps, None), x)
 
 
 _REDUCTIONS = {"none": _lib.REDUCE_NONE, "mean": _lib.REDUCE_MEAN, "sum": _lib.REDUCE_SUM}

@@ -89,6 +89,7 @@ class AdamW:
         table[:, _N] = [p.numel() for p in self.params]
         table[:, _INDEX] = np.arange(len(self.params))
         self._table = table
+        self._shapes, self._empty = [p.shape for p in self.params], [p.numel() == 0 for p in self.params]
 
     def _check_hyper(self):
         if isinstance(self.lr, torch.Tensor):
@@ -126,13 +127,12 @@ class AdamW:
         for p in self.params:
             p.grad = None
 
-    @torch.no_grad()
     def step(self, grads=None, grad_scale=1.0):
         """One update.  grads: one gradient per parameter in the parameter's type or in fp32, or None for a parameter that is left
         alone (with its moments) in this step; by default the parameters' .grad.  grad_scale multiplies every gradient: a number, or
         an fp32 CUDA tensor of one element (loss scaling, clipping by a norm)."""
         params = self.params
-        grads = [p.grad for p in params] if grads is None else list(grads)
+        grads = [p.grad for p in params] if grads is None else grads
         if len(grads) != len(params):
             raise ValueError(f"AdamW: {len(params)} gradients expected, got {len(grads)}")
         self._check_hyper()
@@ -148,32 +148,39 @@ class AdamW:
             if lr.device != self.device:
                 raise ValueError(f"AdamW: lr must be on {self.device}")
             lr, lr_ptr = 0.0, lr.data_ptr()
-        groups = {}
-        for i, (p, g) in enumerate(zip(params, grads)):
-            if g is None or p.numel() == 0:
+        rows, kinds, changed = [], [], False
+        at, strided = self.device.index, torch.strided
+        for i, (p, g, shape) in enumerate(zip(params, grads, self._shapes)):
+            if g is None or self._empty[i]:
                 continue
-            if g.dtype != p.dtype and g.dtype != torch.float32:
-                raise TypeError(f"AdamW: gradient {i} must be {p.dtype} or torch.float32, got {g.dtype}")
-            if g.shape != p.shape or g.device != self.device or g.layout != torch.strided:
-                raise ValueError(f"AdamW: gradient {i} must be a dense {tuple(p.shape)} tensor on {self.device}, got {tuple(g.shape)} on {g.device}")
-            if not p.is_contiguous() or p.device != self.device:
-                raise ValueError(f"AdamW: parameter {i} is no longer contiguous on {self.device}")
+            dtype, gdtype = p.dtype, g.dtype
+            if gdtype is not dtype and gdtype is not torch.float32:
+                raise TypeError(f"AdamW: gradient {i} must be {dtype} or torch.float32, got {gdtype}")
+            if g.shape != shape or g.get_device() != at or g.layout is not strided:
+                raise ValueError(f"AdamW: gradient {i} must be a dense {tuple(shape)} tensor on {self.device}, got {tuple(g.shape)} on {g.device}")
+            if p.shape != shape or not p.is_contiguous() or p.get_device() != at:
+                raise ValueError(f"AdamW: parameter {i} is no longer a contiguous {tuple(shape)} tensor on {self.device}")
             if not g.is_contiguous():
-                g = grads[i] = g.contiguous()
-            groups.setdefault((p.dtype, g.dtype), []).append(i)
-        if not groups:
+                g = g.contiguous()
+                if not changed:
+                    grads, changed = list(grads), True
+                grads[i] = g            # holds the copy until the launch
+            rows.append((i, p.data_ptr(), g.data_ptr()))
+            kinds.append((dtype, gdtype))
+        if not rows:
             return
         entry = _lib.load().b200k_adamw
         b1, b2 = self.betas
-        table = self._table
+        order = list(dict.fromkeys(kinds))
         with _on(self.device):
             stream = _stream()
-            for k, ((dtype, gdtype), at) in enumerate(groups.items()):
-                rows = table[at] if len(at) < len(params) else table
-                rows[:, _P] = [params[i].data_ptr() for i in at]
-                rows[:, _G] = [grads[i].data_ptr() for i in at]
-                _lib.check(entry(rows.ctypes.data, len(at), _DTYPES[dtype], _DTYPES[gdtype], self.state_bits, self._state.data_ptr(), lr, lr_ptr,
-                                 b1, b2, self.eps, self.weight_decay, scale, scale_ptr, self.seed, int(k == len(groups) - 1), stream))
+            for k, kind in enumerate(order):
+                mine = rows if len(order) == 1 else [r for r, x in zip(rows, kinds) if x == kind]
+                pointers = np.array(mine, dtype=np.int64)
+                table = self._table if len(mine) == len(params) else self._table[pointers[:, 0]]
+                table[:, _P:_G + 1] = pointers[:, 1:]
+                _lib.check(entry(table.ctypes.data, len(mine), _DTYPES[kind[0]], _DTYPES[kind[1]], self.state_bits, self._state.data_ptr(), lr, lr_ptr,
+                                 b1, b2, self.eps, self.weight_decay, scale, scale_ptr, self.seed, int(k == len(order) - 1), stream))
 
     def state_dict(self) -> dict:
         """The state as tensors (copies): step, the moments as they are held, and the master copy."""
