@@ -51,7 +51,10 @@ struct LceGemmParams {
   int f16;
   uint32_t idesc, idesc_half;
   uint32_t* status;
+  float log2e;             // STATS, DLOGITS: lce_log2e(K)
   const int* target;       // per row that counts: its target (STATS, DLOGITS)
+  const int64_t* token_target;   // STATS without a gather: per token
+  int width;               // STATS on single CTAs: columns of a tile
   int col_base;            // first vocabulary entry of the piece
   float2* part;            // STATS: [tile column][rows] (maximum * log2 e, sum of exponentials)
   int64_t part_ld;
@@ -60,28 +63,51 @@ struct LceGemmParams {
   const float* row_scale;  // DLOGITS: factor of the row
   const float* alpha;      // DW, DH: factor of the result (device memory)
   const float* add;        // DH: fp32 sum over the earlier pieces, or null
-  float* sum;              // DH: where the sum so far goes, or null for the last piece
-  void* out;               // DH, last piece: dh
+  float* sum;              // DH: where the sum so far goes, max_splits buffers split_stride apart
+  int64_t split_stride;
+  int max_splits, last;    // DH: last = the last piece
+  void* out;               // DH, last piece without splits: dh
   const int* token;        // DH: token of a row
 };
 
+// log2 e, corrected for what the tensor cores lose: each step of 16 along K truncates the running sum towards zero, which takes 2^-25 of it on
+// average, and the running sum is on average the final one times the part of K done, so that a logit comes out K / 16 * 2^-26 of itself too small.
+// (Measured on 2048 x 128000 logits: 8.3e-7, 3.85e-6 and 7.67e-6 at K = 1024, 4096 and 8192; 9.5e-7, 3.8e-6 and 7.6e-6 by the formula.  Without the
+// correction the mean loss is 1.2e-6 off at K = 4096.)
+__host__ __device__ inline float lce_log2e(int K) { return static_cast<float>(1.4426950408889634 * (1.0 + (K + 15) / 16 * 0x1p-26)); }
+
+// Parts that the K axis of the dh product is cut in: with fewer tiles than CTA pairs, or a last wave that is nearly empty, the parts of a tile go to
+// different pairs, which leave fp32 sums that lce_dh_kernel adds.  Cost of s parts, in steps of 64 along K (0.28 us): waves of K / s steps, about 8
+// steps for filling the pipeline and the epilogue of each, and a part's sums written and read (a tile: 0.3 steps of all pairs).  Cutting at all
+// has to gain 3 %.  The whole warp calls it, a lane per s.
+constexpr int LCE_MAX_SPLITS = 32;
+__device__ __forceinline__ int lce_splits(int tiles, int pairs, int num_kb, int max_splits) {
+  if (max_splits <= 1) return 1;
+  const int s = static_cast<int>(lane_id()) + 1;
+  auto cost = [&](int parts) { return static_cast<int64_t>((tiles * parts + pairs - 1) / pairs) * ((num_kb + parts - 1) / parts + 8); };
+  const int64_t c = s == 1 ? cost(1) : cost(s) + cost(1) / 32 + static_cast<int64_t>(tiles) * s * 5 / 16;
+  const uint32_t key = s > max_splits ? 0xFFFFFFFFu : static_cast<uint32_t>(min(c, static_cast<int64_t>((1 << 27) - 1))) << 5 | static_cast<uint32_t>(s - 1);
+  return static_cast<int>(__reduce_min_sync(0xFFFFFFFFu, key) & 31u) + 1;
+}
+
 struct LceWork {
-  int pid_m, pid_n, col0, width;
+  int pid_m, pid_n, col0, width, split;
 };
 struct LceSchedule {
-  int num_pid_m, num_pid_n, group_m, full_work, num_work;
+  int num_pid_m, num_pid_n, group_m, full_work, num_work, splits;
 };
 // Tiles in groups of group_m rows, odd groups backwards; the tiles of a last wave that occupy at most half of the pairs are cut in two column
 // halves (the order and the split of the matmul kernel).
-__device__ __forceinline__ LceSchedule lce_schedule(int M, int N, int group_m, int pairs) {
+__device__ __forceinline__ LceSchedule lce_schedule(int M, int N, int group_m, int pairs, int splits) {
   LceSchedule s;
   s.num_pid_m = (M + 255) >> 8;
   s.num_pid_n = (N + 255) >> 8;
   s.group_m = group_m;
+  s.splits = splits;
   const int tiles = s.num_pid_m * s.num_pid_n;
   const int rest = tiles % pairs;
-  s.full_work = s.num_work = tiles;
-  if (rest > 0 && 2 * rest <= pairs) {
+  s.full_work = s.num_work = tiles * splits;
+  if (splits == 1 && rest > 0 && 2 * rest <= pairs) {
     s.full_work = tiles - rest;
     s.num_work = tiles + rest;
   }
@@ -91,7 +117,12 @@ __device__ __forceinline__ LceWork lce_work(const LceSchedule& s, int w) {
   LceWork r;
   int tile = w, half = 0;
   r.width = 256;
-  if (w >= s.full_work) {
+  r.split = 0;
+  if (s.splits > 1) {                  // the tiles of one part of K after the other
+    const int tiles = s.num_pid_m * s.num_pid_n;
+    r.split = w / tiles;
+    tile = w - r.split * tiles;
+  } else if (w >= s.full_work) {
     tile = s.full_work + ((w - s.full_work) >> 1);
     half = (w - s.full_work) & 1;
     r.width = 128;
@@ -130,6 +161,42 @@ __device__ __forceinline__ void lce_store_chunk(const CUtensorMap* map, const fl
   }
   buf ^= 1;
 }
+
+// 64 columns of a row of logits into its running maximum (in units of log2) and sum of 2^(x - maximum); `in`: the target's place among them, `limit`:
+// the first column that does not count.
+__device__ __forceinline__ void lce_stats_chunk(float (&f)[64], int in, int col0, int limit, float log2e, float* target_logit, float& run_max,
+                                                float& run_sum) {
+  if (in >= 0 && in < 64 && col0 + in < limit) {
+    float t = 0.f;
+#pragma unroll
+    for (int j = 0; j < 64; ++j) t = j == in ? f[j] : t;
+    *target_logit = t;
+  }
+  if (col0 + 64 > limit) {
+#pragma unroll
+    for (int j = 0; j < 64; ++j) f[j] = col0 + j < limit ? f[j] : -INFINITY;
+  }
+  float m = f[0];
+#pragma unroll
+  for (int j = 1; j < 63; j += 2) m = fmax3(m, f[j], f[j + 1]);
+  m = fmaxf(m, f[63]);
+  const float new_max = fmaxf(run_max, m * log2e);
+  const float shift = new_max == -INFINITY ? 0.f : new_max;     // a row of -inf: the sum stays 0
+  float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll
+  for (int j = 0; j < 64; j += 4) {
+    s0 += exp2f(fmaf(f[j], log2e, -shift));
+    s1 += exp2f(fmaf(f[j + 1], log2e, -shift));
+    s2 += exp2f(fmaf(f[j + 2], log2e, -shift));
+    s3 += exp2f(fmaf(f[j + 3], log2e, -shift));
+  }
+  run_sum = fmaf(run_sum, exp2f(run_max - shift), (s0 + s1) + (s2 + s3));
+  run_max = new_max;
+}
+
+// A target as the kernels compare it with columns: outside the vocabulary, or ignored, it matches none.
+constexpr int LCE_NO_TARGET = -(1 << 29);
+__device__ __forceinline__ int lce_target(int64_t y, int V) { return y >= 0 && y < V ? static_cast<int>(y) : LCE_NO_TARGET; }
 
 // A_MN / B_MN: the operand's tile is contiguous along M / N in memory (else along K).
 template <int EPI, bool A_MN, bool B_MN>
@@ -181,10 +248,14 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   tc_fence_after();
   const uint32_t tmem_base = *tmem_ptr_smem;
 
-  const int count = *p.count;
+  const int count = p.count != nullptr ? *p.count : p.M;
   const int M = EPI == LCE_DW ? p.M : count;
   const int num_kb = ((EPI == LCE_DW ? count : p.K) + 63) >> 6;
-  const LceSchedule sched = lce_schedule(M, p.N, p.group_m, num_pairs);
+  const int splits = EPI == LCE_DH ? lce_splits(((M + 255) >> 8) * ((p.N + 255) >> 8), num_pairs, num_kb, p.max_splits) : 1;
+  const LceSchedule sched = lce_schedule(M, p.N, p.group_m, num_pairs, splits);
+  // the steps along K of a work item
+  auto kb_begin = [&](const LceWork& wk) { return EPI == LCE_DH ? static_cast<int>(static_cast<int64_t>(num_kb) * wk.split / splits) : 0; };
+  auto kb_end = [&](const LceWork& wk) { return EPI == LCE_DH ? static_cast<int>(static_cast<int64_t>(num_kb) * (wk.split + 1) / splits) : num_kb; };
 
   if (warp_idx == 0) {
     // ---------------------------------------------------------------- TMA producer (both CTAs)
@@ -198,7 +269,8 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       const int m0 = wk.pid_m * 256 + static_cast<int>(rank) * 128;
       const int n0 = wk.col0 + static_cast<int>(rank) * (wk.width / 2);
       const int b_boxes = wk.width / 128;
-      for (int kb = 0; kb < num_kb; ++kb) {
+      const int kb1 = kb_end(wk);
+      for (int kb = kb_begin(wk); kb < kb1; ++kb) {
         ok = mbar_wait(&empty_bar[stage], phase ^ 1u, ctx, 61);
         if (!ok) break;
         if (lane == 0) {
@@ -230,7 +302,13 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         if (!ok) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * 256;
-        for (int kb = 0; kb < num_kb; ++kb) {
+        int kb0 = 0, kb1 = num_kb;
+        if (EPI == LCE_DH) {
+          const LceWork wk = lce_work(sched, work);
+          kb0 = kb_begin(wk);
+          kb1 = kb_end(wk);
+        }
+        for (int kb = kb0; kb < kb1; ++kb) {
           ok = mbar_wait(&full_bar[stage], phase, ctx, 63);
           if (!ok) break;
           tc_fence_after();
@@ -242,12 +320,12 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
               // K-major: a k step is 32 bytes along the 128-byte rows; M/N-major: 16 rows down, 64-wide chunks one box apart
               const uint64_t a_desc = umma_smem_desc_sw128(a_addr + k * (A_MN ? 2048 : 32), A_MN ? LCE_BOX_BYTES : 16, 1024);
               const uint64_t b_desc = umma_smem_desc_sw128(b_addr + k * (B_MN ? 2048 : 32), B_MN ? LCE_BOX_BYTES : 16, 1024);
-              umma_ss_2cta(d_tmem, a_desc, b_desc, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+              umma_ss_2cta(d_tmem, a_desc, b_desc, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
             }
             const uint32_t e = smem_u32(&empty_bar[stage]);
             umma_commit_2cta(mapa_shared(e, 0));
             umma_commit_2cta(mapa_shared(e, 1));
-            if (kb == num_kb - 1) {
+            if (kb == kb1 - 1) {
               const uint32_t f = smem_u32(&tmem_full_bar[acc]);
               umma_commit_2cta(mapa_shared(f, 0));
               umma_commit_2cta(mapa_shared(f, 1));
@@ -276,7 +354,9 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       // what the row needs, fetched while the main loop still runs
       int target = -1, token = 0;
       float lse2 = 0.f, scale = 0.f;
-      if (EPI == LCE_STATS || EPI == LCE_DLOGITS) target = live ? p.target[row] - p.col_base - wk.col0 : -1;
+      if (EPI == LCE_STATS || EPI == LCE_DLOGITS) {
+        if (live) target = (EPI == LCE_STATS && p.token_target != nullptr ? lce_target(p.token_target[row], p.N) : p.target[row]) - p.col_base - wk.col0;
+      }
       if (EPI == LCE_DLOGITS && live) {
         lse2 = p.lse2[row];
         scale = p.row_scale[row];
@@ -313,36 +393,11 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         const int col0 = wk.col0 + c * 64;
         const int in = target - c * 64;              // the target's place in this chunk
         if constexpr (EPI == LCE_STATS) {
-          if (in >= 0 && in < 64 && col0 + in < p.N) {
-            float t = 0.f;
-#pragma unroll
-            for (int j = 0; j < 64; ++j) t = j == in ? f[j] : t;
-            p.target_logit[row] = t;
-          }
-          if (col0 + 64 > p.N) {
-#pragma unroll
-            for (int j = 0; j < 64; ++j) f[j] = col0 + j < p.N ? f[j] : -INFINITY;
-          }
-          float m = f[0];
-#pragma unroll
-          for (int j = 1; j < 63; j += 2) m = fmax3(m, f[j], f[j + 1]);
-          m = fmaxf(m, f[63]);
-          const float new_max = fmaxf(run_max, m * LOG2E);
-          const float shift = new_max == -INFINITY ? 0.f : new_max;     // a row of -inf: the sum stays 0
-          float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-#pragma unroll
-          for (int j = 0; j < 64; j += 4) {
-            s0 += exp2f(fmaf(f[j], LOG2E, -shift));
-            s1 += exp2f(fmaf(f[j + 1], LOG2E, -shift));
-            s2 += exp2f(fmaf(f[j + 2], LOG2E, -shift));
-            s3 += exp2f(fmaf(f[j + 3], LOG2E, -shift));
-          }
-          run_sum = fmaf(run_sum, exp2f(run_max - shift), (s0 + s1) + (s2 + s3));
-          run_max = new_max;
+          lce_stats_chunk(f, in, col0, p.N, p.log2e, p.target_logit + row, run_max, run_sum);
         } else if constexpr (EPI == LCE_DLOGITS) {
 #pragma unroll
           for (int j = 0; j < 64; ++j) {
-            const float e = exp2f(fmaf(f[j], LOG2E, -lse2)) - (j == in ? 1.f : 0.f);
+            const float e = exp2f(fmaf(f[j], p.log2e, -lse2)) - (j == in ? 1.f : 0.f);
             f[j] = live ? e * scale : 0.f;           // rows behind the last one that counts: zeros, for the K tail of dW
           }
           if (col0 + 64 > p.N) {                       // columns behind the piece: zeros, for the K tail of dh
@@ -358,7 +413,7 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
           // K (= D) is a multiple of 8, so a row of the result ends on a multiple of 8 columns
           if (live) {
             const int cols = min(64, p.N - col0);
-            const int64_t at = static_cast<int64_t>(row) * p.N + col0;
+            const int64_t at = wk.split * p.split_stride + static_cast<int64_t>(row) * p.N + col0;
             if (p.add != nullptr) {
 #pragma unroll
               for (int j = 0; j < 64; j += 4)
@@ -367,7 +422,7 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                   f[j] += a.x; f[j + 1] += a.y; f[j + 2] += a.z; f[j + 3] += a.w;
                 }
             }
-            if (p.sum != nullptr) {
+            if (splits > 1 || !p.last) {
 #pragma unroll
               for (int j = 0; j < 64; j += 4)
                 if (j < cols) *reinterpret_cast<float4*>(p.sum + at + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
@@ -405,9 +460,156 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 }
 
 // ---------------------------------------------------------------------------------------------
+// The statistics of at most 128 tokens: single CTAs (M = 128), one wave or more of tiles of `width` columns, chosen so that every SM gets the same
+// number (lce_narrow_width).  The bound is the stream of W, which the pairs' 256-column tiles would spread unevenly over the SMs (61 tokens, 32000
+// entries: 125 tiles on 74 pairs, 24 us).  The tokens are read where they are: with one tile row nothing is gained by leaving some out.
+// ---------------------------------------------------------------------------------------------
+constexpr int LCE1_STAGES = 4;
+constexpr int LCE1_A_BYTES = 128 * 128, LCE1_B_BYTES = 256 * 128;
+constexpr int LCE1_BAR_OFF = LCE1_STAGES * (LCE1_A_BYTES + LCE1_B_BYTES);
+constexpr int LCE1_SMEM = LCE1_BAR_OFF + (2 * LCE1_STAGES + 4) * 8 + 16 + 1024;
+static_assert(LCE1_SMEM <= 232448, "shared memory budget exceeded");
+
+static int lce_narrow_width(int V, int sms) {
+  const int64_t waves = (V + 256ll * sms - 1) / (256ll * sms);
+  const int64_t width = (V + waves * sms - 1) / (waves * sms);
+  return static_cast<int>((width + 15) / 16 * 16);
+}
+
+__global__ void __launch_bounds__(LCE_THREADS, 1)
+lce_stats_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const LceGemmParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smem_a = smem;
+  uint8_t* smem_b = smem + LCE1_STAGES * LCE1_A_BYTES;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + LCE1_BAR_OFF);
+  uint64_t* empty_bar = full_bar + LCE1_STAGES;
+  uint64_t* tmem_full_bar = empty_bar + LCE1_STAGES;
+  uint64_t* tmem_empty_bar = tmem_full_bar + 2;
+  uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(tmem_empty_bar + 2);
+  uint32_t* abort_smem = tmem_ptr_smem + 1;
+  const int warp_idx = threadIdx.x >> 5;
+  const uint32_t lane = lane_id();
+  WaitCtx ctx{abort_smem, p.status};
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < LCE1_STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tmem_full_bar[a], 1);
+      mbar_init(&tmem_empty_bar[a], LCE_EPI_WARPS);
+    }
+    *abort_smem = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tmap_a);
+    prefetch_tmap(&tmap_b);
+  }
+  if (warp_idx == 1) {
+    tmem_alloc(tmem_ptr_smem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_ptr_smem;
+  const int num_kb = (p.K + 63) >> 6;
+  const int tiles = (p.N + p.width - 1) / p.width;
+
+  if (warp_idx == 0) {
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x)
+      for (int kb = 0; kb < num_kb; ++kb) {
+        ok = mbar_wait(&empty_bar[stage], phase ^ 1u, ctx, 65);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_expect_tx(&full_bar[stage], LCE1_A_BYTES + p.width * 128);
+          tma_load_2d(smem_a + stage * LCE1_A_BYTES, &tmap_a, &full_bar[stage], kb * 64, 0);
+          tma_load_2d(smem_b + stage * LCE1_B_BYTES, &tmap_b, &full_bar[stage], kb * 64, tile * p.width);
+        }
+        __syncwarp();
+        if (++stage == LCE1_STAGES) { stage = 0; phase ^= 1u; }
+      }
+  } else if (warp_idx == 1) {
+    int stage = 0, it = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++it) {
+      const int acc = it & 1;
+      ok = mbar_wait(&tmem_empty_bar[acc], ((it >> 1) & 1) ^ 1u, ctx, 66);
+      if (!ok) break;
+      tc_fence_after();
+      for (int kb = 0; kb < num_kb; ++kb) {
+        ok = mbar_wait(&full_bar[stage], phase, ctx, 67);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t a_addr = smem_u32(smem_a + stage * LCE1_A_BYTES), b_addr = smem_u32(smem_b + stage * LCE1_B_BYTES);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_ss(tmem_base + acc * 256, umma_smem_desc_sw128(a_addr + k * 32, 16, 1024), umma_smem_desc_sw128(b_addr + k * 32, 16, 1024), p.idesc,
+                    (kb > 0 || k > 0) ? 1u : 0u);
+          umma_commit(&empty_bar[stage]);
+          if (kb == num_kb - 1) umma_commit(&tmem_full_bar[acc]);
+        }
+        __syncwarp();
+        if (++stage == LCE1_STAGES) { stage = 0; phase ^= 1u; }
+      }
+    }
+  } else {
+    const int q = warp_idx & 3;
+    const int row = q * 32 + static_cast<int>(lane);
+    const bool live = row < p.M;
+    const int target = live ? lce_target(p.token_target[row], p.N) : LCE_NO_TARGET;
+    int it = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++it) {
+      const int acc = it & 1;
+      const int first = tile * p.width, limit = min(p.N, first + p.width);
+      float run_max = -INFINITY, run_sum = 0.f;
+      ok = mbar_wait(&tmem_full_bar[acc], (it >> 1) & 1, ctx, 68);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * 256;
+      const int chunks = (p.width + 63) >> 6;
+#pragma unroll 1
+      for (int c = 0; c < chunks; ++c) {
+        uint32_t v0[32], v1[32];
+        tmem_ld_x32(t_row + c * 64, v0);
+        tmem_ld_x32(t_row + c * 64 + 32, v1);
+        tmem_wait_ld();
+        if (c == chunks - 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&tmem_empty_bar[acc]);
+        }
+        float f[64];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          f[j] = __uint_as_float(v0[j]);
+          f[32 + j] = __uint_as_float(v1[j]);
+        }
+        const int col0 = first + c * 64;
+        lce_stats_chunk(f, target - col0, col0, limit, p.log2e, p.target_logit + row, run_max, run_sum);
+      }
+      if (live) p.part[static_cast<int64_t>(tile) * p.part_ld + row] = make_float2(run_max, run_sum);
+    }
+  }
+  drain_after_abort(abort_smem);
+  tc_fence_before();
+  __syncthreads();
+  if (warp_idx == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
 // Gather: the rows that count move to the front of `hc`, in order; the other rows of `hc` become zeros.
 // ---------------------------------------------------------------------------------------------
-constexpr int LCE_GATHER_ROWS = 32;
+constexpr int LCE_GATHER_ROWS = 8;      // a warp per row
 
 struct LceGatherParams {
   const uint4* h;
@@ -415,6 +617,7 @@ struct LceGatherParams {
   const int64_t* target;
   int64_t ignore;
   int T, D8, V;            // D8: 16-byte units of a row
+  int cta_rows;            // rows of a CTA, a multiple of LCE_GATHER_ROWS
   uint4* hc;
   int* count;
   int* token;
@@ -438,69 +641,76 @@ struct LceGatherParams {
 template <bool BACKWARD>
 __global__ void __launch_bounds__(256) lce_gather_kernel(const LceGatherParams p) {
   __shared__ int warp_counts[8];
-  __shared__ int place[LCE_GATHER_ROWS];       // row of hc; valid ones >= 0, others -1 - row
-  __shared__ int total_smem;
+  __shared__ int place[LCE_GATHER_ROWS];       // row of hc; that of a row that does not count as -1 - row
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int first = blockIdx.x * LCE_GATHER_ROWS;
-  const bool last_cta = blockIdx.x == gridDim.x - 1;
+  const int first = blockIdx.x * p.cta_rows, end = min(p.T, first + p.cta_rows);
   // tokens that count before this CTA's rows
   int n = 0;
+#pragma unroll 4
   for (int i = threadIdx.x; i < first; i += 256) n += p.target[i] != p.ignore ? 1 : 0;
   n = __reduce_add_sync(0xFFFFFFFFu, n);
   if (lane == 0) warp_counts[warp] = n;
   __syncthreads();
-  if (warp == 0) {
-    int before = __reduce_add_sync(0xFFFFFFFFu, lane < 8 ? warp_counts[lane] : 0);
-    const int t = first + lane;
-    const int64_t y = t < p.T ? p.target[t] : p.ignore;
-    const bool counts = t < p.T && y != p.ignore;
-    const unsigned mask = __ballot_sync(0xFFFFFFFFu, counts);
-    const int at = before + __popc(mask & ((1u << lane) - 1u));   // rows that count before this one
-    if (t < p.T) {
-      const int row = counts ? at : p.T - 1 - (t - at);           // the k-th row that does not count takes the k-th place from the back
-      place[lane] = counts ? row : -1 - row;
-      const bool valid = y >= 0 && y < p.V;
-      p.row_target[row] = counts && valid ? static_cast<int>(y) : -(1 << 29);   // matches no column
-      p.token[row] = t;
-      if (BACKWARD) {
-        p.row_lse2[row] = counts ? p.lse_in[t] * LOG2E : 0.f;
-        float g = 1.f;
-        if (p.gmax != nullptr) {
-          const float m = *p.gmax;
-          g = m > 0.f ? p.d_loss[t] / m : p.d_loss[t];
-        }
-        // a target outside the vocabulary: NaN, in the loss and in every gradient that it enters
-        p.row_scale[row] = counts ? (valid ? g * p.unit : __int_as_float(0x7FC00000)) : 0.f;
-      } else {
-        p.target_logit[row] = __int_as_float(0x7FC00000);         // the product's epilogue puts the logit here
-        if (!counts) {
+  int before = 0;
+  if (warp == 0) before = __reduce_add_sync(0xFFFFFFFFu, lane < 8 ? warp_counts[lane] : 0);
+  for (int top = first; top < end; top += LCE_GATHER_ROWS) {
+    if (warp == 0) {
+      const int t = top + lane;
+      const bool mine = lane < LCE_GATHER_ROWS && t < end;
+      const int64_t y = mine ? p.target[t] : p.ignore;
+      const bool counts = y != p.ignore;
+      const unsigned mask = __ballot_sync(0xFFFFFFFFu, counts);
+      const int at = before + __popc(mask & ((1u << lane) - 1u));   // rows that count before this one
+      if (mine) {
+        const int row = counts ? at : p.T - 1 - (t - at);           // the k-th row that does not count takes the k-th place from the back
+        place[lane] = counts ? row : -1 - row;
+        const int column = lce_target(y, p.V);
+        const bool valid = column != LCE_NO_TARGET;
+        p.row_target[row] = counts ? column : LCE_NO_TARGET;
+        p.token[row] = t;
+        if (BACKWARD) {
+          p.row_lse2[row] = counts ? p.lse_in[t] * LOG2E : 0.f;
+          float g = 1.f;
+          if (p.gmax != nullptr) {
+            const float m = *p.gmax;
+            g = m > 0.f ? p.d_loss[t] / m : p.d_loss[t];
+          }
+          // a target outside the vocabulary: NaN, in the loss and in every gradient that it enters
+          p.row_scale[row] = counts ? (valid ? g * p.unit : __int_as_float(0x7FC00000)) : 0.f;
+        } else if (!counts) {
           p.losses[t] = 0.f;
           p.lse[t] = 0.f;
         }
       }
+      before += __popc(mask);
     }
-    if (lane == 0) total_smem = before + __popc(mask);
+    __syncthreads();
+    if (top + warp < end) {
+      const int code = place[warp];
+      const bool counts = code >= 0;
+      uint4* dst = p.hc + static_cast<int64_t>(counts ? code : -1 - code) * p.D8;
+      uint4* zeros = BACKWARD && !counts && p.dh != nullptr ? p.dh + static_cast<int64_t>(top + warp) * p.D8 : nullptr;
+      const uint4* src = p.h + static_cast<int64_t>(top + warp) * p.ldh8;
+      for (int i = lane; i < p.D8; i += 32 * 8) {
+        uint4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = counts && i + 32 * k < p.D8 ? src[i + 32 * k] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (i + 32 * k < p.D8) {
+            dst[i + 32 * k] = v[k];
+            if (zeros != nullptr) zeros[i + 32 * k] = v[k];
+          }
+      }
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  if (last_cta && threadIdx.x == 0) {
-    const int total = total_smem;
-    *p.count = total;
+  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
+    *p.count = before;
     if (BACKWARD) {
       float a = p.gmax != nullptr ? (*p.gmax > 0.f ? *p.gmax : 1.f) : *p.d_loss;
-      if (p.mean) a /= static_cast<float>(total > 0 ? total : 1);
+      if (p.mean) a /= static_cast<float>(before > 0 ? before : 1);
       *p.alpha = a / p.unit;
-    }
-  }
-  const int rows = min(LCE_GATHER_ROWS, p.T - first);
-  for (int r = warp; r < rows; r += 8) {
-    const int code = place[r];
-    const bool counts = code >= 0;
-    uint4* dst = p.hc + static_cast<int64_t>(counts ? code : -1 - code) * p.D8;
-    const uint4* src = p.h + static_cast<int64_t>(first + r) * p.ldh8;
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    for (int i = lane; i < p.D8; i += 32) {
-      dst[i] = counts ? src[i] : zero;
-      if (BACKWARD && !counts && p.dh != nullptr) p.dh[static_cast<int64_t>(first + r) * p.D8 + i] = zero;
     }
   }
 }
@@ -523,64 +733,107 @@ __global__ void __launch_bounds__(1024) lce_gmax_kernel(const float* __restrict_
   }
 }
 
-// Joins the tile columns' (maximum, sum) of 32 rows: 32 slices of the slots, one row per lane.
-__global__ void __launch_bounds__(1024) lce_join_kernel(const float2* __restrict__ part, int64_t part_ld, int slots, const int* __restrict__ count,
+// Joins the tiles' (maximum, sum) of 32 rows: 32 slices of the slots, one row per lane.  Without a gather (token == null) row and token are the same.
+__global__ void __launch_bounds__(1024) lce_join_kernel(const float2* __restrict__ part, int64_t part_ld, int slots, const int* __restrict__ count, int T,
                                                         const float* __restrict__ target_logit, const int* __restrict__ token,
+                                                        const int64_t* __restrict__ target, int64_t ignore, int V, float log2e,
                                                         float* __restrict__ losses, float* __restrict__ lse) {
   __shared__ float2 joined[32][33];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const int row = blockIdx.x * 32 + lane;
-  const bool live = row < *count;
+  const bool live = row < (token != nullptr ? *count : T);
   float m = -INFINITY, s = 0.f;
-  if (live)
-    for (int i = slice; i < slots; i += 32) {
-      const float2 v = part[static_cast<int64_t>(i) * part_ld + row];
-      const float top = fmaxf(m, v.x);
+  if (live) {
+    for (int i = slice; i < slots; i += 4 * 32) {           // four slots at a time: their loads and exponentials do not wait for one another
+      float2 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = i + 32 * k < slots ? part[static_cast<int64_t>(i + 32 * k) * part_ld + row] : make_float2(-INFINITY, 0.f);
+      const float top = fmaxf(m, fmaxf(fmaxf(v[0].x, v[1].x), fmaxf(v[2].x, v[3].x)));
       const float shift = top == -INFINITY ? 0.f : top;
-      s = s * exp2f(m - shift) + v.y * exp2f(v.x - shift);
+      s *= exp2f(m - shift);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s += v[k].y * exp2f(v[k].x - shift);
       m = top;
     }
+  }
   joined[slice][lane] = make_float2(m, s);
   __syncthreads();
-  if (slice == 0 && live) {
-    for (int i = 1; i < 32; ++i) {
-      const float2 v = joined[i][lane];
-      const float top = fmaxf(m, v.x);
-      const float shift = top == -INFINITY ? 0.f : top;
-      s = s * exp2f(m - shift) + v.y * exp2f(v.x - shift);
-      m = top;
-    }
-    const float lse2 = m + log2f(s);
-    const int t = token[row];
-    lse[t] = lse2 * LN2;
-    losses[t] = fmaf(-target_logit[row], LOG2E, lse2) * LN2;
+  // warp i joins the slices of row i
+  const float2 v = joined[lane][slice];
+  float top = v.x;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+  float sum = v.y * exp2f(v.x - (top == -INFINITY ? 0.f : top));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+  const int mine = blockIdx.x * 32 + slice;
+  if (lane == 0 && mine < (token != nullptr ? *count : T)) {
+    const int t = token != nullptr ? token[mine] : mine;
+    const float lse2 = top + log2f(sum);
+    const int64_t y = target[t];
+    const bool counts = y != ignore, valid = y >= 0 && y < V;
+    lse[t] = counts ? lse2 * LN2 : 0.f;
+    losses[t] = !counts ? 0.f : valid ? fmaf(-target_logit[mine], log2e, lse2) * LN2 : __int_as_float(0x7FC00000);
   }
 }
 
 // Sum or mean of the losses, in an order that depends on T only.
-__global__ void __launch_bounds__(1024) lce_reduce_kernel(const float* __restrict__ losses, int T, const int* __restrict__ count, int mean,
-                                                          float* __restrict__ loss) {
+__global__ void __launch_bounds__(1024) lce_reduce_kernel(const float* __restrict__ losses, const int64_t* __restrict__ target, int64_t ignore, int T,
+                                                          int mean, float* __restrict__ loss) {
   __shared__ double warps[32];
+  __shared__ int counts[32];
   double s = 0.0;
-  for (int i = threadIdx.x; i < T; i += 1024) s += static_cast<double>(losses[i]);
+  int n = 0;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < T; i += 1024) {
+    s += static_cast<double>(losses[i]);
+    n += target[i] != ignore ? 1 : 0;
+  }
+  n = __reduce_add_sync(0xFFFFFFFFu, n);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = s;
+  if ((threadIdx.x & 31) == 0) {
+    warps[threadIdx.x >> 5] = s;
+    counts[threadIdx.x >> 5] = n;
+  }
   __syncthreads();
   if (threadIdx.x < 32) {
     s = warps[threadIdx.x];
+    n = __reduce_add_sync(0xFFFFFFFFu, counts[threadIdx.x]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-    if (threadIdx.x == 0) {
-      const int n = *count;
-      *loss = static_cast<float>(mean ? s / (n > 0 ? n : 1) : s);
+    if (threadIdx.x == 0) *loss = static_cast<float>(mean ? s / (n > 0 ? n : 1) : s);
+  }
+}
+
+// dh from the fp32 sums of the parts of K, where the product was cut in several (a CTA per row that counts).
+__global__ void __launch_bounds__(256) lce_dh_kernel(const LceGemmParams p, int pairs) {
+  const int count = *p.count;
+  const int row = blockIdx.x;
+  if (row >= count) return;
+  const int splits = lce_splits(((count + 255) >> 8) * ((p.N + 255) >> 8), pairs, (p.K + 63) >> 6, p.max_splits);
+  if (splits == 1) return;
+  const float alpha = *p.alpha;
+  uint16_t* out = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(p.token[row]) * p.N;
+  for (int c = threadIdx.x * 4; c < p.N; c += 1024) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) {
+      const float4 v = *reinterpret_cast<const float4*>(p.sum + k * p.split_stride + static_cast<int64_t>(row) * p.N + c);
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
     }
+    *reinterpret_cast<uint2*>(out + c) = make_uint2(lce_pack2(s.x * alpha, s.y * alpha, p.f16), lce_pack2(s.z * alpha, s.w * alpha, p.f16));
   }
 }
 
 // ---------------------------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------------------------
+// Slots of the forward's workspace with few tokens: tiles of lce_narrow_width, at most one per SM and wave, and a wave is 256 columns per SM or all there is.
+constexpr int LCE_NARROW_SLOTS = 512;
+// Tokens up to which the forward reads h where it is (one tile row: leaving tokens out would save nothing), and up to which it runs on single CTAs.
+constexpr int LCE_DIRECT_TOKENS = 256, LCE_NARROW_TOKENS = 128;
+
 // Bytes of dlogits that a piece of the vocabulary may take.
 constexpr int64_t LCE_PIECE_BYTES = int64_t(512) << 20;
 
@@ -594,7 +847,7 @@ static int lce_piece(int T, int V) {
 
 struct LceLayout {
   int64_t hc, token, row_target, count, alpha, gmax, a, b, part, dl, sum, total;   // byte offsets
-  int slots, piece, pieces;
+  int slots, piece, pieces, max_splits;
   int64_t ld_dl;
 };
 static LceLayout lce_layout(int T, int D, int V, bool backward) {
@@ -613,7 +866,8 @@ static LceLayout lce_layout(int T, int D, int V, bool backward) {
   l.a = take(4ll * T);           // forward: target logits; backward: lse * log2 e
   l.hc = take(2ll * T * D);
   if (!backward) {
-    l.slots = 2 * ((V + 255) / 256);
+    l.slots = 2 * ((V + 255) / 256);       // two per tile of 256; tiles of single CTAs are never narrower than 16 and no more than four per SM
+    if (T <= LCE_NARROW_TOKENS && l.slots < LCE_NARROW_SLOTS) l.slots = LCE_NARROW_SLOTS;
     l.part = take(8ll * T * l.slots);
   } else {
     l.b = take(4ll * T);         // row factors
@@ -621,7 +875,12 @@ static LceLayout lce_layout(int T, int D, int V, bool backward) {
     l.pieces = (V + l.piece - 1) / l.piece;
     l.ld_dl = (l.piece + 7) / 8 * 8;
     l.dl = take(2ll * T * l.ld_dl);
-    if (l.pieces > 1) l.sum = take(4ll * T * D);
+    // as many parts as could fill the pairs eight times over
+    const int64_t tiles = static_cast<int64_t>((T + 255) / 256) * ((D + 255) / 256);
+    const int64_t splits = 8 * 74 / tiles;
+    // (several pieces carry one sum from piece to piece: their dlogits take up the 512 MiB, so that there are tiles enough)
+    l.max_splits = static_cast<int>(l.pieces > 1 || splits < 1 ? 1 : splits > LCE_MAX_SPLITS ? LCE_MAX_SPLITS : splits);
+    if (l.pieces > 1 || l.max_splits > 1) l.sum = take(4ll * T * D * l.max_splits);
   }
   l.total = at;
   return l;
@@ -653,6 +912,16 @@ static int lce_check_workspace(const LceArgs& a, const LceLayout& l, const char*
   return B200K_OK;
 }
 
+// Rows of a gathering CTA: about a thousand CTAs, each of which counts the tokens before its own.
+static int lce_gather_rows(int T) { return (T / 1024 / LCE_GATHER_ROWS + 1) * LCE_GATHER_ROWS; }
+
+// CTA pairs of a launch: enough for every tile's halves, or for the parts of K.
+static int lce_pairs(const LceGemmParams& p, const DeviceInfo* dev) {
+  const int64_t tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256) * (p.max_splits > 2 ? p.max_splits : 2);
+  const int max_pairs = dev->sm_count / 2;
+  return static_cast<int>(tiles < max_pairs ? tiles : max_pairs);
+}
+
 template <int EPI, bool A_MN, bool B_MN>
 static int lce_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, LceGemmParams p, const DeviceInfo* dev, cudaStream_t stream) {
   p.group_m = 8;
@@ -660,10 +929,7 @@ static int lce_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensor
   p.idesc_half = umma_idesc_16bit_f32(256, 128, A_MN, B_MN, p.f16);
   p.status = dev->status_word;
   B200K_CHECK_CUDA(cudaFuncSetAttribute(lce_gemm_kernel<EPI, A_MN, B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, LCE_SMEM));
-  const int64_t tiles = static_cast<int64_t>((p.M + 255) / 256) * ((p.N + 255) / 256);
-  const int max_pairs = dev->sm_count / 2;
-  // twice the tiles: a short launch is one wave of column halves
-  const int pairs = static_cast<int>(2 * tiles < max_pairs ? 2 * tiles : max_pairs);
+  const int pairs = lce_pairs(p, dev);
   lce_gemm_kernel<EPI, A_MN, B_MN><<<2 * pairs, LCE_THREADS, LCE_SMEM, stream>>>(ta, tb, tc, p);
   count_launch();
   B200K_CHECK_LAUNCH("lce_gemm_kernel");
@@ -695,44 +961,67 @@ int lce_fwd(const LceArgs& a, cudaStream_t stream) {
   const DeviceInfo* dev = lce_device(what);
   if (dev == nullptr) return B200K_ERR_NO_DEVICE;
   char* ws = static_cast<char*>(a.workspace);
-  int* count = reinterpret_cast<int*>(ws + l.count);
-  int* token = reinterpret_cast<int*>(ws + l.token);
-
-  LceGatherParams g{};
-  g.h = static_cast<const uint4*>(a.h);
-  g.ldh8 = a.ldh / 8;
-  g.target = a.target;
-  g.ignore = a.ignore_index;
-  g.T = a.T; g.D8 = a.D / 8; g.V = a.V;
-  g.hc = reinterpret_cast<uint4*>(ws + l.hc);
-  g.count = count;
-  g.token = token;
-  g.row_target = reinterpret_cast<int*>(ws + l.row_target);
-  g.target_logit = reinterpret_cast<float*>(ws + l.a);
-  g.losses = a.losses;
-  g.lse = a.lse;
-  lce_gather_kernel<false><<<(a.T + LCE_GATHER_ROWS - 1) / LCE_GATHER_ROWS, 256, 0, stream>>>(g);
-  count_launch();
-  B200K_CHECK_LAUNCH("lce_gather_kernel");
-
-  CUtensorMap th, tw;
-  if ((rc = make_tmap_bf16_2d(&th, ws + l.hc, a.D, a.T, a.D, 64, 64)) != 0) return rc;
-  if ((rc = make_tmap_bf16_2d(&tw, a.w, a.D, a.V, a.ldw, 64, 64)) != 0) return rc;
+  float* target_logit = reinterpret_cast<float*>(ws + l.a);
+  const bool direct = a.T <= LCE_DIRECT_TOKENS;
   LceGemmParams p{};
-  p.count = count;
   p.M = a.T; p.N = a.V; p.K = a.D;
   p.f16 = a.dtype == B200K_DTYPE_F16;
-  p.target = g.row_target;
+  p.log2e = lce_log2e(a.D);
   p.part = reinterpret_cast<float2*>(ws + l.part);
   p.part_ld = a.T;
-  p.target_logit = g.target_logit;
-  if ((rc = lce_gemm<LCE_STATS, false, false>(th, tw, th, p, dev, stream)) != 0) return rc;
-
-  lce_join_kernel<<<(a.T + 31) / 32, 1024, 0, stream>>>(p.part, p.part_ld, l.slots, count, g.target_logit, token, a.losses, a.lse);
+  p.target_logit = target_logit;
+  const void* rows = a.h;
+  int64_t ld_rows = a.ldh;
+  if (direct) {
+    p.token_target = a.target;
+  } else {
+    LceGatherParams g{};
+    g.h = static_cast<const uint4*>(a.h);
+    g.ldh8 = a.ldh / 8;
+    g.target = a.target;
+    g.ignore = a.ignore_index;
+    g.T = a.T; g.D8 = a.D / 8; g.V = a.V;
+    g.hc = reinterpret_cast<uint4*>(ws + l.hc);
+    g.count = reinterpret_cast<int*>(ws + l.count);
+    g.token = reinterpret_cast<int*>(ws + l.token);
+    g.row_target = reinterpret_cast<int*>(ws + l.row_target);
+    g.losses = a.losses;
+    g.lse = a.lse;
+    g.cta_rows = lce_gather_rows(a.T);
+  lce_gather_kernel<false><<<(a.T + g.cta_rows - 1) / g.cta_rows, 256, 0, stream>>>(g);
+    count_launch();
+    B200K_CHECK_LAUNCH("lce_gather_kernel");
+    p.count = g.count;
+    p.target = g.row_target;
+    p.token = g.token;
+    rows = ws + l.hc;
+    ld_rows = a.D;
+  }
+  int slots = 2 * ((a.V + 255) / 256);
+  CUtensorMap th, tw;
+  if (a.T <= LCE_NARROW_TOKENS) {
+    p.width = lce_narrow_width(a.V, dev->sm_count);
+    slots = (a.V + p.width - 1) / p.width;
+    if (slots > l.slots) return set_error(B200K_ERR_INVALID_ARG, "%s: workspace slots", what);
+    if ((rc = make_tmap_bf16_2d(&th, rows, a.D, a.T, ld_rows, 64, 128)) != 0) return rc;
+    if ((rc = make_tmap_bf16_2d(&tw, a.w, a.D, a.V, a.ldw, 64, p.width)) != 0) return rc;
+    p.idesc = umma_idesc_16bit_f32(128, p.width, 0, 0, p.f16);
+    p.status = dev->status_word;
+    B200K_CHECK_CUDA(cudaFuncSetAttribute(lce_stats_narrow_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LCE1_SMEM));
+    lce_stats_narrow_kernel<<<slots < dev->sm_count ? slots : dev->sm_count, LCE_THREADS, LCE1_SMEM, stream>>>(th, tw, p);
+    count_launch();
+    B200K_CHECK_LAUNCH("lce_stats_narrow_kernel");
+  } else {
+    if ((rc = make_tmap_bf16_2d(&th, rows, a.D, a.T, ld_rows, 64, 64)) != 0) return rc;
+    if ((rc = make_tmap_bf16_2d(&tw, a.w, a.D, a.V, a.ldw, 64, 64)) != 0) return rc;
+    if ((rc = lce_gemm<LCE_STATS, false, false>(th, tw, th, p, dev, stream)) != 0) return rc;
+  }
+  lce_join_kernel<<<(a.T + 31) / 32, 1024, 0, stream>>>(p.part, p.part_ld, slots, p.count, a.T, target_logit, p.token, a.target, a.ignore_index, a.V,
+                                                        p.log2e, a.losses, a.lse);
   count_launch();
   B200K_CHECK_LAUNCH("lce_join_kernel");
   if (a.reduction != B200K_REDUCE_NONE) {
-    lce_reduce_kernel<<<1, 1024, 0, stream>>>(a.losses, a.T, count, a.reduction == B200K_REDUCE_MEAN, a.loss);
+    lce_reduce_kernel<<<1, 1024, 0, stream>>>(a.losses, a.target, a.ignore_index, a.T, a.reduction == B200K_REDUCE_MEAN, a.loss);
     count_launch();
     B200K_CHECK_LAUNCH("lce_reduce_kernel");
   }
@@ -781,13 +1070,14 @@ int lce_bwd(const LceArgs& a, cudaStream_t stream) {
   g.alpha = reinterpret_cast<float*>(ws + l.alpha);
   g.unit = a.dtype == B200K_DTYPE_F16 ? LCE_F16_SCALE : 1.f;
   g.mean = a.reduction == B200K_REDUCE_MEAN;
-  lce_gather_kernel<true><<<(a.T + LCE_GATHER_ROWS - 1) / LCE_GATHER_ROWS, 256, 0, stream>>>(g);
+  g.cta_rows = lce_gather_rows(a.T);
+  lce_gather_kernel<true><<<(a.T + g.cta_rows - 1) / g.cta_rows, 256, 0, stream>>>(g);
   count_launch();
   B200K_CHECK_LAUNCH("lce_gather_kernel");
 
   CUtensorMap th;
   if ((rc = make_tmap_bf16_2d(&th, ws + l.hc, a.D, a.T, a.D, 64, 64)) != 0) return rc;
-  float* sum = l.pieces > 1 ? reinterpret_cast<float*>(ws + l.sum) : nullptr;
+  float* sum = l.pieces > 1 || l.max_splits > 1 ? reinterpret_cast<float*>(ws + l.sum) : nullptr;
   for (int k = 0; k < l.pieces; ++k) {
     const int v0 = k * l.piece;
     const int n = a.V - v0 < l.piece ? a.V - v0 : l.piece;
@@ -801,6 +1091,7 @@ int lce_bwd(const LceArgs& a, cudaStream_t stream) {
     p.count = g.count;
     p.f16 = a.dtype == B200K_DTYPE_F16;
     p.alpha = g.alpha;
+    p.log2e = lce_log2e(a.D);
     p.M = a.T; p.N = n; p.K = a.D;
     p.target = g.row_target;
     p.col_base = v0;
@@ -815,11 +1106,19 @@ int lce_bwd(const LceArgs& a, cudaStream_t stream) {
     }
     if (a.dh != nullptr) {
       p.M = a.T; p.N = a.D; p.K = n;
+      p.max_splits = l.max_splits;
       p.add = k > 0 ? sum : nullptr;
-      p.sum = k + 1 < l.pieces ? sum : nullptr;
+      p.sum = sum;
+      p.split_stride = static_cast<int64_t>(a.T) * a.D;
+      p.last = k + 1 == l.pieces;
       p.out = a.dh;
       p.token = g.token;
       if ((rc = lce_gemm<LCE_DH, false, true>(tdl, tw, tw, p, dev, stream)) != 0) return rc;
+      if (p.max_splits > 1) {
+        lce_dh_kernel<<<a.T, 256, 0, stream>>>(p, lce_pairs(p, dev));
+        count_launch();
+        B200K_CHECK_LAUNCH("lce_dh_kernel");
+      }
     }
   }
   return B200K_OK;
