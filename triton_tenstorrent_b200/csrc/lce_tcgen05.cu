@@ -162,6 +162,13 @@ __device__ __forceinline__ void lce_store_chunk(const CUtensorMap* map, const fl
   buf ^= 1;
 }
 
+// 2^x in one instruction, results below 2^-126 as 0 (a probability that small is below everything it is added to).
+__device__ __forceinline__ float lce_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // 64 columns of a row of logits into its running maximum (in units of log2) and sum of 2^(x - maximum); `in`: the target's place among them, `limit`:
 // the first column that does not count.
 __device__ __forceinline__ void lce_stats_chunk(float (&f)[64], int in, int col0, int limit, float log2e, float* target_logit, float& run_max,
@@ -185,12 +192,12 @@ __device__ __forceinline__ void lce_stats_chunk(float (&f)[64], int in, int col0
   float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
   for (int j = 0; j < 64; j += 4) {
-    s0 += exp2f(fmaf(f[j], log2e, -shift));
-    s1 += exp2f(fmaf(f[j + 1], log2e, -shift));
-    s2 += exp2f(fmaf(f[j + 2], log2e, -shift));
-    s3 += exp2f(fmaf(f[j + 3], log2e, -shift));
+    s0 += lce_exp2(fmaf(f[j], log2e, -shift));
+    s1 += lce_exp2(fmaf(f[j + 1], log2e, -shift));
+    s2 += lce_exp2(fmaf(f[j + 2], log2e, -shift));
+    s3 += lce_exp2(fmaf(f[j + 3], log2e, -shift));
   }
-  run_sum = fmaf(run_sum, exp2f(run_max - shift), (s0 + s1) + (s2 + s3));
+  run_sum = fmaf(run_sum, lce_exp2(run_max - shift), (s0 + s1) + (s2 + s3));
   run_max = new_max;
 }
 
@@ -397,7 +404,7 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         } else if constexpr (EPI == LCE_DLOGITS) {
 #pragma unroll
           for (int j = 0; j < 64; ++j) {
-            const float e = exp2f(fmaf(f[j], p.log2e, -lse2)) - (j == in ? 1.f : 0.f);
+            const float e = lce_exp2(fmaf(f[j], p.log2e, -lse2)) - (j == in ? 1.f : 0.f);
             f[j] = live ? e * scale : 0.f;           // rows behind the last one that counts: zeros, for the K tail of dW
           }
           if (col0 + 64 > p.N) {                       // columns behind the piece: zeros, for the K tail of dh
@@ -750,9 +757,9 @@ __global__ void __launch_bounds__(1024) lce_join_kernel(const float2* __restrict
       for (int k = 0; k < 4; ++k) v[k] = i + 32 * k < slots ? part[static_cast<int64_t>(i + 32 * k) * part_ld + row] : make_float2(-INFINITY, 0.f);
       const float top = fmaxf(m, fmaxf(fmaxf(v[0].x, v[1].x), fmaxf(v[2].x, v[3].x)));
       const float shift = top == -INFINITY ? 0.f : top;
-      s *= exp2f(m - shift);
+      s *= lce_exp2(m - shift);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s += v[k].y * exp2f(v[k].x - shift);
+      for (int k = 0; k < 4; ++k) s += v[k].y * lce_exp2(v[k].x - shift);
       m = top;
     }
   }
@@ -763,7 +770,7 @@ __global__ void __launch_bounds__(1024) lce_join_kernel(const float2* __restrict
   float top = v.x;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-  float sum = v.y * exp2f(v.x - (top == -INFINITY ? 0.f : top));
+  float sum = v.y * lce_exp2(v.x - (top == -INFINITY ? 0.f : top));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
   const int mine = blockIdx.x * 32 + slice;

@@ -707,19 +707,22 @@ def _tma_rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _lce_forward(h, weight, targets, ignore_index, reduction):
-    """(losses, lse, loss), on the device."""
+    """(losses, lse, loss), on the device; loss is None with reduction "none"."""
     lib = _lib.load()
-    hd, wd, td = _tma_rows(_to_device(h)), _tma_rows(_to_device(weight)), _to_device(targets).contiguous()
+    hd, wd, td = _tma_rows(_to_device(h)), _tma_rows(_to_device(weight)), _to_device(targets)
+    if not td.is_contiguous():
+        td = td.contiguous()
     (T, D), V = hd.shape, wd.shape[0]
-    out = torch.empty((2, T), device=hd.device, dtype=torch.float32)
-    loss = torch.empty((), device=hd.device, dtype=torch.float32)
+    out = torch.empty((2, *targets.shape), device=hd.device, dtype=torch.float32)
+    loss = None if reduction == "none" else torch.empty((), device=hd.device, dtype=torch.float32)
     size = lib.b200k_lce_workspace(T, D, V, 0)
     work = torch.empty(size, device=hd.device, dtype=torch.uint8)
+    losses = out.data_ptr()
     with _on(hd.device):
-        _lib.check(lib.b200k_lce_fwd(hd.data_ptr(), wd.data_ptr(), td.data_ptr(), out.data_ptr(), out.data_ptr() + 4 * T, loss.data_ptr(),
+        _lib.check(lib.b200k_lce_fwd(hd.data_ptr(), wd.data_ptr(), td.data_ptr(), losses, losses + 4 * T, 0 if loss is None else loss.data_ptr(),
                                      work.data_ptr(), size, T, D, V, _pitch(hd), _pitch(wd), ignore_index, _REDUCTIONS[reduction],
                                      _DTYPES[h.dtype], _stream()))
-    return out[0].view(targets.shape), out[1].view(targets.shape), loss
+    return out[0], out[1], loss
 
 
 def linear_cross_entropy_with_lse(h, weight, targets, ignore_index: int = -100):
