@@ -39,6 +39,23 @@ void count_launch();
     if (e__ != cudaSuccess) return set_error(B200K_ERR_CUDA, "%s: %s", #expr, cudaGetErrorString(e__)); \
   } while (0)
 
+// Launches a kernel that calls grid_wait (ptx.cuh) behind a kernel of this library in the same stream: its launch latency and setup overlap that
+// kernel's end.  Every kernel of such a chain calls grid_wait, so that the end of one implies the end of those before it.
+template <typename... P, typename... A>
+inline cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = block;
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
+}
+
 // 2-D bf16 tensor map: `inner` contiguous elements per row, `outer` rows, row pitch `ld` elements,
 // box = box_inner x box_outer elements, 128-byte swizzle (box_inner * 2 bytes at most 128; narrower rows are
 // padded to 128 bytes in shared memory),

@@ -495,6 +495,7 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
       stage_at += 2 * stage_rows * ring.row_bytes;
       if (++stage == ring.stages) { stage = stage_at = 0; phase ^= 1u; }
     }
+    grid_launch_dependents();
     if (part != nullptr) {
       float* out_w = part + static_cast<int64_t>(blockIdx.x) * cols;
       float* out_b = part + static_cast<int64_t>(gridDim.x + blockIdx.x) * cols;
@@ -544,6 +545,7 @@ template <typename W>
 __global__ void __launch_bounds__(1024) ln_dw_join_kernel(const float* __restrict__ part, W* __restrict__ dw, W* __restrict__ db, int parts,
                                                           int64_t cols) {
   __shared__ float sums[32][33];
+  grid_wait();
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   const float* p = part + static_cast<int64_t>(blockIdx.y) * parts * cols;
@@ -732,8 +734,8 @@ static int ln_bwd(const LayerNormArgs& a, const DeviceInfo* dev, cudaStream_t st
     if (rc != B200K_OK) return rc;
   }
   if (sums) {
-    ln_dw_join_kernel<W><<<dim3(static_cast<unsigned>((a.cols + 31) / 32), 2), 1024, 0, stream>>>(a.workspace, static_cast<W*>(a.dw),
-                                                                                                 static_cast<W*>(a.db), parts, a.cols);
+    B200K_CHECK_CUDA(launch_dependent(ln_dw_join_kernel<W>, dim3(static_cast<unsigned>((a.cols + 31) / 32), 2), dim3(1024), 0, stream, a.workspace,
+                                      static_cast<W*>(a.dw), static_cast<W*>(a.db), parts, a.cols));
     count_launch();
     B200K_CHECK_LAUNCH("ln_dw_join_kernel");
   }

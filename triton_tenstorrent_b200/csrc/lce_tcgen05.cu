@@ -17,6 +17,7 @@
 // Bound: the tensor pipe; with few tokens the stream of W from HBM.
 #include <string.h>
 
+#include "attn_common.cuh"
 #include "launch.h"
 #include "ptx.cuh"
 
@@ -162,13 +163,6 @@ __device__ __forceinline__ void lce_store_chunk(const CUtensorMap* map, const fl
   buf ^= 1;
 }
 
-// 2^x in one instruction, results below 2^-126 as 0 (a probability that small is below everything it is added to).
-__device__ __forceinline__ float lce_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // 64 columns of a row of logits into its running maximum (in units of log2) and sum of 2^(x - maximum); `in`: the target's place among them, `limit`:
 // the first column that does not count.
 __device__ __forceinline__ void lce_stats_chunk(float (&f)[64], int in, int col0, int limit, float log2e, float* target_logit, float& run_max,
@@ -192,12 +186,12 @@ __device__ __forceinline__ void lce_stats_chunk(float (&f)[64], int in, int col0
   float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
   for (int j = 0; j < 64; j += 4) {
-    s0 += lce_exp2(fmaf(f[j], log2e, -shift));
-    s1 += lce_exp2(fmaf(f[j + 1], log2e, -shift));
-    s2 += lce_exp2(fmaf(f[j + 2], log2e, -shift));
-    s3 += lce_exp2(fmaf(f[j + 3], log2e, -shift));
+    s0 += ex2_approx(fmaf(f[j], log2e, -shift));
+    s1 += ex2_approx(fmaf(f[j + 1], log2e, -shift));
+    s2 += ex2_approx(fmaf(f[j + 2], log2e, -shift));
+    s3 += ex2_approx(fmaf(f[j + 3], log2e, -shift));
   }
-  run_sum = fmaf(run_sum, lce_exp2(run_max - shift), (s0 + s1) + (s2 + s3));
+  run_sum = fmaf(run_sum, ex2_approx(run_max - shift), (s0 + s1) + (s2 + s3));
   run_max = new_max;
 }
 
@@ -254,6 +248,8 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   cluster_wait();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_ptr_smem;
+  grid_launch_dependents();
+  grid_wait();
 
   const int count = p.count != nullptr ? *p.count : p.M;
   const int M = EPI == LCE_DW ? p.M : count;
@@ -404,7 +400,7 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         } else if constexpr (EPI == LCE_DLOGITS) {
 #pragma unroll
           for (int j = 0; j < 64; ++j) {
-            const float e = lce_exp2(fmaf(f[j], p.log2e, -lse2)) - (j == in ? 1.f : 0.f);
+            const float e = ex2_approx(fmaf(f[j], p.log2e, -lse2)) - (j == in ? 1.f : 0.f);
             f[j] = live ? e * scale : 0.f;           // rows behind the last one that counts: zeros, for the K tail of dW
           }
           if (col0 + 64 > p.N) {                       // columns behind the piece: zeros, for the K tail of dh
@@ -520,6 +516,7 @@ lce_stats_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_ptr_smem;
+  grid_launch_dependents();
   const int num_kb = (p.K + 63) >> 6;
   const int tiles = (p.N + p.width - 1) / p.width;
 
@@ -647,6 +644,8 @@ struct LceGatherParams {
 
 template <bool BACKWARD>
 __global__ void __launch_bounds__(256) lce_gather_kernel(const LceGatherParams p) {
+  grid_launch_dependents();
+  grid_wait();
   __shared__ int warp_counts[8];
   __shared__ int place[LCE_GATHER_ROWS];       // row of hc; that of a row that does not count as -1 - row
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -726,6 +725,7 @@ __global__ void __launch_bounds__(256) lce_gather_kernel(const LceGatherParams p
 __global__ void __launch_bounds__(1024) lce_gmax_kernel(const float* __restrict__ g, const int64_t* __restrict__ target, int64_t ignore, int T,
                                                         float* __restrict__ gmax) {
   __shared__ float warps[32];
+  grid_launch_dependents();
   float m = 0.f;
   for (int i = threadIdx.x; i < T; i += 1024) {
     const float a = fabsf(g[i]);
@@ -746,6 +746,8 @@ __global__ void __launch_bounds__(1024) lce_join_kernel(const float2* __restrict
                                                         const int64_t* __restrict__ target, int64_t ignore, int V, float log2e,
                                                         float* __restrict__ losses, float* __restrict__ lse) {
   __shared__ float2 joined[32][33];
+  grid_launch_dependents();
+  grid_wait();
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const int row = blockIdx.x * 32 + lane;
   const bool live = row < (token != nullptr ? *count : T);
@@ -757,9 +759,9 @@ __global__ void __launch_bounds__(1024) lce_join_kernel(const float2* __restrict
       for (int k = 0; k < 4; ++k) v[k] = i + 32 * k < slots ? part[static_cast<int64_t>(i + 32 * k) * part_ld + row] : make_float2(-INFINITY, 0.f);
       const float top = fmaxf(m, fmaxf(fmaxf(v[0].x, v[1].x), fmaxf(v[2].x, v[3].x)));
       const float shift = top == -INFINITY ? 0.f : top;
-      s *= lce_exp2(m - shift);
+      s *= ex2_approx(m - shift);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s += v[k].y * lce_exp2(v[k].x - shift);
+      for (int k = 0; k < 4; ++k) s += v[k].y * ex2_approx(v[k].x - shift);
       m = top;
     }
   }
@@ -770,7 +772,7 @@ __global__ void __launch_bounds__(1024) lce_join_kernel(const float2* __restrict
   float top = v.x;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-  float sum = v.y * lce_exp2(v.x - (top == -INFINITY ? 0.f : top));
+  float sum = v.y * ex2_approx(v.x - (top == -INFINITY ? 0.f : top));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
   const int mine = blockIdx.x * 32 + slice;
@@ -789,6 +791,7 @@ __global__ void __launch_bounds__(1024) lce_reduce_kernel(const float* __restric
                                                           int mean, float* __restrict__ loss) {
   __shared__ double warps[32];
   __shared__ int counts[32];
+  grid_wait();
   double s = 0.0;
   int n = 0;
 #pragma unroll 4
@@ -815,6 +818,8 @@ __global__ void __launch_bounds__(1024) lce_reduce_kernel(const float* __restric
 
 // dh from the fp32 sums of the parts of K, where the product was cut in several (a CTA per row that counts).
 __global__ void __launch_bounds__(256) lce_dh_kernel(const LceGemmParams p, int pairs) {
+  grid_launch_dependents();
+  grid_wait();
   const int count = *p.count;
   const int row = blockIdx.x;
   if (row >= count) return;
@@ -937,7 +942,12 @@ static int lce_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensor
   p.status = dev->status_word;
   B200K_CHECK_CUDA(cudaFuncSetAttribute(lce_gemm_kernel<EPI, A_MN, B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, LCE_SMEM));
   const int pairs = lce_pairs(p, dev);
-  lce_gemm_kernel<EPI, A_MN, B_MN><<<2 * pairs, LCE_THREADS, LCE_SMEM, stream>>>(ta, tb, tc, p);
+  // the forward's with few tokens is the first of its chain
+  if (p.count == nullptr) {
+    lce_gemm_kernel<EPI, A_MN, B_MN><<<2 * pairs, LCE_THREADS, LCE_SMEM, stream>>>(ta, tb, tc, p);
+  } else {
+    B200K_CHECK_CUDA(launch_dependent(lce_gemm_kernel<EPI, A_MN, B_MN>, dim3(2 * pairs), dim3(LCE_THREADS), LCE_SMEM, stream, ta, tb, tc, p));
+  }
   count_launch();
   B200K_CHECK_LAUNCH("lce_gemm_kernel");
   return B200K_OK;
@@ -1023,12 +1033,13 @@ int lce_fwd(const LceArgs& a, cudaStream_t stream) {
     if ((rc = make_tmap_bf16_2d(&tw, a.w, a.D, a.V, a.ldw, 64, 64)) != 0) return rc;
     if ((rc = lce_gemm<LCE_STATS, false, false>(th, tw, th, p, dev, stream)) != 0) return rc;
   }
-  lce_join_kernel<<<(a.T + 31) / 32, 1024, 0, stream>>>(p.part, p.part_ld, slots, p.count, a.T, target_logit, p.token, a.target, a.ignore_index, a.V,
-                                                        p.log2e, a.losses, a.lse);
+  B200K_CHECK_CUDA(launch_dependent(lce_join_kernel, dim3((a.T + 31) / 32), dim3(1024), 0, stream, p.part, p.part_ld, slots, p.count, a.T, target_logit,
+                                    p.token, a.target, a.ignore_index, a.V, p.log2e, a.losses, a.lse));
   count_launch();
   B200K_CHECK_LAUNCH("lce_join_kernel");
   if (a.reduction != B200K_REDUCE_NONE) {
-    lce_reduce_kernel<<<1, 1024, 0, stream>>>(a.losses, a.target, a.ignore_index, a.T, a.reduction == B200K_REDUCE_MEAN, a.loss);
+    B200K_CHECK_CUDA(launch_dependent(lce_reduce_kernel, dim3(1), dim3(1024), 0, stream, a.losses, a.target, a.ignore_index, a.T,
+                                      a.reduction == B200K_REDUCE_MEAN ? 1 : 0, a.loss));
     count_launch();
     B200K_CHECK_LAUNCH("lce_reduce_kernel");
   }
@@ -1078,7 +1089,11 @@ int lce_bwd(const LceArgs& a, cudaStream_t stream) {
   g.unit = a.dtype == B200K_DTYPE_F16 ? LCE_F16_SCALE : 1.f;
   g.mean = a.reduction == B200K_REDUCE_MEAN;
   g.cta_rows = lce_gather_rows(a.T);
-  lce_gather_kernel<true><<<(a.T + g.cta_rows - 1) / g.cta_rows, 256, 0, stream>>>(g);
+  if (each) {
+    B200K_CHECK_CUDA(launch_dependent(lce_gather_kernel<true>, dim3((a.T + g.cta_rows - 1) / g.cta_rows), dim3(256), 0, stream, g));
+  } else {
+    lce_gather_kernel<true><<<(a.T + g.cta_rows - 1) / g.cta_rows, 256, 0, stream>>>(g);
+  }
   count_launch();
   B200K_CHECK_LAUNCH("lce_gather_kernel");
 
@@ -1122,7 +1137,7 @@ int lce_bwd(const LceArgs& a, cudaStream_t stream) {
       p.token = g.token;
       if ((rc = lce_gemm<LCE_DH, false, true>(tdl, tw, tw, p, dev, stream)) != 0) return rc;
       if (p.max_splits > 1) {
-        lce_dh_kernel<<<a.T, 256, 0, stream>>>(p, lce_pairs(p, dev));
+        B200K_CHECK_CUDA(launch_dependent(lce_dh_kernel, dim3(a.T), dim3(256), 0, stream, p, lce_pairs(p, dev)));
         count_launch();
         B200K_CHECK_LAUNCH("lce_dh_kernel");
       }

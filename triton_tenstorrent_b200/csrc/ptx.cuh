@@ -513,6 +513,12 @@ __device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
   return d;
 }
 
+// Programmatic dependent launch.  A kernel started by launch_dependent (launch.h) may begin while the kernel before it in the stream still runs: it
+// must call grid_wait before it touches global memory, which returns when that kernel has finished and its writes are visible.
+// grid_launch_dependents lets the kernel behind this one begin; that one's grid_wait still waits for this one's end.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // Named barrier among `nthreads` threads (ids 1..15; 0 is __syncthreads).
 __device__ __forceinline__ void named_bar_sync(uint32_t id, uint32_t nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
