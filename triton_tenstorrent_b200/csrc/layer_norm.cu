@@ -140,6 +140,7 @@ __device__ __forceinline__ bool ln_inside(int k, int c, int cols) { return (TPR 
 
 struct LnRing {
   int stage_rows, stages, row_bytes;   // rows of a stage; row_bytes: a row's place in it, a multiple of 16
+  int weight_bytes;                    // before the ring: a copy of w, where a thread's part does not fit its registers
 };
 
 // One operand's rows, and where its memory ends (nothing outside [base, end) is read).
@@ -380,7 +381,9 @@ __global__ void __launch_bounds__(ln_threads<TPR>(), ln_per_sm<TPR, true>())
 ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, const float* __restrict__ mean, const float* __restrict__ rstd,
               T* __restrict__ dx, float* __restrict__ part, int rows, int cols, int64_t lddx, const LnRing ring, uint32_t* status) {
   constexpr int GROUPS = ln_groups<TPR>();
-  constexpr bool HOLD = PER * VEC <= 16;       // w stays in registers, and u and h do between the row sum and dx
+  // Up to 16 elements a thread, w stays in registers, and u and h do between the row sum and dx.  With 32, half as many warps share a row's fixed work
+  // (about 80 instructions a warp); w is read from shared memory, and x and dy once more from the ring.
+  constexpr bool HOLD = PER * VEC <= 16;
   using V = typename Lanes<VEC>::V;
   constexpr int N = Lanes<VEC>::N;
   extern __shared__ __align__(16) char ring_mem[];
@@ -398,10 +401,24 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
   const int group = threadIdx.x / TPR;
   if (group == GROUPS) {
     const LnSource src[2] = {sg, sx};
-    ln_fetch_all<T, 2>(src, ring, rows, cols * static_cast<int>(sizeof(T)), ring_mem, full, empty, ctx);
+    ln_fetch_all<T, 2>(src, ring, rows, cols * static_cast<int>(sizeof(T)), ring_mem + ring.weight_bytes, full, empty, ctx);
   } else {
     const int lane = threadIdx.x % TPR;
+    W* const held_w = reinterpret_cast<W*>(ring_mem);
+    if constexpr (!HOLD) {                  // each thread copies what it will read itself
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        const int c = (lane + k * TPR) * VEC;
+        V t[N];
+        ln_weight<W, VEC>(w, c, cols, 1.f, t);
+        if (c < cols) store_lanes<W, VEC>(held_w + c, t);
+      }
+    }
     V fw[HOLD ? PER : 1][N], aw[PER][N], ab[PER][N];
+    if constexpr (!HOLD) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) fw[0][j] = vsplat<V>(0.f);     // behind the row's end it meets a zero dy
+    }
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
       if constexpr (HOLD) ln_weight<W, VEC>(w, (lane + k * TPR) * VEC, cols, 1.f, fw[k]);
@@ -410,7 +427,7 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
     }
     const float inv_n = 1.f / static_cast<float>(cols);
     const int stage_rows = TPR == 32 ? ring.stage_rows : 1;
-    const char* const my_ring = ring_mem + lane * VEC * static_cast<int>(sizeof(T));
+    const char* const my_ring = ring_mem + ring.weight_bytes + lane * VEC * static_cast<int>(sizeof(T));
     T* const my_dx = dx + lane * VEC;
     int stage = 0, stage_at = 0, slot = 0;
     uint32_t phase = 0;
@@ -442,7 +459,9 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
 #pragma unroll
             for (int j = 0; j < N; ++j) g[j] = h[j] = vsplat<V>(0.f);
           }
-          if constexpr (!HOLD) ln_weight<W, VEC>(w, c, cols, 1.f, fw[0]);
+          if constexpr (!HOLD) {
+            if (ln_inside<TPR, PER>(k, c, cols)) load_lanes<W, VEC>(held_w + c, fw[0]);
+          }
 #pragma unroll
           for (int j = 0; j < N; ++j) h[j] = vmul(vadd(h[j], minus), q);
         };
@@ -581,12 +600,14 @@ static LnSource ln_source(const void* p, int64_t rows, int64_t cols, int64_t ld,
   return LnSource{base, ld * size, base + ((rows - 1) * ld + cols) * size};
 }
 // The ring of a CTA: a few KB per stage (a row or a batch of them for a CTA-wide row, some for every warp otherwise) and as many stages as the CTA's
-// share of the shared memory holds.  stages < 2: the rows are too long.
-static LnRing ln_ring(int64_t cols, int size, int align, int operands, int groups, int per_sm, int batch) {
+// share of the shared memory holds.  stages < 1: the rows are too long.
+constexpr int LN_SMEM = 212 * 1024;     // shared memory that the CTAs of an SM divide
+static LnRing ln_ring(int64_t cols, int size, int align, int operands, int groups, int per_sm, int batch, int weight_size) {
   LnRing r;
   r.row_bytes = static_cast<int>((cols * size + 15) / 16 * 16) + (align == 16 ? 0 : 16);
   r.stage_rows = groups == 1 ? batch : r.row_bytes * operands <= 256 ? 4 * groups : r.row_bytes * operands <= 1024 ? 2 * groups : groups;
-  const int64_t stages = static_cast<int64_t>(208 * 1024) / per_sm / (static_cast<int64_t>(r.stage_rows) * r.row_bytes * operands);
+  r.weight_bytes = static_cast<int>((cols * weight_size + 15) / 16 * 16);
+  const int64_t stages = (static_cast<int64_t>(LN_SMEM) / per_sm - r.weight_bytes) / (static_cast<int64_t>(r.stage_rows) * r.row_bytes * operands);
   r.stages = static_cast<int>(stages > LN_MAX_STAGES ? LN_MAX_STAGES : stages);
   return r;
 }
@@ -594,11 +615,11 @@ static LnRing ln_ring(int64_t cols, int size, int align, int operands, int group
 template <typename T, typename W, int VEC, int PER, int TPR>
 static int ln_fwd_rows(const LayerNormArgs& a, int align, const DeviceInfo* dev, cudaStream_t stream, bool* done) {
   constexpr int GROUPS = ln_groups<TPR>(), PER_SM = ln_per_sm<TPR, false>(), BATCH = TPR == 512 && PER * VEC <= 16 ? 2 : 1;
-  const LnRing ring = ln_ring(a.cols, sizeof(T), align, 1, GROUPS, PER_SM, BATCH);
-  if (ring.stages < 2 || (TPR > 32 && a.cols <= TPR * VEC * (PER / 2))) return B200K_OK;   // the second is what ln_inside relies on
+  const LnRing ring = ln_ring(a.cols, sizeof(T), align, 1, GROUPS, PER_SM, BATCH, 0);
+  if (ring.stages < 1 || (TPR > 32 && a.cols <= TPR * VEC * (PER / 2))) return B200K_OK;   // the second is what ln_inside relies on
   auto kernel = ln_fwd_kernel<T, W, VEC, PER, TPR, BATCH>;
   const int smem = ring.stages * ring.stage_rows * ring.row_bytes;
-  B200K_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 208 * 1024));
+  B200K_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LN_SMEM));
   const int64_t most = (a.rows + ring.stage_rows - 1) / ring.stage_rows, grid = static_cast<int64_t>(dev->sm_count) * PER_SM;
   kernel<<<static_cast<unsigned>(most < grid ? most : grid), ln_threads<TPR>(), smem, stream>>>(
       ln_source(a.x, a.rows, a.cols, a.ldx, sizeof(T)), static_cast<const W*>(a.w), static_cast<const W*>(a.b), static_cast<T*>(a.y), a.mean, a.rstd,
@@ -612,11 +633,11 @@ static int ln_fwd_rows(const LayerNormArgs& a, int align, const DeviceInfo* dev,
 template <typename T, typename W, int VEC, int PER, int TPR>
 static int ln_bwd_rows(const LayerNormArgs& a, int align, const DeviceInfo* dev, float* part, int* parts, cudaStream_t stream, bool* done) {
   constexpr int GROUPS = ln_groups<TPR>(), PER_SM = ln_per_sm<TPR, true>();
-  const LnRing ring = ln_ring(a.cols, sizeof(T), align, 2, GROUPS, PER_SM, 1);
-  if (ring.stages < 2 || (TPR > 32 && a.cols <= TPR * VEC * (PER / 2))) return B200K_OK;   // the second is what ln_inside relies on
+  const LnRing ring = ln_ring(a.cols, sizeof(T), align, 2, GROUPS, PER_SM, 1, PER * VEC > 16 ? sizeof(W) : 0);
+  if (ring.stages < 1 || (TPR > 32 && a.cols <= TPR * VEC * (PER / 2))) return B200K_OK;   // the second is what ln_inside relies on
   auto kernel = ln_bwd_kernel<T, W, VEC, PER, TPR>;
-  const int smem = 2 * ring.stages * ring.stage_rows * ring.row_bytes;
-  B200K_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 208 * 1024));
+  const int smem = ring.weight_bytes + 2 * ring.stages * ring.stage_rows * ring.row_bytes;
+  B200K_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LN_SMEM));
   int64_t grid = (a.rows + ring.stage_rows - 1) / ring.stage_rows;
   if (grid > static_cast<int64_t>(dev->sm_count) * PER_SM) grid = static_cast<int64_t>(dev->sm_count) * PER_SM;
   if (grid > LN_MAX_PARTS) grid = LN_MAX_PARTS;
@@ -631,11 +652,12 @@ static int ln_bwd_rows(const LayerNormArgs& a, int align, const DeviceInfo* dev,
 }
 
 // Calls f with the kernel shape for rows of `cols` elements of `size` bytes whose operands share `align`: (VEC, PER, TPR) as integral constants.
-// 16 elements a thread or less, 32 beyond 8192; false beyond 16384 elements.  A warp takes a row of up to 512; a CTA-wide shape is the smallest one
+// 16 elements a thread or less; 32 beyond 8192, where no more threads are to be had, and for the backward's rows beyond 4096 that are read element
+// by element or by pairs (8192 x 7999 bf16: 144 -> 122 us, x 7998: 107 -> 102; with 16-byte accesses 16 are faster, x 8192: 103 against 118); false beyond 16384 elements.  A warp takes a row of up to 512; a CTA-wide shape is the smallest one
 // that holds the row, so that more than half of it is filled.
 template <int N>
 using Int = std::integral_constant<int, N>;
-template <int SIZE, typename F>
+template <int SIZE, bool BWD, typename F>
 static bool ln_shape(int64_t cols, int align, F&& f) {
   constexpr int V = 16 / SIZE;
   if (align == 16) {
@@ -657,7 +679,7 @@ static bool ln_shape(int64_t cols, int align, F&& f) {
     else if (cols <= 1024) f(Int<2>(), Int<4>(), Int<128>());
     else if (cols <= 2048) f(Int<2>(), Int<8>(), Int<128>());
     else if (cols <= 4096) f(Int<2>(), Int<8>(), Int<256>());
-    else if (cols <= 8192) f(Int<2>(), Int<8>(), Int<512>());
+    else if (cols <= 8192) f(Int<2>(), Int<BWD ? 16 : 8>(), Int<BWD ? 256 : 512>());
     else if (cols <= 16384) f(Int<2>(), Int<16>(), Int<512>());
     else return false;
     return true;
@@ -667,7 +689,7 @@ static bool ln_shape(int64_t cols, int align, F&& f) {
   else if (cols <= 1024) f(Int<1>(), Int<8>(), Int<128>());
   else if (cols <= 2048) f(Int<1>(), Int<16>(), Int<128>());
   else if (cols <= 4096) f(Int<1>(), Int<16>(), Int<256>());
-  else if (cols <= 8192) f(Int<1>(), Int<16>(), Int<512>());
+  else if (cols <= 8192) f(Int<1>(), Int<BWD ? 32 : 16>(), Int<BWD ? 256 : 512>());
   else if (cols <= 16384) f(Int<1>(), Int<32>(), Int<512>());
   else return false;
   return true;
@@ -687,7 +709,7 @@ static int ln_fwd(const LayerNormArgs& a, const DeviceInfo* dev, cudaStream_t st
   const int align = ln_common_alignment<T, W>(ln_alignment({reinterpret_cast<uintptr_t>(a.x), reinterpret_cast<uintptr_t>(a.y), a.cols * S, a.ldx * S, a.ldy * S}), a.w, a.b);
   int rc = B200K_OK;
   bool done = false;
-  if (a.rows < (int64_t(1) << 30)) ln_shape<S>(a.cols, align, [&](auto vec, auto per, auto tpr) { rc = ln_fwd_rows<T, W, vec(), per(), tpr()>(a, align, dev, stream, &done); });
+  if (a.rows < (int64_t(1) << 30)) ln_shape<S, false>(a.cols, align, [&](auto vec, auto per, auto tpr) { rc = ln_fwd_rows<T, W, vec(), per(), tpr()>(a, align, dev, stream, &done); });
   if (rc != B200K_OK || done) return rc;
   const unsigned grid = static_cast<unsigned>(a.rows < (1 << 30) ? a.rows : (1 << 30));
   ln_fwd_loop_kernel<T, W><<<grid, 512, 0, stream>>>(static_cast<const T*>(a.x), static_cast<const W*>(a.w), static_cast<const W*>(a.b),
@@ -704,7 +726,7 @@ static int ln_bwd_main(const LayerNormArgs& a, const DeviceInfo* dev, float* par
                                                             a.cols * S, a.ldx * S, a.lddy * S, a.dx == nullptr ? 0 : a.lddx * S}), a.w, nullptr);
   int rc = B200K_OK;
   bool done = false;
-  if (a.rows < (int64_t(1) << 30)) ln_shape<S>(a.cols, align, [&](auto vec, auto per, auto tpr) { rc = ln_bwd_rows<T, W, vec(), per(), tpr()>(a, align, dev, part, parts, stream, &done); });
+  if (a.rows < (int64_t(1) << 30)) ln_shape<S, true>(a.cols, align, [&](auto vec, auto per, auto tpr) { rc = ln_bwd_rows<T, W, vec(), per(), tpr()>(a, align, dev, part, parts, stream, &done); });
   if (rc != B200K_OK || done) return rc;
   const T* dy = static_cast<const T*>(a.dy);
   const T* x = static_cast<const T*>(a.x);
