@@ -253,6 +253,16 @@ def test_skipped_gradients_mixed_types_and_autograd():
 
 
 @pytest.mark.gpu
+def test_a_backward_pass_that_needs_the_old_values_fails():
+    w = torch.randn(32, device="cuda", requires_grad=True)
+    opt = tt.AdamW([w])
+    loss = (w * w).sum()
+    opt.step([torch.ones(32, device="cuda")])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("count", [41, 400, 401, 833])
 def test_many_tensors(count):
     shapes = [(1 + 37 * i % 500,) for i in range(count)]

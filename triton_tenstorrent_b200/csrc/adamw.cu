@@ -59,6 +59,7 @@ struct AdamwParams {
   // Powers of two that come as parameters: a shift and add by a constant would run on the ALU pipe, which the byte and bit work of the 8-bit moments
   // fills before anything else; a multiply-add by a number the compiler does not know runs on the FMA pipe.
   uint32_t two4, two5, two16, two19, two20;
+  float minus_zero;              // -0: what a product that must stay a rounded product is added to (see below)
   int n;                         // tensors in the table
   int advance;                   // this launch ends the step
 };
@@ -311,7 +312,7 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const __grid_const
 
   auto twice = [](float x) { return pack_f32x2(x, x); };
   const uint64_t k_scale = twice(grad_scale), k_b1 = twice(q.b1), k_c1 = twice(q.one_minus_b1), k_b2 = twice(q.b2), k_c2 = twice(q.one_minus_b2),
-                 k_bc2 = twice(inv_sqrt_bc2), k_eps = twice(q.eps), k_decay = twice(decay), k_step = twice(-step_size);
+                 k_bc2 = twice(inv_sqrt_bc2), k_eps = twice(q.eps), k_decay = twice(decay), k_step = twice(-step_size), k_zero = twice(q.minus_zero);
 
   // the next block's loads are under way while this one is worked on
   AdamwBlock<P, G, MASTER, BITS> next;
@@ -351,8 +352,10 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const __grid_const
           v2[j] = mul_f32x2(v2[j], v2[j]);
         }
         const uint64_t g2 = mul_f32x2(pack_f32x2(g[2 * j], g[2 * j + 1]), k_scale);
-        m2[j] = add_f32x2(mul_f32x2(m2[j], k_b1), mul_f32x2(g2, k_c1));
-        v2[j] = add_f32x2(mul_f32x2(v2[j], k_b2), mul_f32x2(mul_f32x2(g2, g2), k_c2));
+        // A packed product that only feeds a packed sum was seen merged with it into one multiply-add (a code in a million then differs): a
+        // multiply-add with a -0 that the compiler does not know is the product, and stays apart.
+        m2[j] = add_f32x2(fma_f32x2(m2[j], k_b1, k_zero), fma_f32x2(g2, k_c1, k_zero));
+        v2[j] = add_f32x2(fma_f32x2(v2[j], k_b2, k_zero), fma_f32x2(mul_f32x2(g2, g2), k_c2, k_zero));
       }
       sqrt4(v2, root[h]);
 #pragma unroll
@@ -545,6 +548,7 @@ int adamw(const AdamwArgs& a, cudaStream_t stream) {
   q.eps = static_cast<float>(a.eps);
   q.grad_scale = a.grad_scale;
   q.seed = a.seed;
+  q.minus_zero = -0.f;
   q.two4 = 1u << 4;
   q.two5 = 1u << 5;
   q.two16 = 1u << 16;

@@ -50,6 +50,8 @@ class AdamW:
         for i, p in enumerate(self.params):
             if not isinstance(p, torch.Tensor) or p.dtype not in _DTYPES:
                 raise TypeError(f"AdamW: parameter {i} must be an fp32, bf16 or fp16 tensor")
+            if p.is_inference():
+                raise ValueError(f"AdamW: parameter {i} is an inference tensor")
             if not p.is_cuda or p.device != self.params[0].device:
                 raise ValueError(f"AdamW: parameter {i} must live on the same CUDA device as the first one (got {p.device})")
             if not p.is_contiguous():
@@ -181,6 +183,8 @@ class AdamW:
                 table[:, _P:_G + 1] = pointers[:, 1:]
                 _lib.check(entry(table.ctypes.data, len(mine), _DTYPES[kind[0]], _DTYPES[kind[1]], self.state_bits, self._state.data_ptr(), lr, lr_ptr,
                                  b1, b2, self.eps, self.weight_decay, scale, scale_ptr, self.seed, int(k == len(order) - 1), stream))
+        # a backward pass that still needs an old value must fail instead of using the new one
+        torch.autograd.graph.increment_version([params[r[0]] for r in rows])
 
     def state_dict(self) -> dict:
         """The state as tensors (copies): step, the moments as they are held, and the master copy."""
