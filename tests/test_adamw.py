@@ -380,3 +380,53 @@ def test_entry_point_refusals():
     for blocks in (-1, 4):
         assert lib.b200k_adamw_moments(None, None, None, None, None, None, blocks, None) == _lib.ERR_INVALID_ARG
     assert ops._DTYPES[torch.bfloat16] == _lib.DTYPE_BF16
+
+
+def plain_decode(codes, scales, bits):
+    mag = (codes & ((1 << (4 + bits)) - 1)).to(torch.int32)
+    value = ((mag << (23 - bits)) + (127 << 23)).view(torch.float32)
+    value = torch.where(mag == 0, torch.zeros_like(value), value)
+    value = torch.where((codes >= 128) & (bits == 3), -value, value)
+    return (value.view(-1, BLOCK) * scales[:, None]).view(-1)
+
+
+def plain_encode(x, random16, bits):
+    mag = x.abs().view(-1, BLOCK)
+    exponent = ((mag.amax(dim=1).view(torch.int32) + ((1 << (24 - bits)) - 1)) >> 23).clamp(min=16)
+    scales, inverse = ((exponent - 15) << 23).view(torch.float32), ((269 - exponent) << 23).view(torch.float32)
+    y = (mag * inverse[:, None]).view(-1)
+    least = 1 + 2.0 ** -bits
+    raw = (y.view(torch.int32) - (127 << 23) + (random16 << (7 - bits)).to(torch.int32)) >> (23 - bits)
+    small = ((2 * random16 + 1).to(torch.float32) * (least * 2.0 ** -17) < y) if bits == 3 else y > 0
+    code = torch.where(y < least, small.to(torch.int32), raw)
+    return (torch.where(x < 0, code + 128, code) if bits == 3 else code).to(torch.uint8), scales
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("spread,size", [(0.0, 1.0), (1.5, 1e-3), (3.0, 1e-8), (6.0, 1e8), (12.0, 1.0), (12.0, 1e-18)])
+def test_8_bit_moments_equal_the_formula_in_ieee_fp32(spread, size):
+    """Every product, sum and root that reaches a moment is one IEEE operation in the order of the formula, so that scales and codes (but for the
+    sign of a zero) are equal, not near: nothing may be merged into a multiply-add, and the root is the correctly rounded one over the whole
+    range of a squared gradient, subnormal and near-overflowing ones included."""
+    n, steps = 1 << 21, 3
+    g = torch.Generator(device="cuda").manual_seed(int(spread * 10))
+    rn = lambda: torch.randn(n, generator=g, device="cuda")  # noqa: E731
+    opt = tt.AdamW([torch.zeros(n, device="cuda")], betas=(0.9, 0.999), state_bits=8, seed=9)
+    m8 = r8 = torch.zeros(n, dtype=torch.uint8, device="cuda")
+    ms = rs = torch.zeros(n // BLOCK, device="cuda")
+    for t in range(1, steps + 1):
+        grad = (rn() * torch.exp(rn() * spread) * size).clamp(-1e19, 1e19)
+        grad[torch.rand(n, generator=g, device="cuda") < 0.05] = 0.0
+        grad[: 4 * BLOCK] = 0.0
+        opt.step([grad])
+        m = plain_decode(m8, ms, 3) * 0.9 + grad * (1 - 0.9)
+        r = plain_decode(r8, rs, 4)
+        root = torch.sqrt(r * r * 0.999 + (grad * grad) * (1 - 0.999))
+        lo, hi = (torch.from_numpy(x).cuda() for x in random16(n, 0, t, 9))
+        m8, ms = plain_encode(m, lo, 3)
+        r8, rs = plain_encode(root, hi, 4)
+        held = opt.state_dict()
+        assert torch.equal(held["exp_avg_scale"], ms) and torch.equal(held["exp_avg_sq_root_scale"], rs)
+        assert torch.equal(held["exp_avg_sq_root"], r8)
+        got = held["exp_avg"]
+        assert bool(((got == m8) | ((got & 127 == 0) & (m8 & 127 == 0))).all())

@@ -59,7 +59,6 @@ struct AdamwParams {
   // Powers of two that come as parameters: a shift and add by a constant would run on the ALU pipe, which the byte and bit work of the 8-bit moments
   // fills before anything else; a multiply-add by a number the compiler does not know runs on the FMA pipe.
   uint32_t two4, two5, two16, two19, two20;
-  float minus_zero;              // -0: what a product that must stay a rounded product is added to (see below)
   int n;                         // tensors in the table
   int advance;                   // this launch ends the step
 };
@@ -233,15 +232,12 @@ __device__ __forceinline__ uint64_t sqrt_in_range(uint64_t x) {
   h = fma_f32x2(h, r, h);
   return fma_f32x2(fma_f32x2(g, g, mul_f32x2(x, pack_f32x2(-1.f, -1.f))), h, g);
 }
-__device__ __forceinline__ void sqrt4(const uint64_t (&x)[2], float (&root)[4]) {
-  float f[4];
-  unpack_f32x2(x[0], f[0], f[1]);
-  unpack_f32x2(x[1], f[2], f[3]);
+__device__ __forceinline__ void sqrt4(const float (&f)[4], float (&root)[4]) {
   const float lo = min3(min3(f[0], f[1], f[2]), f[3], f[3]);
   const float hi = max_nan(max_nan(f[0], f[1], f[2]), f[3], f[3]);
   if (lo >= 0x1p-60f && hi <= 0x1p120f) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) unpack_f32x2(sqrt_in_range(x[j]), root[2 * j], root[2 * j + 1]);
+    for (int j = 0; j < 2; ++j) unpack_f32x2(sqrt_in_range(pack_f32x2(f[2 * j], f[2 * j + 1])), root[2 * j], root[2 * j + 1]);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j) root[j] = __fsqrt_rn(f[j]);
@@ -310,10 +306,6 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const __grid_const
   P* const tp = static_cast<P*>(t.p);
   const bool aligned = ((reinterpret_cast<uintptr_t>(tp) & (4 * sizeof(P) - 1)) | (reinterpret_cast<uintptr_t>(t.g) & (4 * sizeof(G) - 1))) == 0;
 
-  auto twice = [](float x) { return pack_f32x2(x, x); };
-  const uint64_t k_scale = twice(grad_scale), k_b1 = twice(q.b1), k_c1 = twice(q.one_minus_b1), k_b2 = twice(q.b2), k_c2 = twice(q.one_minus_b2),
-                 k_bc2 = twice(inv_sqrt_bc2), k_eps = twice(q.eps), k_decay = twice(decay), k_step = twice(-step_size), k_zero = twice(q.minus_zero);
-
   // the next block's loads are under way while this one is worked on
   AdamwBlock<P, G, MASTER, BITS> next;
   int64_t base = begin + warp * ADAMW_BLOCK;
@@ -340,38 +332,26 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const __grid_const
         values4<float>(now.m[h], m);
         values4<float>(now.v[h], v);
       }
-      // two elements at a time: each product and sum is rounded as a scalar one
-      uint64_t m2[2], v2[2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        m2[j] = pack_f32x2(m[2 * j], m[2 * j + 1]);
-        v2[j] = pack_f32x2(v[2 * j], v[2 * j + 1]);
+      for (int j = 0; j < 4; ++j) {
         if (BITS == 8) {
-          m2[j] = mul_f32x2(m2[j], pack_f32x2(now.scale_m, now.scale_m));
-          v2[j] = mul_f32x2(v2[j], pack_f32x2(now.scale_r, now.scale_r));
-          v2[j] = mul_f32x2(v2[j], v2[j]);
+          m[j] = __fmul_rn(m[j], now.scale_m);
+          v[j] = __fmul_rn(v[j], now.scale_r);
+          v[j] = __fmul_rn(v[j], v[j]);
         }
-        const uint64_t g2 = mul_f32x2(pack_f32x2(g[2 * j], g[2 * j + 1]), k_scale);
-        // A packed product that only feeds a packed sum was seen merged with it into one multiply-add (a code in a million then differs): a
-        // multiply-add with a -0 that the compiler does not know is the product, and stays apart.
-        m2[j] = add_f32x2(fma_f32x2(m2[j], k_b1, k_zero), fma_f32x2(g2, k_c1, k_zero));
-        v2[j] = add_f32x2(fma_f32x2(v2[j], k_b2, k_zero), fma_f32x2(mul_f32x2(g2, g2), k_c2, k_zero));
+        g[j] = __fmul_rn(g[j], grad_scale);
+        m[j] = __fadd_rn(__fmul_rn(m[j], q.b1), __fmul_rn(g[j], q.one_minus_b1));
+        v[j] = __fadd_rn(__fmul_rn(v[j], q.b2), __fmul_rn(__fmul_rn(g[j], g[j]), q.one_minus_b2));
+        m1[h][j] = m[j];
       }
-      sqrt4(v2, root[h]);
+      sqrt4(v, root[h]);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < 4; ++j) {
         // p alone may round otherwise than the plain formula: the quotient takes an approximate reciprocal (1 unit in the last place), of an
         // update that is itself a small part of p.  The divisor is zero or a normal number: sqrt of the smallest fp32 is 2^-74.5.
-        float d0, d1;
-        unpack_f32x2(fma_f32x2(pack_f32x2(root[h][2 * j], root[h][2 * j + 1]), k_bc2, k_eps), d0, d1);
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d0) : "f"(d0));
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d1) : "f"(d1));
-        const uint64_t update = mul_f32x2(m2[j], pack_f32x2(d0, d1));
-        unpack_f32x2(fma_f32x2(update, k_step, mul_f32x2(pack_f32x2(p[2 * j], p[2 * j + 1]), k_decay)), p[2 * j], p[2 * j + 1]);
-        unpack_f32x2(m2[j], m[2 * j], m[2 * j + 1]);
-        unpack_f32x2(v2[j], v[2 * j], v[2 * j + 1]);
-        m1[h][2 * j] = m[2 * j];
-        m1[h][2 * j + 1] = m[2 * j + 1];
+        float inverse;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(fmaf(root[h][j], inv_sqrt_bc2, q.eps)));
+        p[j] = p[j] * decay - m[j] * inverse * step_size;
       }
       if (BITS == 8) {                     // behind the tensor's end all of it is zero
         peak_m = max_nan(max_nan(peak_m, fabsf(m[0]), fabsf(m[1])), fabsf(m[2]), fabsf(m[3]));
@@ -548,7 +528,6 @@ int adamw(const AdamwArgs& a, cudaStream_t stream) {
   q.eps = static_cast<float>(a.eps);
   q.grad_scale = a.grad_scale;
   q.seed = a.seed;
-  q.minus_zero = -0.f;
   q.two4 = 1u << 4;
   q.two5 = 1u << 5;
   q.two16 = 1u << 16;

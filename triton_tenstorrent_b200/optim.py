@@ -91,7 +91,9 @@ class AdamW:
         table[:, _N] = [p.numel() for p in self.params]
         table[:, _INDEX] = np.arange(len(self.params))
         self._table = table
-        self._shapes, self._empty = [p.shape for p in self.params], [p.numel() == 0 for p in self.params]
+        self._shapes = [p.shape for p in self.params]
+        kinds = {p.dtype for p in self.params}
+        self._dtype = kinds.pop() if len(kinds) == 1 and all(p.numel() for p in self.params) else None     # the one type, if there is one
 
     def _check_hyper(self):
         if isinstance(self.lr, torch.Tensor):
@@ -150,41 +152,59 @@ class AdamW:
             if lr.device != self.device:
                 raise ValueError(f"AdamW: lr must be on {self.device}")
             lr, lr_ptr = 0.0, lr.data_ptr()
-        rows, kinds, changed = [], [], False
-        at, strided = self.device.index, torch.strided
-        for i, (p, g, shape) in enumerate(zip(params, grads, self._shapes)):
-            if g is None or self._empty[i]:
+        # the usual case first, in few steps per tensor: every gradient there, one type each, nothing to copy
+        at, shapes, table, first = self.device.index, self._shapes, self._table, grads[0]
+        dtype, gdtype = self._dtype, None if first is None else first.dtype
+        try:
+            usual = (dtype is not None and (gdtype is dtype or gdtype is torch.float32)
+                     and all([g is not None and g.dtype is gdtype and g.shape == s and g.is_contiguous() and g.get_device() == at
+                              for g, s in zip(grads, shapes)])
+                     and all([p.dtype is dtype and p.shape == s and p.is_contiguous() and p.get_device() == at for p, s in zip(params, shapes)]))
+        except RuntimeError:        # a sparse gradient has no contiguity
+            usual = False
+        if usual:
+            table[:, _P] = [p.data_ptr() for p in params]
+            table[:, _G] = [g.data_ptr() for g in grads]
+            launches, touched = [(dtype, gdtype, table)], params
+        else:
+            launches, touched, grads = self._sort(grads)
+            if not touched:
+                return
+        entry = _lib.load().b200k_adamw
+        b1, b2 = self.betas
+        with _on(self.device):
+            stream = _stream()
+            for k, (dtype, gdtype, rows) in enumerate(launches):
+                _lib.check(entry(rows.ctypes.data, len(rows), _DTYPES[dtype], _DTYPES[gdtype], self.state_bits, self._state.data_ptr(), lr, lr_ptr,
+                                 b1, b2, self.eps, self.weight_decay, scale, scale_ptr, self.seed, int(k == len(launches) - 1), stream))
+        # a backward pass that still needs an old value must fail instead of using the new one
+        torch.autograd.graph.increment_version(touched)
+
+    def _sort(self, grads):
+        """The general case of step(): ([(parameter type, gradient type, table)], the parameters that take part, the gradients with copies of
+        those that are not contiguous)."""
+        grads, rows, touched = list(grads), {}, []
+        at = self.device.index
+        for i, (p, g, shape) in enumerate(zip(self.params, grads, self._shapes)):
+            if g is None or shape.numel() == 0:
                 continue
-            dtype, gdtype = p.dtype, g.dtype
-            if gdtype is not dtype and gdtype is not torch.float32:
-                raise TypeError(f"AdamW: gradient {i} must be {dtype} or torch.float32, got {gdtype}")
-            if g.shape != shape or g.get_device() != at or g.layout is not strided:
+            if g.dtype is not p.dtype and g.dtype is not torch.float32:
+                raise TypeError(f"AdamW: gradient {i} must be {p.dtype} or torch.float32, got {g.dtype}")
+            if g.shape != shape or g.get_device() != at or g.layout is not torch.strided:
                 raise ValueError(f"AdamW: gradient {i} must be a dense {tuple(shape)} tensor on {self.device}, got {tuple(g.shape)} on {g.device}")
             if p.shape != shape or not p.is_contiguous() or p.get_device() != at:
                 raise ValueError(f"AdamW: parameter {i} is no longer a contiguous {tuple(shape)} tensor on {self.device}")
             if not g.is_contiguous():
-                g = g.contiguous()
-                if not changed:
-                    grads, changed = list(grads), True
-                grads[i] = g            # holds the copy until the launch
-            rows.append((i, p.data_ptr(), g.data_ptr()))
-            kinds.append((dtype, gdtype))
-        if not rows:
-            return
-        entry = _lib.load().b200k_adamw
-        b1, b2 = self.betas
-        order = list(dict.fromkeys(kinds))
-        with _on(self.device):
-            stream = _stream()
-            for k, kind in enumerate(order):
-                mine = rows if len(order) == 1 else [r for r, x in zip(rows, kinds) if x == kind]
-                pointers = np.array(mine, dtype=np.int64)
-                table = self._table if len(mine) == len(params) else self._table[pointers[:, 0]]
-                table[:, _P:_G + 1] = pointers[:, 1:]
-                _lib.check(entry(table.ctypes.data, len(mine), _DTYPES[kind[0]], _DTYPES[kind[1]], self.state_bits, self._state.data_ptr(), lr, lr_ptr,
-                                 b1, b2, self.eps, self.weight_decay, scale, scale_ptr, self.seed, int(k == len(order) - 1), stream))
-        # a backward pass that still needs an old value must fail instead of using the new one
-        torch.autograd.graph.increment_version([params[r[0]] for r in rows])
+                g = grads[i] = g.contiguous()
+            rows.setdefault((p.dtype, g.dtype), []).append((i, p.data_ptr(), g.data_ptr()))
+            touched.append(p)
+        launches = []
+        for (dtype, gdtype), mine in rows.items():
+            pointers = np.array(mine, dtype=np.int64)
+            table = self._table[pointers[:, 0]]
+            table[:, _P:_G + 1] = pointers[:, 1:]
+            launches.append((dtype, gdtype, table))
+        return launches, touched, grads
 
     def state_dict(self) -> dict:
         """The state as tensors (copies): step, the moments as they are held, and the master copy."""
