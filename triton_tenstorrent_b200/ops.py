@@ -561,11 +561,12 @@ def _norm_weight(name, x, t, like=None):
     """weight / bias of a norm: [last dimension], x's type or fp32, on x's device."""
     if t is None:
         return None
-    if t.dtype not in (x.dtype, torch.float32):
-        raise TypeError(f"layer_norm: {name} must be {x.dtype} or torch.float32, got {t.dtype}")
-    if like is not None and t.dtype != like.dtype:
-        raise TypeError(f"layer_norm: weight and bias have different types {like.dtype} and {t.dtype}")
-    if tuple(t.shape) != (x.shape[-1],):
+    dtype = t.dtype
+    if dtype is not x.dtype and dtype is not torch.float32:
+        raise TypeError(f"layer_norm: {name} must be {x.dtype} or torch.float32, got {dtype}")
+    if like is not None and dtype is not like.dtype:
+        raise TypeError(f"layer_norm: weight and bias have different types {like.dtype} and {dtype}")
+    if t.dim() != 1 or t.shape[0] != x.shape[-1]:
         raise ValueError(f"layer_norm: {name} must be [{x.shape[-1]}], got {tuple(t.shape)}")
     if t.device != x.device:
         raise ValueError("layer_norm: tensors on different devices")
@@ -612,10 +613,10 @@ def layer_norm_with_stats(x, weight=None, bias=None, eps: float = 1e-5):
     _layer_norm_check(x, weight, bias, eps)
     if not x.is_cuda:
         _require_cuda()
-    stats = torch.empty((2, *x.shape[:-1]), device=x.device if x.is_cuda else "cuda", dtype=torch.float32)
-    y = _layer_norm_call(x, weight, bias, eps, stats)
-    mean, rstd = stats.unbind(0)
-    return _like_input(y, x), _like_input(mean, x), _like_input(rstd, x)
+        stats = torch.empty((2, *x.shape[:-1]), device="cuda", dtype=torch.float32)
+        return (_layer_norm_call(x, weight, bias, eps, stats).cpu(), *stats.cpu().unbind(0))
+    stats = torch.empty((2, *x.shape[:-1]), device=x.device, dtype=torch.float32)
+    return (_layer_norm_call(x, weight, bias, eps, stats), *stats.unbind(0))
 
 
 def layer_norm_backward(dy, x, weight, mean, rstd, need_dx: bool = True, need_dw: bool = True, need_db: bool = True):
@@ -623,31 +624,37 @@ def layer_norm_backward(dy, x, weight, mean, rstd, need_dx: bool = True, need_dw
     layer_norm_with_stats returned.  dw and db have the weight's type (fp32 without a weight).  A gradient that is not needed is None; a
     frozen norm then reads x and dy once only."""
     _norm_input("layer_norm_backward", x)
-    if dy.shape != x.shape or dy.dtype != x.dtype:
-        raise ValueError(f"layer_norm_backward: dy must be {x.dtype} {tuple(x.shape)} like x, got {dy.dtype} {tuple(dy.shape)}")
-    if any(t.dtype != torch.float32 or t.shape != x.shape[:-1] for t in (mean, rstd)):
-        raise ValueError(f"layer_norm_backward: mean and rstd must be fp32 {tuple(x.shape[:-1])}")
-    if any(t.device != x.device for t in (dy, mean, rstd)):
+    shape, rows_shape, dtype, device = x.shape, x.shape[:-1], x.dtype, x.device
+    if dy.shape != shape or dy.dtype is not dtype:
+        raise ValueError(f"layer_norm_backward: dy must be {dtype} {tuple(shape)} like x, got {dy.dtype} {tuple(dy.shape)}")
+    if mean.dtype is not torch.float32 or rstd.dtype is not torch.float32 or mean.shape != rows_shape or rstd.shape != rows_shape:
+        raise ValueError(f"layer_norm_backward: mean and rstd must be fp32 {tuple(rows_shape)}")
+    if dy.device != device or mean.device != device or rstd.device != device:
         raise ValueError("layer_norm_backward: tensors on different devices")
     w = _norm_weight("weight", x, weight)
     lib = _lib.load()
-    w = None if w is None else _to_device(w).contiguous()
-    xd, gd = _rows_of(_to_device(x)), _rows_of(_to_device(dy))
-    md, rd = (_to_device(t).contiguous() for t in (mean, rstd))
+    host = not x.is_cuda
+    if host:
+        w = None if w is None else _to_device(w)
+        x, dy, mean, rstd = (_to_device(t) for t in (x, dy, mean, rstd))
+    xd, gd = _rows_of(x), _rows_of(dy)
+    md, rd = mean if mean.is_contiguous() else mean.contiguous(), rstd if rstd.is_contiguous() else rstd.contiguous()
+    w = w if w is None or w.is_contiguous() else w.contiguous()
     rows, cols = xd.shape
     wtype = torch.float32 if w is None else w.dtype
-    dx = torch.empty((rows, cols), device=xd.device, dtype=x.dtype) if need_dx else None
+    dx = torch.empty(shape, device=xd.device, dtype=dtype) if need_dx else None
     dw = torch.empty(cols, device=xd.device, dtype=wtype) if need_dw else None
     db = torch.empty(cols, device=xd.device, dtype=wtype) if need_db else None
     floats = lib.b200k_layer_norm_bwd_workspace(rows, cols) if need_dw or need_db else 0
-    work = torch.empty(floats, device=xd.device, dtype=torch.float32)
-    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    work = torch.empty(floats, device=xd.device, dtype=torch.float32) if floats else None
     with _on(xd.device):
-        _lib.check(lib.b200k_layer_norm_bwd(gd.data_ptr(), xd.data_ptr(), ptr(w), md.data_ptr(), rd.data_ptr(), ptr(dx), ptr(dw), ptr(db),
-                                            work.data_ptr(), floats, rows, cols, _pitch(gd), _pitch(xd), cols, _DTYPES[x.dtype],
-                                            _DTYPES[wtype], _stream()))
-    return (None if dx is None else _like_input(dx.view(x.shape), x), None if dw is None else _like_input(dw, x),
-            None if db is None else _like_input(db, x))
+        _lib.check(lib.b200k_layer_norm_bwd(gd.data_ptr(), xd.data_ptr(), 0 if w is None else w.data_ptr(), md.data_ptr(), rd.data_ptr(),
+                                            0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(),
+                                            0 if db is None else db.data_ptr(), 0 if work is None else work.data_ptr(), floats, rows, cols,
+                                            _pitch(gd), _pitch(xd), cols, _DTYPES[dtype], _DTYPES[wtype], _stream()))
+    if host:
+        return tuple(None if t is None else t.cpu() for t in (dx, dw, db))
+    return dx, dw, db
 
 
 class _layer_norm(torch.autograd.Function):
