@@ -212,20 +212,10 @@ __device__ __forceinline__ void ln_fetch_all(const LnSource (&src)[NSRC], const 
 }
 
 // Sums over the TPR threads of a row; every thread gets them.  A CTA-wide sum takes a slot of `scratch` of its own per call in a row of calls (two
-// suffice: a barrier lies between the reads of one call and the writes of the call after the next).
-template <int WARPS>
-__device__ __forceinline__ float2 join_warps(const float2* scratch) {
-  float2 v = make_float2(0.f, 0.f);
-#pragma unroll
-  for (int i = 0; i < WARPS; i += 2) {
-    const float4 t = *reinterpret_cast<const float4*>(scratch + i);
-    v.x += t.x + t.z;
-    v.y += t.y + t.w;
-  }
-  return v;
-}
+// suffice: a barrier lies between the reads of one call and the writes of the call after the next).  Across warps the partial sums are joined by
+// shuffles too: with 16 warps, reading all of them in every thread costs 48 instructions a warp and row against 11.
 template <int TPR>
-__device__ __forceinline__ float2 row_sum2(float2 v, float2 (*scratch)[32], int slot) {
+__device__ __forceinline__ float2 row_sum2(float2 v, float (*scratch)[32], int slot) {
   const int lane = threadIdx.x & 31;
   // the lower half of the warp goes on with x, the upper half with y
   const bool upper = lane >= 16;
@@ -233,13 +223,36 @@ __device__ __forceinline__ float2 row_sum2(float2 v, float2 (*scratch)[32], int 
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
   if constexpr (TPR > 32) {
-    float* mine = &scratch[slot][threadIdx.x >> 5].x;
-    if ((lane & 15) == 0) mine[lane >> 4] = t;
+    constexpr int WARPS = TPR / 32;
+    static_assert(WARPS <= 16, "half a warp joins them");
+    if ((lane & 15) == 0) scratch[slot][(threadIdx.x >> 5) + (lane & 16)] = t;
     named_bar_sync(1, TPR);
-    return join_warps<TPR / 32>(scratch[slot]);
-  } else {
-    return make_float2(__shfl_sync(0xFFFFFFFFu, t, 0), __shfl_sync(0xFFFFFFFFu, t, 16));
+    t = scratch[slot][(lane & (WARPS - 1)) + (lane & 16)];
+#pragma unroll
+    for (int o = WARPS / 2; o > 0; o >>= 1) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
   }
+  return make_float2(__shfl_sync(0xFFFFFFFFu, t, 0), __shfl_sync(0xFFFFFFFFu, t, 16));
+}
+template <int TPR>
+__device__ __forceinline__ float row_sum(float t, float (*scratch)[32], int slot) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
+  if constexpr (TPR > 32) {
+    constexpr int WARPS = TPR / 32;
+    if (lane == 0) scratch[slot][threadIdx.x >> 5] = t;
+    named_bar_sync(1, TPR);
+    t = scratch[slot][lane & (WARPS - 1)];
+#pragma unroll
+    for (int o = WARPS / 2; o > 0; o >>= 1) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
+  }
+  return t;
+}
+// The sums of one row (in x) or of two.
+template <int TPR, int BATCH>
+__device__ __forceinline__ float2 batch_sum(float2 v, float (*scratch)[32], int slot) {
+  if constexpr (BATCH == 2) return row_sum2<TPR>(v, scratch, slot);
+  return make_float2(row_sum<TPR>(v.x, scratch, slot), 0.f);
 }
 
 // One access of w or b, or what stands for it where there is none.
@@ -264,7 +277,7 @@ ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ 
   constexpr int N = Lanes<VEC>::N;
   extern __shared__ __align__(16) char ring_mem[];
   __shared__ uint64_t full[LN_MAX_STAGES], empty[LN_MAX_STAGES];
-  __shared__ __align__(16) float2 scratch[2][32];
+  __shared__ float scratch[2][32];
   __shared__ uint32_t abort_flag;
   if (threadIdx.x < LN_MAX_STAGES) {
     mbar_init(&full[threadIdx.x], 1);
@@ -318,7 +331,7 @@ ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ 
           }
           (h == 0 ? s.x : s.y) = vsum(t);
         }
-        s = row_sum2<TPR>(s, scratch, 0);
+        s = batch_sum<TPR, BATCH>(s, scratch, 0);
         if (TPR > 32 && lane == 0) mbar_arrive(&empty[stage]);       // every thread holds its part of the stage's rows in registers
         const float mu[2] = {s.x * inv_n, s.y * inv_n};
         s = make_float2(0.f, 0.f);
@@ -338,7 +351,7 @@ ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ 
           }
           (h == 0 ? s.x : s.y) = vsum(t);
         }
-        s = row_sum2<TPR>(s, scratch, 1);
+        s = batch_sum<TPR, BATCH>(s, scratch, 1);
         const float rs[2] = {rsqrtf(s.x * inv_n + eps), rsqrtf(s.y * inv_n + eps)};
 #pragma unroll
         for (int h = 0; h < BATCH; ++h) {
@@ -388,7 +401,7 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
   constexpr int N = Lanes<VEC>::N;
   extern __shared__ __align__(16) char ring_mem[];
   __shared__ uint64_t full[LN_MAX_STAGES], empty[LN_MAX_STAGES];
-  __shared__ __align__(16) float2 scratch[2][32];
+  __shared__ float scratch[2][32];
   __shared__ uint32_t abort_flag;
   if (threadIdx.x < LN_MAX_STAGES) {
     mbar_init(&full[threadIdx.x], 1);
@@ -438,7 +451,9 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
       for (int i = group; i < stage_rows; i += GROUPS) {
         r = top + i;
         if (TPR == 32 && r >= rows) break;
-        const V minus = vsplat<V>(-mu), q = vsplat<V>(rs);
+        // h = x rstd - mean rstd: the product rounded once is as far off as the mean itself, which is rounded too
+        const V shift = vsplat<V>(-mu * rs), q = vsplat<V>(rs);
+        const float rs_now = rs;
         {                                                       // the next row's statistics
           const int n = i + GROUPS < stage_rows ? r + GROUPS : top + gridDim.x * stage_rows + group;
           if (n < rows) {
@@ -463,7 +478,7 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
             if (ln_inside<TPR, PER>(k, c, cols)) load_lanes<W, VEC>(held_w + c, fw[0]);
           }
 #pragma unroll
-          for (int j = 0; j < N; ++j) h[j] = vmul(vadd(h[j], minus), q);
+          for (int j = 0; j < N; ++j) h[j] = vfma(h[j], q, shift);
         };
         V g[HOLD ? PER : 1][N], h[HOLD ? PER : 1][N];
         V s1 = vsplat<V>(0.f), s2 = vsplat<V>(0.f);
@@ -489,7 +504,7 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
         s = row_sum2<TPR>(s, scratch, slot);
         slot ^= 1;
         if (dx != nullptr) {
-          const V c1 = vsplat<V>(-s.x * inv_n), c2 = vsplat<V>(-s.y * inv_n);
+          const V c1 = vsplat<V>(-s.x * inv_n * rs_now), c2 = vsplat<V>(-s.y * inv_n * rs_now);
           T* out = my_dx + r * lddx;
 #pragma unroll
           for (int k = 0; k < PER; ++k) {
@@ -502,7 +517,7 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
               for (int j = 0; j < N; ++j) gk[j] = vmul(gk[j], fw[0][j]);
             }
 #pragma unroll
-            for (int j = 0; j < N; ++j) gk[j] = vmul(vfma(hk[j], c2, vadd(gk[j], c1)), q);
+            for (int j = 0; j < N; ++j) gk[j] = vfma(hk[j], c2, vfma(gk[j], q, c1));
             if (ln_inside<TPR, PER>(k, c, cols)) store_lanes<T, VEC>(out + k * TPR * VEC, gk);
           }
         }
