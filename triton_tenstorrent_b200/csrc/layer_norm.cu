@@ -125,8 +125,12 @@ constexpr int LN_GROUPS = 8;          // rows at a time of a CTA whose warps tak
 constexpr int LN_MAX_STAGES = 8;
 template <int TPR>
 __host__ __device__ constexpr int ln_groups() { return TPR == 32 ? LN_GROUPS : 1; }
-template <int TPR>
-__host__ __device__ constexpr int ln_threads() { return TPR * ln_groups<TPR>() + 32; }
+// With rows on 16-byte boundaries and a CTA per row, fetching a row is two instructions, and the first thread does it behind the barrier of the
+// row sum: a fetching warp would cost the others registers (17 warps leave them 96 each, 16 warps 128).
+template <typename T, int VEC, int PER, int TPR>
+__host__ __device__ constexpr bool ln_self_fetch() { return TPR > 32 && VEC * sizeof(T) == 16 && PER * VEC <= 16; }
+template <typename T, int VEC, int PER, int TPR>
+__host__ __device__ constexpr int ln_threads() { return TPR * ln_groups<TPR>() + (ln_self_fetch<T, VEC, PER, TPR>() ? 0 : 32); }
 // CTAs of one SM.  The backward writes a partial sum per CTA, so that it takes fewer.
 template <int TPR, bool BWD>
 __host__ __device__ constexpr int ln_per_sm() {
@@ -170,6 +174,15 @@ __device__ __noinline__ void ln_patch(const char* a, int row_len, const char* fr
   const char* tail = bytes == 0 || from + bytes < a ? a : from + bytes;
   for (const char* q = a; q < head; q += sizeof(T)) *reinterpret_cast<T*>(dst + (q - a)) = *reinterpret_cast<const T*>(q);
   for (const char* q = tail; q < z; q += sizeof(T)) *reinterpret_cast<T*>(dst + (q - a)) = *reinterpret_cast<const T*>(q);
+}
+
+// One thread fetches `count` rows (from r on) of each operand into a stage; rows on 16-byte boundaries.
+template <int NSRC>
+__device__ __forceinline__ void ln_fetch_rows(const LnSource (&src)[NSRC], int row_bytes, int r, int count, char* stage, uint64_t* bar) {
+  mbar_expect_tx(bar, static_cast<uint32_t>(NSRC * count * row_bytes));
+  for (int i = 0; i < count; ++i)
+#pragma unroll
+    for (int k = 0; k < NSRC; ++k) bulk_load(stage + (i * NSRC + k) * row_bytes, src[k].base + (r + i) * src[k].pitch, row_bytes, bar);
 }
 
 // The fetching warp: blocks of stage_rows rows, a lane per row.
@@ -268,7 +281,7 @@ __device__ __forceinline__ void ln_weight(const W* w, int c, int cols, float dfl
 
 // BATCH rows are worked on at a time (1 or 2): with one CTA on an SM a second row fills the waits of the first.
 template <typename T, typename W, int VEC, int PER, int TPR, int BATCH>
-__global__ void __launch_bounds__(ln_threads<TPR>(), ln_per_sm<TPR, false>())
+__global__ void __launch_bounds__(ln_threads<T, VEC, PER, TPR>(), ln_per_sm<TPR, false>())
 ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ b, T* __restrict__ y, float* __restrict__ mean,
               float* __restrict__ rstd, int rows, int cols, int64_t ldy, float eps, const LnRing ring, uint32_t* status) {
   constexpr int GROUPS = ln_groups<TPR>();
@@ -288,8 +301,9 @@ ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ 
   __syncthreads();
   const WaitCtx ctx{&abort_flag, status};
   const int group = threadIdx.x / TPR;
-  if (group == GROUPS) {
-    const LnSource src[1] = {sx};
+  constexpr bool SELF = ln_self_fetch<T, VEC, PER, TPR>();
+  const LnSource src[1] = {sx};
+  if (!SELF && group == GROUPS) {
     ln_fetch_all<T, 1>(src, ring, rows, cols * static_cast<int>(sizeof(T)), ring_mem, full, empty, ctx);
   } else {
     const int lane = threadIdx.x % TPR;
@@ -303,6 +317,12 @@ ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ 
     }
     const float inv_n = 1.f / static_cast<float>(cols);
     const int stage_rows = TPR == 32 ? ring.stage_rows : BATCH;
+    const int64_t ahead = static_cast<int64_t>(gridDim.x) * BATCH * ring.stages;      // from a stage's rows to its next ones
+    if (SELF && threadIdx.x == 0)
+      for (int i = 0; i < ring.stages; ++i) {
+        const int64_t r = (blockIdx.x + static_cast<int64_t>(i) * gridDim.x) * BATCH;
+        if (r < rows) ln_fetch_rows<1>(src, ring.row_bytes, static_cast<int>(r), min(BATCH, rows - static_cast<int>(r)), ring_mem + i * BATCH * ring.row_bytes, &full[i]);
+      }
     const char* const my_ring = ring_mem + lane * VEC * static_cast<int>(sizeof(T));
     T* const my_y = y + lane * VEC;
     int stage = 0, stage_at = 0;
@@ -332,7 +352,16 @@ ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ 
           (h == 0 ? s.x : s.y) = vsum(t);
         }
         s = batch_sum<TPR, BATCH>(s, scratch, 0);
-        if (TPR > 32 && lane == 0) mbar_arrive(&empty[stage]);       // every thread holds its part of the stage's rows in registers
+        if (TPR > 32 && lane == 0) {                                 // every thread holds its part of the stage's rows in registers
+          if constexpr (SELF) {
+            if (top + ahead < rows) {
+              const int n = static_cast<int>(top + ahead);
+              ln_fetch_rows<1>(src, ring.row_bytes, n, min(BATCH, rows - n), ring_mem + stage_at, &full[stage]);
+            }
+          } else {
+            mbar_arrive(&empty[stage]);
+          }
+        }
         const float mu[2] = {s.x * inv_n, s.y * inv_n};
         s = make_float2(0.f, 0.f);
 #pragma unroll
@@ -390,7 +419,7 @@ ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ 
 
 // Backward.  The columns' sums of dy h and dy stay in registers until the end: one partial sum per CTA (part[2][gridDim.x][cols], first dw's).
 template <typename T, typename W, int VEC, int PER, int TPR>
-__global__ void __launch_bounds__(ln_threads<TPR>(), ln_per_sm<TPR, true>())
+__global__ void __launch_bounds__(ln_threads<T, VEC, PER, TPR>(), ln_per_sm<TPR, true>())
 ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, const float* __restrict__ mean, const float* __restrict__ rstd,
               T* __restrict__ dx, float* __restrict__ part, int rows, int cols, int64_t lddx, const LnRing ring, uint32_t* status) {
   constexpr int GROUPS = ln_groups<TPR>();
@@ -412,8 +441,9 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
   __syncthreads();
   const WaitCtx ctx{&abort_flag, status};
   const int group = threadIdx.x / TPR;
-  if (group == GROUPS) {
-    const LnSource src[2] = {sg, sx};
+  constexpr bool SELF = ln_self_fetch<T, VEC, PER, TPR>();
+  const LnSource src[2] = {sg, sx};
+  if (!SELF && group == GROUPS) {
     ln_fetch_all<T, 2>(src, ring, rows, cols * static_cast<int>(sizeof(T)), ring_mem + ring.weight_bytes, full, empty, ctx);
   } else {
     const int lane = threadIdx.x % TPR;
@@ -440,6 +470,12 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
     }
     const float inv_n = 1.f / static_cast<float>(cols);
     const int stage_rows = TPR == 32 ? ring.stage_rows : 1;
+    const int64_t ahead = static_cast<int64_t>(gridDim.x) * ring.stages;      // from a stage's row to its next one
+    if (SELF && threadIdx.x == 0)
+      for (int i = 0; i < ring.stages; ++i) {
+        const int64_t n = blockIdx.x + static_cast<int64_t>(i) * gridDim.x;
+        if (n < rows) ln_fetch_rows<2>(src, ring.row_bytes, static_cast<int>(n), 1, ring_mem + 2 * i * ring.row_bytes, &full[i]);
+      }
     const char* const my_ring = ring_mem + ring.weight_bytes + lane * VEC * static_cast<int>(sizeof(T));
     T* const my_dx = dx + lane * VEC;
     int stage = 0, stage_at = 0, slot = 0;
@@ -497,12 +533,14 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
           }
         }
         float2 s = make_float2(vsum(s1), vsum(s2));
-        if (TPR > 32 && HOLD) {                                 // the stage's only row is in registers
+        if (TPR > 32 && HOLD && !SELF) {                        // the stage's only row is in registers
           __syncwarp();
           if ((lane & 31) == 0) mbar_arrive(&empty[stage]);
         }
         s = row_sum2<TPR>(s, scratch, slot);
         slot ^= 1;
+        if (SELF && threadIdx.x == 0 && top + ahead < rows)     // and, behind the barrier, in every thread's
+          ln_fetch_rows<2>(src, ring.row_bytes, static_cast<int>(top + ahead), 1, ring_mem + stage_at, &full[stage]);
         if (dx != nullptr) {
           const V c1 = vsplat<V>(-s.x * inv_n * rs_now), c2 = vsplat<V>(-s.y * inv_n * rs_now);
           T* out = my_dx + r * lddx;
@@ -636,7 +674,7 @@ static int ln_fwd_rows(const LayerNormArgs& a, int align, const DeviceInfo* dev,
   const int smem = ring.stages * ring.stage_rows * ring.row_bytes;
   B200K_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LN_SMEM));
   const int64_t most = (a.rows + ring.stage_rows - 1) / ring.stage_rows, grid = static_cast<int64_t>(dev->sm_count) * PER_SM;
-  kernel<<<static_cast<unsigned>(most < grid ? most : grid), ln_threads<TPR>(), smem, stream>>>(
+  kernel<<<static_cast<unsigned>(most < grid ? most : grid), ln_threads<T, VEC, PER, TPR>(), smem, stream>>>(
       ln_source(a.x, a.rows, a.cols, a.ldx, sizeof(T)), static_cast<const W*>(a.w), static_cast<const W*>(a.b), static_cast<T*>(a.y), a.mean, a.rstd,
       static_cast<int>(a.rows), static_cast<int>(a.cols), a.ldy, a.eps, ring, dev->status_word);
   count_launch();
@@ -657,7 +695,7 @@ static int ln_bwd_rows(const LayerNormArgs& a, int align, const DeviceInfo* dev,
   if (grid > static_cast<int64_t>(dev->sm_count) * PER_SM) grid = static_cast<int64_t>(dev->sm_count) * PER_SM;
   if (grid > LN_MAX_PARTS) grid = LN_MAX_PARTS;
   *parts = static_cast<int>(grid);
-  kernel<<<static_cast<unsigned>(grid), ln_threads<TPR>(), smem, stream>>>(
+  kernel<<<static_cast<unsigned>(grid), ln_threads<T, VEC, PER, TPR>(), smem, stream>>>(
       ln_source(a.dy, a.rows, a.cols, a.lddy, sizeof(T)), ln_source(a.x, a.rows, a.cols, a.ldx, sizeof(T)), static_cast<const W*>(a.w), a.mean,
       a.rstd, static_cast<T*>(a.dx), part, static_cast<int>(a.rows), static_cast<int>(a.cols), a.lddx, ring, dev->status_word);
   count_launch();
@@ -679,7 +717,7 @@ static bool ln_shape(int64_t cols, int align, F&& f) {
     const int64_t u = cols / V;
     if (u <= 32) f(Int<V>(), Int<1>(), Int<32>());
     else if (u <= 64) f(Int<V>(), Int<2>(), Int<32>());
-    else if (u <= 512 / V) f(Int<V>(), Int<4>(), Int<32>());
+    else if (u <= 512 / V) f(Int<V>(), Int<16 / V>(), Int<32>());       // fp32 alone: 64 accesses hold 512 16-bit elements
     else if (u <= 1024 / V) f(Int<V>(), Int<8 / V>(), Int<128>());
     else if (u <= 2 * 1024 / V) f(Int<V>(), Int<16 / V>(), Int<128>());
     else if (u <= 4 * 1024 / V) f(Int<V>(), Int<16 / V>(), Int<256>());
