@@ -125,10 +125,10 @@ constexpr int LN_GROUPS = 8;          // rows at a time of a CTA whose warps tak
 constexpr int LN_MAX_STAGES = 8;
 template <int TPR>
 __host__ __device__ constexpr int ln_groups() { return TPR == 32 ? LN_GROUPS : 1; }
-// With rows on 16-byte boundaries and a CTA per row, fetching a row is two instructions, and the first thread does it behind the barrier of the
-// row sum: a fetching warp would cost the others registers (17 warps leave them 96 each, 16 warps 128).
+// With a CTA per row, fetching a row is a few instructions, and the first thread does it behind the barrier of the row sum: a fetching warp would
+// cost the others registers (17 warps leave them 96 each, 16 warps 128).
 template <typename T, int VEC, int PER, int TPR>
-__host__ __device__ constexpr bool ln_self_fetch() { return TPR > 32 && VEC * sizeof(T) == 16 && PER * VEC <= 16; }
+__host__ __device__ constexpr bool ln_self_fetch() { return TPR > 32; }
 template <typename T, int VEC, int PER, int TPR>
 __host__ __device__ constexpr int ln_threads() { return TPR * ln_groups<TPR>() + (ln_self_fetch<T, VEC, PER, TPR>() ? 0 : 32); }
 // CTAs of one SM.  The backward writes a partial sum per CTA, so that it takes fewer.
@@ -176,13 +176,39 @@ __device__ __noinline__ void ln_patch(const char* a, int row_len, const char* fr
   for (const char* q = tail; q < z; q += sizeof(T)) *reinterpret_cast<T*>(dst + (q - a)) = *reinterpret_cast<const T*>(q);
 }
 
-// One thread fetches `count` rows (from r on) of each operand into a stage; rows on 16-byte boundaries.
-template <int NSRC>
-__device__ __forceinline__ void ln_fetch_rows(const LnSource (&src)[NSRC], int row_bytes, int r, int count, char* stage, uint64_t* bar) {
-  mbar_expect_tx(bar, static_cast<uint32_t>(NSRC * count * row_bytes));
-  for (int i = 0; i < count; ++i)
+// One thread fetches `count` rows (one or two, from r on) of each operand into a stage.  ALIGNED: rows are whole 16-byte blocks.
+template <typename T, bool ALIGNED, int NSRC>
+__device__ __forceinline__ void ln_fetch_rows(const LnSource (&src)[NSRC], const LnRing& ring, int row_len, int r, int count, char* stage, uint64_t* bar) {
+  if constexpr (ALIGNED) {
+    mbar_expect_tx(bar, static_cast<uint32_t>(NSRC * count * row_len));
+    for (int i = 0; i < count; ++i)
 #pragma unroll
-    for (int k = 0; k < NSRC; ++k) bulk_load(stage + (i * NSRC + k) * row_bytes, src[k].base + (r + i) * src[k].pitch, row_bytes, bar);
+      for (int k = 0; k < NSRC; ++k) bulk_load(stage + (i * NSRC + k) * row_len, src[k].base + (r + i) * src[k].pitch, row_len, bar);
+  } else {
+    uint32_t bytes[2][NSRC], total = 0;
+    const char* from[2][NSRC];
+    char* dst[2][NSRC];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < NSRC; ++k) {
+        bytes[i][k] = 0;
+        if (i < count) {
+          const char* a = src[k].base + (r + i) * src[k].pitch;
+          bytes[i][k] = ln_span(src[k], a, row_len, &from[i][k]);
+          char* row = stage + (i * NSRC + k) * ring.row_bytes + (reinterpret_cast<uintptr_t>(a) & 15u);
+          dst[i][k] = row + (from[i][k] - a);
+          if (from[i][k] > a || from[i][k] + bytes[i][k] < a + row_len) ln_patch<T>(a, row_len, from[i][k], bytes[i][k], row);
+          total += bytes[i][k];
+        }
+      }
+    mbar_expect_tx(bar, total);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < NSRC; ++k)
+        if (i < count && bytes[i][k] > 0) bulk_load(dst[i][k], from[i][k], bytes[i][k], bar);
+  }
 }
 
 // The fetching warp: blocks of stage_rows rows, a lane per row.
@@ -301,10 +327,11 @@ ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ 
   __syncthreads();
   const WaitCtx ctx{&abort_flag, status};
   const int group = threadIdx.x / TPR;
-  constexpr bool SELF = ln_self_fetch<T, VEC, PER, TPR>();
+  constexpr bool SELF = ln_self_fetch<T, VEC, PER, TPR>(), ALIGNED = VEC * sizeof(T) == 16;
+  const int row_len = cols * static_cast<int>(sizeof(T));
   const LnSource src[1] = {sx};
   if (!SELF && group == GROUPS) {
-    ln_fetch_all<T, 1>(src, ring, rows, cols * static_cast<int>(sizeof(T)), ring_mem, full, empty, ctx);
+    ln_fetch_all<T, 1>(src, ring, rows, row_len, ring_mem, full, empty, ctx);
   } else {
     const int lane = threadIdx.x % TPR;
     V fw[HOLD ? PER : 1][N], fb[HOLD ? PER : 1][N];
@@ -321,7 +348,7 @@ ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ 
     if (SELF && threadIdx.x == 0)
       for (int i = 0; i < ring.stages; ++i) {
         const int64_t r = (blockIdx.x + static_cast<int64_t>(i) * gridDim.x) * BATCH;
-        if (r < rows) ln_fetch_rows<1>(src, ring.row_bytes, static_cast<int>(r), min(BATCH, rows - static_cast<int>(r)), ring_mem + i * BATCH * ring.row_bytes, &full[i]);
+        if (r < rows) ln_fetch_rows<T, ALIGNED, 1>(src, ring, row_len, static_cast<int>(r), min(BATCH, rows - static_cast<int>(r)), ring_mem + i * BATCH * ring.row_bytes, &full[i]);
       }
     const char* const my_ring = ring_mem + lane * VEC * static_cast<int>(sizeof(T));
     T* const my_y = y + lane * VEC;
@@ -353,13 +380,9 @@ ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ 
         }
         s = batch_sum<TPR, BATCH>(s, scratch, 0);
         if (TPR > 32 && lane == 0) {                                 // every thread holds its part of the stage's rows in registers
-          if constexpr (SELF) {
-            if (top + ahead < rows) {
-              const int n = static_cast<int>(top + ahead);
-              ln_fetch_rows<1>(src, ring.row_bytes, n, min(BATCH, rows - n), ring_mem + stage_at, &full[stage]);
-            }
-          } else {
-            mbar_arrive(&empty[stage]);
+          if (top + ahead < rows) {
+            const int n = static_cast<int>(top + ahead);
+            ln_fetch_rows<T, ALIGNED, 1>(src, ring, row_len, n, min(BATCH, rows - n), ring_mem + stage_at, &full[stage]);
           }
         }
         const float mu[2] = {s.x * inv_n, s.y * inv_n};
@@ -434,17 +457,18 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
   __shared__ uint32_t abort_flag;
   if (threadIdx.x < LN_MAX_STAGES) {
     mbar_init(&full[threadIdx.x], 1);
-    mbar_init(&empty[threadIdx.x], TPR == 32 ? GROUPS : TPR / 32);
+    mbar_init(&empty[threadIdx.x], GROUPS);
   }
   if (threadIdx.x == 0) abort_flag = 0;
   fence_mbar_init();
   __syncthreads();
   const WaitCtx ctx{&abort_flag, status};
   const int group = threadIdx.x / TPR;
-  constexpr bool SELF = ln_self_fetch<T, VEC, PER, TPR>();
+  constexpr bool SELF = ln_self_fetch<T, VEC, PER, TPR>(), ALIGNED = VEC * sizeof(T) == 16;
+  const int row_len = cols * static_cast<int>(sizeof(T));
   const LnSource src[2] = {sg, sx};
   if (!SELF && group == GROUPS) {
-    ln_fetch_all<T, 2>(src, ring, rows, cols * static_cast<int>(sizeof(T)), ring_mem + ring.weight_bytes, full, empty, ctx);
+    ln_fetch_all<T, 2>(src, ring, rows, row_len, ring_mem + ring.weight_bytes, full, empty, ctx);
   } else {
     const int lane = threadIdx.x % TPR;
     W* const held_w = reinterpret_cast<W*>(ring_mem);
@@ -470,11 +494,15 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
     }
     const float inv_n = 1.f / static_cast<float>(cols);
     const int stage_rows = TPR == 32 ? ring.stage_rows : 1;
-    const int64_t ahead = static_cast<int64_t>(gridDim.x) * ring.stages;      // from a stage's row to its next one
+    // Rows that are under way beside the one worked on.  When that one is not held in registers, its stage is only free when the next row's barrier is
+    // passed, so that one stage less is.
+    const int under_way = HOLD || ring.stages == 1 ? ring.stages : ring.stages - 1;
+    const int64_t ahead = static_cast<int64_t>(gridDim.x) * under_way;
+    char* const stages = ring_mem + ring.weight_bytes;
     if (SELF && threadIdx.x == 0)
-      for (int i = 0; i < ring.stages; ++i) {
+      for (int i = 0; i < under_way; ++i) {
         const int64_t n = blockIdx.x + static_cast<int64_t>(i) * gridDim.x;
-        if (n < rows) ln_fetch_rows<2>(src, ring.row_bytes, static_cast<int>(n), 1, ring_mem + 2 * i * ring.row_bytes, &full[i]);
+        if (n < rows) ln_fetch_rows<T, ALIGNED, 2>(src, ring, row_len, static_cast<int>(n), 1, stages + 2 * i * ring.row_bytes, &full[i]);
       }
     const char* const my_ring = ring_mem + ring.weight_bytes + lane * VEC * static_cast<int>(sizeof(T));
     T* const my_dx = dx + lane * VEC;
@@ -533,14 +561,16 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
           }
         }
         float2 s = make_float2(vsum(s1), vsum(s2));
-        if (TPR > 32 && HOLD && !SELF) {                        // the stage's only row is in registers
-          __syncwarp();
-          if ((lane & 31) == 0) mbar_arrive(&empty[stage]);
-        }
         s = row_sum2<TPR>(s, scratch, slot);
         slot ^= 1;
-        if (SELF && threadIdx.x == 0 && top + ahead < rows)     // and, behind the barrier, in every thread's
-          ln_fetch_rows<2>(src, ring.row_bytes, static_cast<int>(top + ahead), 1, ring_mem + stage_at, &full[stage]);
+        if (SELF && threadIdx.x == 0 && top + ahead < rows) {   // behind the barrier every thread is past the row before, or holds this one
+          if (HOLD) {
+            ln_fetch_rows<T, ALIGNED, 2>(src, ring, row_len, static_cast<int>(top + ahead), 1, stages + stage_at, &full[stage]);
+          } else if (ring.stages > 1) {
+            const int before = stage == 0 ? ring.stages - 1 : stage - 1;
+            ln_fetch_rows<T, ALIGNED, 2>(src, ring, row_len, static_cast<int>(top + ahead), 1, stages + 2 * before * ring.row_bytes, &full[before]);
+          }
+        }
         if (dx != nullptr) {
           const V c1 = vsplat<V>(-s.x * inv_n * rs_now), c2 = vsplat<V>(-s.y * inv_n * rs_now);
           T* out = my_dx + r * lddx;
@@ -560,9 +590,12 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
           }
         }
       }
-      if (TPR == 32 || !HOLD) {
+      if (TPR == 32) {
         __syncwarp();
-        if ((lane & 31) == 0) mbar_arrive(&empty[stage]);
+        if (lane == 0) mbar_arrive(&empty[stage]);
+      } else if (!HOLD && ring.stages == 1) {
+        named_bar_sync(2, TPR);                                 // the only stage is free
+        if (threadIdx.x == 0 && top + ahead < rows) ln_fetch_rows<T, ALIGNED, 2>(src, ring, row_len, static_cast<int>(top + ahead), 1, stages, &full[0]);
       }
       stage_at += 2 * stage_rows * ring.row_bytes;
       if (++stage == ring.stages) { stage = stage_at = 0; phase ^= 1u; }
@@ -732,7 +765,7 @@ static bool ln_shape(int64_t cols, int align, F&& f) {
     else if (cols <= 1024) f(Int<2>(), Int<4>(), Int<128>());
     else if (cols <= 2048) f(Int<2>(), Int<8>(), Int<128>());
     else if (cols <= 4096) f(Int<2>(), Int<8>(), Int<256>());
-    else if (cols <= 8192) f(Int<2>(), Int<BWD ? 16 : 8>(), Int<BWD ? 256 : 512>());
+    else if (cols <= 8192) f(Int<2>(), Int<8>(), Int<512>());
     else if (cols <= 16384) f(Int<2>(), Int<16>(), Int<512>());
     else return false;
     return true;
@@ -742,7 +775,7 @@ static bool ln_shape(int64_t cols, int align, F&& f) {
   else if (cols <= 1024) f(Int<1>(), Int<8>(), Int<128>());
   else if (cols <= 2048) f(Int<1>(), Int<16>(), Int<128>());
   else if (cols <= 4096) f(Int<1>(), Int<16>(), Int<256>());
-  else if (cols <= 8192) f(Int<1>(), Int<BWD ? 32 : 16>(), Int<BWD ? 256 : 512>());
+  else if (cols <= 8192) f(Int<1>(), Int<16>(), Int<512>());
   else if (cols <= 16384) f(Int<1>(), Int<32>(), Int<512>());
   else return false;
   return true;
