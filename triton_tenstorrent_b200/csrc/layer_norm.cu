@@ -112,29 +112,29 @@ __global__ void __launch_bounds__(256) ln_dw_loop_kernel(const T* __restrict__ d
 }
 
 // ---------------------------------------------------------------------------------------------
-// Rows of up to TPR * PER * VEC elements.  A CTA has one warp that fetches and TPR (or, with a warp per row, LN_GROUPS * 32) threads that work:
-// the fetching warp keeps a ring of rows in shared memory filled, whatever the others wait for.
+// Rows of up to TPR * PER * VEC elements, TPR threads to a row: a whole CTA, or (TPR = 32) a warp, LN_GROUPS of them in a CTA.  The rows to come are on
+// their way into a ring in shared memory meanwhile.
 //
 // A row is worked on in steps that wait for one another (load, row sum, second sum, store), and registers for enough rows at a time do not exist
-// next to the backward's 2 N running sums; the ring keeps 60 to 190 KB per SM on their way instead.  (Fetching by one of the working warps,
-// between two row sums, was measured at 2800 GB/s for 16384 x 4096 bf16: the address arithmetic then sits on the path that every row waits for.)
+// next to the backward's 2 N running sums; the ring keeps 60 to 190 KB per SM on their way instead, whatever the arithmetic waits for.
 // Rows come as untiled bulk copies of the 16-byte blocks that they touch, so that any length and alignment arrives at full rate; only the
 // reads from shared memory and the stores go by VEC, the widest access that the operands' alignment allows.
+// A CTA-wide row is fetched by the CTA's first thread, behind a barrier that the row sum needs anyway; a warp of its own for it, as the CTAs of
+// narrow rows have, would cost the others registers (17 warps leave them 96 each, 16 warps 128: backward, 16384 x 4096 bf16, 82 against 64 us).
+//
+// Measured, inputs larger than L2, of 6460 GB/s: 16384 x 4096 bf16 forward 46 us (5.8 TB/s), backward 64 us (6.3 TB/s); 8192 x 8192 bf16 with fp32
+// weights 49 and 75 us.  Rows on odd boundaries (16384 x 4095 bf16: 76 and 85 us) are bound by their 2-byte stores and the LSU.
 // ---------------------------------------------------------------------------------------------
 constexpr int LN_GROUPS = 8;          // rows at a time of a CTA whose warps take a row each
 constexpr int LN_MAX_STAGES = 8;
 template <int TPR>
 __host__ __device__ constexpr int ln_groups() { return TPR == 32 ? LN_GROUPS : 1; }
-// With a CTA per row, fetching a row is a few instructions, and the first thread does it behind the barrier of the row sum: a fetching warp would
-// cost the others registers (17 warps leave them 96 each, 16 warps 128).
-template <typename T, int VEC, int PER, int TPR>
-__host__ __device__ constexpr bool ln_self_fetch() { return TPR > 32; }
-template <typename T, int VEC, int PER, int TPR>
-__host__ __device__ constexpr int ln_threads() { return TPR * ln_groups<TPR>() + (ln_self_fetch<T, VEC, PER, TPR>() ? 0 : 32); }
+template <int TPR>
+__host__ __device__ constexpr int ln_threads() { return TPR * ln_groups<TPR>() + (TPR == 32 ? 32 : 0); }      // with the fetching warp
 // CTAs of one SM.  The backward writes a partial sum per CTA, so that it takes fewer.
-template <int TPR, bool BWD>
+template <int TPR, int E, bool BWD>
 __host__ __device__ constexpr int ln_per_sm() {
-  return TPR == 32 ? (BWD ? 2 : 3) : TPR == 128 ? (BWD ? 4 : 5) : TPR == 256 ? (BWD ? 2 : 3) : 1;
+  return TPR == 32 ? (BWD && E > 8 ? 2 : 3) : TPR == 128 ? (BWD ? 4 : E > 8 ? 5 : 6) : TPR == 256 ? (BWD ? 2 : 3) : 1;
 }
 
 // Whether access k of a thread can lie behind the row's end.  A CTA-wide row fills more than half of its shape (ln_shape), so the first half of the
@@ -305,9 +305,10 @@ __device__ __forceinline__ void ln_weight(const W* w, int c, int cols, float dfl
   }
 }
 
-// BATCH rows are worked on at a time (1 or 2): with one CTA on an SM a second row fills the waits of the first.
+// BATCH rows are worked on at a time (1 or 2): with one CTA on an SM, or a row so short that a warp mostly waits, a second one fills the waits of the
+// first.
 template <typename T, typename W, int VEC, int PER, int TPR, int BATCH>
-__global__ void __launch_bounds__(ln_threads<T, VEC, PER, TPR>(), ln_per_sm<TPR, false>())
+__global__ void __launch_bounds__(ln_threads<TPR>(), ln_per_sm<TPR, PER * VEC, false>())
 ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ b, T* __restrict__ y, float* __restrict__ mean,
               float* __restrict__ rstd, int rows, int cols, int64_t ldy, float eps, const LnRing ring, uint32_t* status) {
   constexpr int GROUPS = ln_groups<TPR>();
@@ -327,7 +328,7 @@ ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ 
   __syncthreads();
   const WaitCtx ctx{&abort_flag, status};
   const int group = threadIdx.x / TPR;
-  constexpr bool SELF = ln_self_fetch<T, VEC, PER, TPR>(), ALIGNED = VEC * sizeof(T) == 16;
+  constexpr bool SELF = TPR > 32, ALIGNED = VEC * sizeof(T) == 16;
   const int row_len = cols * static_cast<int>(sizeof(T));
   const LnSource src[1] = {sx};
   if (!SELF && group == GROUPS) {
@@ -442,7 +443,7 @@ ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ 
 
 // Backward.  The columns' sums of dy h and dy stay in registers until the end: one partial sum per CTA (part[2][gridDim.x][cols], first dw's).
 template <typename T, typename W, int VEC, int PER, int TPR>
-__global__ void __launch_bounds__(ln_threads<T, VEC, PER, TPR>(), ln_per_sm<TPR, true>())
+__global__ void __launch_bounds__(ln_threads<TPR>(), ln_per_sm<TPR, PER * VEC, true>())
 ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, const float* __restrict__ mean, const float* __restrict__ rstd,
               T* __restrict__ dx, float* __restrict__ part, int rows, int cols, int64_t lddx, const LnRing ring, uint32_t* status) {
   constexpr int GROUPS = ln_groups<TPR>();
@@ -464,7 +465,7 @@ ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, con
   __syncthreads();
   const WaitCtx ctx{&abort_flag, status};
   const int group = threadIdx.x / TPR;
-  constexpr bool SELF = ln_self_fetch<T, VEC, PER, TPR>(), ALIGNED = VEC * sizeof(T) == 16;
+  constexpr bool SELF = TPR > 32, ALIGNED = VEC * sizeof(T) == 16;
   const int row_len = cols * static_cast<int>(sizeof(T));
   const LnSource src[2] = {sg, sx};
   if (!SELF && group == GROUPS) {
@@ -691,7 +692,7 @@ constexpr int LN_SMEM = 212 * 1024;     // shared memory that the CTAs of an SM 
 static LnRing ln_ring(int64_t cols, int size, int align, int operands, int groups, int per_sm, int batch, int weight_size) {
   LnRing r;
   r.row_bytes = static_cast<int>((cols * size + 15) / 16 * 16) + (align == 16 ? 0 : 16);
-  r.stage_rows = groups == 1 ? batch : r.row_bytes * operands <= 256 ? 4 * groups : r.row_bytes * operands <= 1024 ? 2 * groups : groups;
+  r.stage_rows = groups == 1 ? batch : r.row_bytes * operands <= 256 ? 4 * groups : r.row_bytes * operands <= 1024 || batch == 2 ? 2 * groups : groups;
   r.weight_bytes = static_cast<int>((cols * weight_size + 15) / 16 * 16);
   const int64_t stages = (static_cast<int64_t>(LN_SMEM) / per_sm - r.weight_bytes) / (static_cast<int64_t>(r.stage_rows) * r.row_bytes * operands);
   r.stages = static_cast<int>(stages > LN_MAX_STAGES ? LN_MAX_STAGES : stages);
@@ -700,14 +701,14 @@ static LnRing ln_ring(int64_t cols, int size, int align, int operands, int group
 
 template <typename T, typename W, int VEC, int PER, int TPR>
 static int ln_fwd_rows(const LayerNormArgs& a, int align, const DeviceInfo* dev, cudaStream_t stream, bool* done) {
-  constexpr int GROUPS = ln_groups<TPR>(), PER_SM = ln_per_sm<TPR, false>(), BATCH = TPR == 512 && PER * VEC <= 16 ? 2 : 1;
+  constexpr int GROUPS = ln_groups<TPR>(), PER_SM = ln_per_sm<TPR, PER * VEC, false>(), BATCH = (TPR == 512 && PER * VEC <= 16) || (TPR == 32 && PER * VEC <= 8) ? 2 : 1;
   const LnRing ring = ln_ring(a.cols, sizeof(T), align, 1, GROUPS, PER_SM, BATCH, 0);
   if (ring.stages < 1 || (TPR > 32 && a.cols <= TPR * VEC * (PER / 2))) return B200K_OK;   // the second is what ln_inside relies on
   auto kernel = ln_fwd_kernel<T, W, VEC, PER, TPR, BATCH>;
   const int smem = ring.stages * ring.stage_rows * ring.row_bytes;
   B200K_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LN_SMEM));
   const int64_t most = (a.rows + ring.stage_rows - 1) / ring.stage_rows, grid = static_cast<int64_t>(dev->sm_count) * PER_SM;
-  kernel<<<static_cast<unsigned>(most < grid ? most : grid), ln_threads<T, VEC, PER, TPR>(), smem, stream>>>(
+  kernel<<<static_cast<unsigned>(most < grid ? most : grid), ln_threads<TPR>(), smem, stream>>>(
       ln_source(a.x, a.rows, a.cols, a.ldx, sizeof(T)), static_cast<const W*>(a.w), static_cast<const W*>(a.b), static_cast<T*>(a.y), a.mean, a.rstd,
       static_cast<int>(a.rows), static_cast<int>(a.cols), a.ldy, a.eps, ring, dev->status_word);
   count_launch();
@@ -718,7 +719,7 @@ static int ln_fwd_rows(const LayerNormArgs& a, int align, const DeviceInfo* dev,
 
 template <typename T, typename W, int VEC, int PER, int TPR>
 static int ln_bwd_rows(const LayerNormArgs& a, int align, const DeviceInfo* dev, float* part, int* parts, cudaStream_t stream, bool* done) {
-  constexpr int GROUPS = ln_groups<TPR>(), PER_SM = ln_per_sm<TPR, true>();
+  constexpr int GROUPS = ln_groups<TPR>(), PER_SM = ln_per_sm<TPR, PER * VEC, true>();
   const LnRing ring = ln_ring(a.cols, sizeof(T), align, 2, GROUPS, PER_SM, 1, PER * VEC > 16 ? sizeof(W) : 0);
   if (ring.stages < 1 || (TPR > 32 && a.cols <= TPR * VEC * (PER / 2))) return B200K_OK;   // the second is what ln_inside relies on
   auto kernel = ln_bwd_kernel<T, W, VEC, PER, TPR>;
@@ -728,7 +729,7 @@ static int ln_bwd_rows(const LayerNormArgs& a, int align, const DeviceInfo* dev,
   if (grid > static_cast<int64_t>(dev->sm_count) * PER_SM) grid = static_cast<int64_t>(dev->sm_count) * PER_SM;
   if (grid > LN_MAX_PARTS) grid = LN_MAX_PARTS;
   *parts = static_cast<int>(grid);
-  kernel<<<static_cast<unsigned>(grid), ln_threads<T, VEC, PER, TPR>(), smem, stream>>>(
+  kernel<<<static_cast<unsigned>(grid), ln_threads<TPR>(), smem, stream>>>(
       ln_source(a.dy, a.rows, a.cols, a.lddy, sizeof(T)), ln_source(a.x, a.rows, a.cols, a.ldx, sizeof(T)), static_cast<const W*>(a.w), a.mean,
       a.rstd, static_cast<T*>(a.dx), part, static_cast<int>(a.rows), static_cast<int>(a.cols), a.lddx, ring, dev->status_word);
   count_launch();
@@ -738,12 +739,11 @@ static int ln_bwd_rows(const LayerNormArgs& a, int align, const DeviceInfo* dev,
 }
 
 // Calls f with the kernel shape for rows of `cols` elements of `size` bytes whose operands share `align`: (VEC, PER, TPR) as integral constants.
-// 16 elements a thread or less; 32 beyond 8192, where no more threads are to be had, and for the backward's rows beyond 4096 that are read element
-// by element or by pairs (8192 x 7999 bf16: 144 -> 122 us, x 7998: 107 -> 102; with 16-byte accesses 16 are faster, x 8192: 103 against 118); false beyond 16384 elements.  A warp takes a row of up to 512; a CTA-wide shape is the smallest one
-// that holds the row, so that more than half of it is filled.
+// 16 elements a thread or less, 32 beyond 8192, where no more threads are to be had; false beyond 16384 elements.  A warp takes a row of up to 512; a
+// CTA-wide shape is the smallest one that holds the row, so that more than half of it is filled.
 template <int N>
 using Int = std::integral_constant<int, N>;
-template <int SIZE, bool BWD, typename F>
+template <int SIZE, typename F>
 static bool ln_shape(int64_t cols, int align, F&& f) {
   constexpr int V = 16 / SIZE;
   if (align == 16) {
@@ -795,7 +795,7 @@ static int ln_fwd(const LayerNormArgs& a, const DeviceInfo* dev, cudaStream_t st
   const int align = ln_common_alignment<T, W>(ln_alignment({reinterpret_cast<uintptr_t>(a.x), reinterpret_cast<uintptr_t>(a.y), a.cols * S, a.ldx * S, a.ldy * S}), a.w, a.b);
   int rc = B200K_OK;
   bool done = false;
-  if (a.rows < (int64_t(1) << 30)) ln_shape<S, false>(a.cols, align, [&](auto vec, auto per, auto tpr) { rc = ln_fwd_rows<T, W, vec(), per(), tpr()>(a, align, dev, stream, &done); });
+  if (a.rows < (int64_t(1) << 30)) ln_shape<S>(a.cols, align, [&](auto vec, auto per, auto tpr) { rc = ln_fwd_rows<T, W, vec(), per(), tpr()>(a, align, dev, stream, &done); });
   if (rc != B200K_OK || done) return rc;
   const unsigned grid = static_cast<unsigned>(a.rows < (1 << 30) ? a.rows : (1 << 30));
   ln_fwd_loop_kernel<T, W><<<grid, 512, 0, stream>>>(static_cast<const T*>(a.x), static_cast<const W*>(a.w), static_cast<const W*>(a.b),
@@ -812,7 +812,7 @@ static int ln_bwd_main(const LayerNormArgs& a, const DeviceInfo* dev, float* par
                                                             a.cols * S, a.ldx * S, a.lddy * S, a.dx == nullptr ? 0 : a.lddx * S}), a.w, nullptr);
   int rc = B200K_OK;
   bool done = false;
-  if (a.rows < (int64_t(1) << 30)) ln_shape<S, true>(a.cols, align, [&](auto vec, auto per, auto tpr) { rc = ln_bwd_rows<T, W, vec(), per(), tpr()>(a, align, dev, part, parts, stream, &done); });
+  if (a.rows < (int64_t(1) << 30)) ln_shape<S>(a.cols, align, [&](auto vec, auto per, auto tpr) { rc = ln_bwd_rows<T, W, vec(), per(), tpr()>(a, align, dev, part, parts, stream, &done); });
   if (rc != B200K_OK || done) return rc;
   const T* dy = static_cast<const T*>(a.dy);
   const T* x = static_cast<const T*>(a.x);
