@@ -253,6 +253,35 @@ def test_skipped_gradients_mixed_types_and_autograd():
 
 
 @pytest.mark.gpu
+def test_parameters_that_move_between_steps():
+    w = torch.nn.Parameter(torch.randn(8, 8, device="cuda"))
+    v = torch.nn.Parameter(torch.randn(5, device="cuda"))
+    opt, plain = tt.AdamW([w, v]), [w.detach().clone(), v.detach().clone()]
+    twin = tt.AdamW(plain)
+    g = [torch.randn(8, 8, device="cuda"), torch.randn(5, device="cuda")]
+    opt.step(g)
+    twin.step(g)
+    w.data = w.data.clone()                          # another place, the same shape: followed
+    opt.step(g)
+    twin.step(g)
+    assert torch.equal(w, plain[0]) and torch.equal(v, plain[1])
+    kept = w.data
+    for moved in (torch.zeros(4, 8, device="cuda"), torch.zeros(8, 8), torch.zeros(8, 8, device="cuda").t()[:, ::2], kept.t()):
+        w.data = moved
+        with pytest.raises(ValueError, match="no longer"):
+            opt.step(g)
+    w.data = kept
+    opt.step(g)
+    twin.step(g)
+    assert torch.equal(w, plain[0]) and opt.step_count() == 3
+    sparse = torch.zeros(5, device="cuda").to_sparse()
+    with pytest.raises((ValueError, RuntimeError)):
+        opt.step([g[0], sparse])
+    opt.step([None, g[1]])
+    assert opt.step_count() == 4
+
+
+@pytest.mark.gpu
 def test_a_backward_pass_that_needs_the_old_values_fails():
     w = torch.randn(32, device="cuda", requires_grad=True)
     opt = tt.AdamW([w])

@@ -3,6 +3,7 @@ include/b200k.h)."""
 from __future__ import annotations
 
 import math
+import operator
 import struct
 
 import numpy as np
@@ -15,6 +16,11 @@ __all__ = ["AdamW"]
 
 _BLOCK = 256                       # elements that share a scale of the 8-bit moments
 _P, _G, _MASTER, _M, _V, _MS, _VS, _N, _INDEX = range(9)     # columns of the table: fields of b200k_adamw_tensor
+
+
+# per-tensor queries of step(), called through map
+_size, _data_ptr, _is_contiguous, _get_device, _get_dtype = (torch.Tensor.size, torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.get_device,
+                                                             operator.attrgetter("dtype"))
 
 
 class AdamW:
@@ -93,6 +99,7 @@ class AdamW:
         self._table = table
         self._shapes = [p.shape for p in self.params]
         kinds = {p.dtype for p in self.params}
+        self._at = None
         self._dtype = kinds.pop() if len(kinds) == 1 and all(p.numel() for p in self.params) else None     # the one type, if there is one
 
     def _check_hyper(self):
@@ -152,19 +159,24 @@ class AdamW:
             if lr.device != self.device:
                 raise ValueError(f"AdamW: lr must be on {self.device}")
             lr, lr_ptr = 0.0, lr.data_ptr()
-        # the usual case first, in few steps per tensor: every gradient there, one type each, nothing to copy
-        at, shapes, table, first = self.device.index, self._shapes, self._table, grads[0]
-        dtype, gdtype = self._dtype, None if first is None else first.dtype
+        # The usual case first, with few steps per tensor: every gradient there, one type each, nothing to copy.  The parameters' shapes and places
+        # are looked at again when one of them has moved.
+        table, dtype, gdtype = self._table, self._dtype, getattr(grads[0], "dtype", None)
         try:
-            usual = (dtype is not None and (gdtype is dtype or gdtype is torch.float32)
-                     and all([g is not None and g.dtype is gdtype and g.shape == s and g.is_contiguous() and g.get_device() == at
-                              for g, s in zip(grads, shapes)])
-                     and all([p.dtype is dtype and p.shape == s and p.is_contiguous() and p.get_device() == at for p, s in zip(params, shapes)]))
-        except RuntimeError:        # a sparse gradient has no contiguity
+            usual = (dtype is not None and (gdtype is dtype or gdtype is torch.float32) and list(map(_size, grads)) == self._shapes
+                     and all(map(_is_contiguous, grads)) and all(map(_is_contiguous, params))
+                     and set(map(_get_device, grads)) == {self.device.index} and set(map(_get_dtype, grads)) == {gdtype})
+            if usual:
+                at = list(map(_data_ptr, params))
+                if at != self._at:
+                    usual = list(map(_size, params)) == self._shapes and set(map(_get_device, params)) == {self.device.index} and (
+                        set(map(_get_dtype, params)) == {dtype})
+                    self._at = at if usual else None
+                table[:, _P] = at
+                table[:, _G] = list(map(_data_ptr, grads))
+        except (TypeError, RuntimeError):        # a gradient that is None, or has no contiguity
             usual = False
         if usual:
-            table[:, _P] = [p.data_ptr() for p in params]
-            table[:, _G] = [g.data_ptr() for g in grads]
             launches, touched = [(dtype, gdtype, table)], params
         else:
             launches, touched, grads = self._sort(grads)
