@@ -282,6 +282,19 @@ def test_parameters_that_move_between_steps():
 
 
 @pytest.mark.gpu
+def test_a_parameter_that_shrinks_in_place_is_refused():
+    w, v = torch.nn.Parameter(torch.randn(8, 8, device="cuda")), torch.nn.Parameter(torch.randn(5, device="cuda"))
+    opt, g = tt.AdamW([w, v]), [torch.randn(8, 8, device="cuda"), torch.randn(5, device="cuda")]
+    opt.step(g)
+    whole = w.data
+    before = whole.clone()
+    w.data = whole[:4]                               # the same address
+    with pytest.raises(ValueError, match="no longer"):
+        opt.step(g)
+    assert torch.equal(whole, before) and opt.step_count() == 1
+
+
+@pytest.mark.gpu
 def test_a_backward_pass_that_needs_the_old_values_fails():
     w = torch.randn(32, device="cuda", requires_grad=True)
     opt = tt.AdamW([w])

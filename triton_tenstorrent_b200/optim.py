@@ -99,7 +99,6 @@ class AdamW:
         self._table = table
         self._shapes = [p.shape for p in self.params]
         kinds = {p.dtype for p in self.params}
-        self._at = None
         self._dtype = kinds.pop() if len(kinds) == 1 and all(p.numel() for p in self.params) else None     # the one type, if there is one
 
     def _check_hyper(self):
@@ -159,20 +158,16 @@ class AdamW:
             if lr.device != self.device:
                 raise ValueError(f"AdamW: lr must be on {self.device}")
             lr, lr_ptr = 0.0, lr.data_ptr()
-        # The usual case first, with few steps per tensor: every gradient there, one type each, nothing to copy.  The parameters' shapes and places
-        # are looked at again when one of them has moved.
+        # The usual case first, with few steps per tensor: every gradient there, one type each, nothing to copy.
         table, dtype, gdtype = self._table, self._dtype, getattr(grads[0], "dtype", None)
         try:
             usual = (dtype is not None and (gdtype is dtype or gdtype is torch.float32) and list(map(_size, grads)) == self._shapes
                      and all(map(_is_contiguous, grads)) and all(map(_is_contiguous, params))
-                     and set(map(_get_device, grads)) == {self.device.index} and set(map(_get_dtype, grads)) == {gdtype})
+                     and set(map(_get_device, grads)) == {self.device.index} and set(map(_get_dtype, grads)) == {gdtype}
+                     and list(map(_size, params)) == self._shapes and set(map(_get_device, params)) == {self.device.index}
+                     and set(map(_get_dtype, params)) == {dtype})
             if usual:
-                at = list(map(_data_ptr, params))
-                if at != self._at:
-                    usual = list(map(_size, params)) == self._shapes and set(map(_get_device, params)) == {self.device.index} and (
-                        set(map(_get_dtype, params)) == {dtype})
-                    self._at = at if usual else None
-                table[:, _P] = at
+                table[:, _P] = list(map(_data_ptr, params))
                 table[:, _G] = list(map(_data_ptr, grads))
         except (TypeError, RuntimeError):        # a gradient that is None, or has no contiguity
             usual = False
