@@ -257,7 +257,7 @@ int64_t b200k_layer_norm_bwd_workspace(int64_t rows, int64_t cols);
  * Cross entropy of a linear output layer without keeping its logits (no counterpart in the reference; the loss behind the last
  * product of a training step):  logits = h W^T, lse_i = log sum_v exp(logits[i, v]), losses_i = lse_i - logits[i, target_i].
  *   h           [T, D], w [V, D] of type `dtype` (bf16 or fp16), unit inner stride, row pitches ldh / ldw in elements (multiples of 8, as is D;
- *               base pointers 16-byte aligned); any T >= 0 and V >= 1
+ *               base pointers 16-byte aligned); T >= 0, V >= 1, each size at most 2^30
  *   target      int64 [T]; a token whose target is ignore_index carries no loss: its loss, its lse and its row of dh are 0, and what its row
  *               of h holds does not matter.  Any other target outside [0, V) makes the token's loss NaN, and with it what that enters.
  *   losses, lse fp32 [T] (natural logarithm); loss: one float, the mean over the tokens that carry a loss (0 without any) or the sum,
@@ -298,7 +298,8 @@ int64_t b200k_lce_workspace(int T, int D, int V, int backward);
  * m, v and master are 16-byte aligned; p and g need the alignment of their type only (aligned ones are faster).
  * state: 40 bytes of device memory {double beta1^t, beta2^t; int64 t; double 1/(1-beta1^(t+1)); float 1/sqrt(1-beta2^(t+1)); uint32 0}, read by
  * every call and moved on to t + 1 by a call with advance = 1 (the last of a step), so that a captured step counts on when it is replayed.
- * lr_dev, grad_scale_dev: one device float each that replaces lr / grad_scale, or null.
+ * lr_dev, grad_scale_dev: one device float each that replaces lr / grad_scale, or null.  eps is 0 or at least 2^-126 (the kernel's reciprocal
+ * takes subnormal numbers for zero).
  */
 typedef struct b200k_adamw_tensor {
   void* p;

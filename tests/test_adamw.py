@@ -400,6 +400,14 @@ def test_refusals():
             tt.AdamW(params, **kw)
 
 
+def test_subnormal_eps_is_refused():
+    with pytest.raises(ValueError, match="2\\^-126"):
+        tt.AdamW([torch.zeros(4)], eps=1e-39)
+    rows = np.zeros((1, 9), dtype=np.int64)
+    assert _lib.load().b200k_adamw(rows.ctypes.data, 1, 0, 0, 32, 4096, 1e-3, None, 0.9, 0.999, 1e-39, 0.0, 1.0, None, 0, 1, None) == _lib.ERR_INVALID_ARG
+    assert "2^-126" in _lib.last_error()
+
+
 def test_entry_point_refusals():
     lib = _lib.load()
     rows = np.zeros((2, 9), dtype=np.int64)

@@ -305,6 +305,16 @@ def test_refusals():
             tt.linear_cross_entropy_backward(*args, **kw)
 
 
+def test_sizes_beyond_the_entry_points_integers_are_refused():
+    row, wide, one = torch.zeros(1, 8).bfloat16(), torch.zeros(1, 1).bfloat16(), torch.zeros(1, dtype=torch.int64)
+    many = (1 << 32) + 5                                  # 5 in 32 bits
+    for bad in [dict(h=row.expand(many, 8), targets=one.expand(many)), dict(weight=row.expand(many, 8)), dict(h=wide.expand(1, 1 << 32), weight=wide.expand(1, 1 << 32)),
+                dict(ignore_index=1 << 63)]:
+        with pytest.raises(ValueError, match="at most 2|int64"):
+            tt.linear_cross_entropy(**{"h": row, "weight": row, "targets": one, **bad})
+    assert _lib.load().b200k_lce_fwd(256, 256, 256, 256, 256, 256, 256, 1 << 40, 4, (1 << 30) + 8, 4, (1 << 30) + 8, (1 << 30) + 8, -100, 0, 1, None) == _lib.ERR_INVALID_ARG
+
+
 def test_entry_point_refusals():
     lib = _lib.load()
     assert lib.b200k_lce_workspace(0, 64, 10, 0) == 0

@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const __grid_const
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         // p alone may round otherwise than the plain formula: the quotient takes an approximate reciprocal (1 unit in the last place), of an
-        // update that is itself a small part of p.  The divisor is zero or a normal number: sqrt of the smallest fp32 is 2^-74.5.
+        // update that is itself a small part of p.  The divisor is zero or a normal number: sqrt of the smallest fp32 is 2^-74.5, eps is 0 or normal.
         float inverse;
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(fmaf(root[h][j], inv_sqrt_bc2, q.eps)));
         p[j] = p[j] * decay - m[j] * inverse * step_size;
@@ -497,6 +497,8 @@ int adamw(const AdamwArgs& a, cudaStream_t stream) {
     return set_error(B200K_ERR_INVALID_ARG, "adamw: betas must be in [0, 1) (got %g, %g)", a.beta1, a.beta2);
   if (!(a.eps >= 0.0) || !(a.weight_decay >= 0.0) || (a.lr_dev == nullptr && !(a.lr >= 0.0)))
     return set_error(B200K_ERR_INVALID_ARG, "adamw: lr, eps and weight_decay must be >= 0 (got %g, %g, %g)", a.lr, a.eps, a.weight_decay);
+  // the reciprocal takes a subnormal divisor for zero, and eps is all there is of it where v is 0
+  if (a.eps > 0.0 && a.eps < 0x1p-126) return set_error(B200K_ERR_INVALID_ARG, "adamw: eps must be 0 or at least 2^-126 (got %g)", a.eps);
   const bool master = a.tensors[0].master != nullptr;
   if (master && a.dtype == B200K_DTYPE_F32) return set_error(B200K_ERR_INVALID_ARG, "adamw: fp32 parameters take no master copy");
   const size_t psize = a.dtype == B200K_DTYPE_F32 ? 4 : 2, gsize = a.gdtype == B200K_DTYPE_F32 ? 4 : 2;

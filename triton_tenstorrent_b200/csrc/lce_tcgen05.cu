@@ -903,7 +903,7 @@ int64_t lce_workspace(int T, int D, int V, int backward) { return lce_layout(T, 
 
 static int lce_check(const LceArgs& a, const char* what) {
   if (a.T < 0 || a.D < 8 || a.V < 1 || (a.D & 7)) return set_error(B200K_ERR_INVALID_ARG, "%s: T >= 0, V >= 1 and D a positive multiple of 8 expected (got %d, %d, %d)", what, a.T, a.V, a.D);
-  if (a.V > (1 << 30) || a.T > (1 << 30)) return set_error(B200K_ERR_INVALID_ARG, "%s: at most 2^30 tokens and vocabulary entries", what);
+  if (a.V > (1 << 30) || a.T > (1 << 30) || a.D > (1 << 30)) return set_error(B200K_ERR_INVALID_ARG, "%s: at most 2^30 tokens, vocabulary entries and columns", what);
   if (a.dtype != B200K_DTYPE_BF16 && a.dtype != B200K_DTYPE_F16) return set_error(B200K_ERR_INVALID_ARG, "%s: bf16 or fp16 operands expected (got type %d)", what, a.dtype);
   if (a.reduction < B200K_REDUCE_NONE || a.reduction > B200K_REDUCE_SUM) return set_error(B200K_ERR_INVALID_ARG, "%s: bad reduction %d", what, a.reduction);
   if (static_cast<int64_t>((a.T + 255) / 256) * ((a.V + 255) / 256) > 0x3FFFFFFF || static_cast<int64_t>((a.V + 255) / 256) * ((a.D + 255) / 256) > 0x3FFFFFFF)
@@ -1006,7 +1006,7 @@ int lce_fwd(const LceArgs& a, cudaStream_t stream) {
     g.losses = a.losses;
     g.lse = a.lse;
     g.cta_rows = lce_gather_rows(a.T);
-  lce_gather_kernel<false><<<(a.T + g.cta_rows - 1) / g.cta_rows, 256, 0, stream>>>(g);
+    lce_gather_kernel<false><<<(a.T + g.cta_rows - 1) / g.cta_rows, 256, 0, stream>>>(g);
     count_launch();
     B200K_CHECK_LAUNCH("lce_gather_kernel");
     p.count = g.count;

@@ -688,7 +688,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5) -> torch.Tensor:
 _REDUCTIONS = {"none": _lib.REDUCE_NONE, "mean": _lib.REDUCE_MEAN, "sum": _lib.REDUCE_SUM}
 
 
-def _lce_check(name, h, weight, targets, reduction):
+def _lce_check(name, h, weight, targets, ignore_index, reduction):
     if reduction not in _REDUCTIONS:
         raise ValueError(f"{name}: unknown reduction {reduction!r} (expected 'none', 'mean' or 'sum')")
     if h.dtype not in (torch.bfloat16, torch.float16) or weight.dtype != h.dtype:
@@ -701,6 +701,10 @@ def _lce_check(name, h, weight, targets, reduction):
         raise ValueError(f"{name}: D must be a positive multiple of 8 (16-byte rows); got {weight.shape[1]}")
     if targets.shape != h.shape[:-1]:
         raise ValueError(f"{name}: targets must be {tuple(h.shape[:-1])} like h without its last dimension, got {tuple(targets.shape)}")
+    if max(targets.numel(), *weight.shape) > 1 << 30:
+        raise ValueError(f"{name}: at most 2^30 tokens, vocabulary entries and columns, got {targets.numel()}, {tuple(weight.shape)}")
+    if not -1 << 63 <= ignore_index < 1 << 63:
+        raise ValueError(f"{name}: ignore_index must be an int64, got {ignore_index}")
     if weight.device != h.device or targets.device != h.device:
         raise ValueError(f"{name}: tensors on different devices")
 
@@ -735,7 +739,7 @@ def _lce_forward(h, weight, targets, ignore_index, reduction):
 def linear_cross_entropy_with_lse(h, weight, targets, ignore_index: int = -100):
     """Returns (losses, lse), fp32 in the shape of targets: lse = log sum_v exp(h . weight[v]) and losses = lse - h . weight[target].  Both are 0
     for a token whose target is ignore_index.  Not differentiable; lse is what linear_cross_entropy_backward takes."""
-    _lce_check("linear_cross_entropy", h, weight, targets, "none")
+    _lce_check("linear_cross_entropy", h, weight, targets, ignore_index, "none")
     losses, lse, _ = _lce_forward(h, weight, targets, ignore_index, "none")
     return _like_input(losses, h), _like_input(lse, h)
 
@@ -744,7 +748,7 @@ def linear_cross_entropy_backward(h, weight, targets, lse, d_loss, ignore_index:
                                   need_dw: bool = True):
     """(dh, dw) from the lse of the forward and the fp32 gradient of the losses (reduction "none": in the shape of targets) or of their mean or
     sum (one element).  A gradient that is not needed is None."""
-    _lce_check("linear_cross_entropy_backward", h, weight, targets, reduction)
+    _lce_check("linear_cross_entropy_backward", h, weight, targets, ignore_index, reduction)
     if lse.dtype != torch.float32 or lse.shape != targets.shape or lse.device != h.device:
         raise ValueError(f"linear_cross_entropy_backward: lse must be fp32 {tuple(targets.shape)} on h's device")
     if d_loss.dtype != torch.float32 or d_loss.device != h.device or (d_loss.shape != targets.shape if reduction == "none" else d_loss.numel() != 1):
@@ -787,7 +791,7 @@ def linear_cross_entropy(h, weight, targets, ignore_index: int = -100, reduction
     reduction "mean" (over the tokens whose target is not ignore_index; 0 without any), "sum", or "none" (fp32 in the shape of targets, 0 for
     ignored tokens).  What h holds for ignored tokens does not matter, NaN included; any other target outside [0, V) makes its token's loss
     NaN.  Differentiable in h and weight."""
-    _lce_check("linear_cross_entropy", h, weight, targets, reduction)
+    _lce_check("linear_cross_entropy", h, weight, targets, ignore_index, reduction)
     if torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad):
         return _linear_cross_entropy.apply(h, weight, targets, ignore_index, reduction)
     losses, _, loss = _lce_forward(h, weight, targets, ignore_index, reduction)

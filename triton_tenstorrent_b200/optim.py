@@ -38,7 +38,8 @@ class AdamW:
                     update below half a unit in its last place
 
     The moments live in flat buffers in which parameter i begins at element offsets[i], a multiple of 256 (split() gives views in the
-    parameters' shapes).  One step count serves all parameters and lives on the device, so that a captured step() can be replayed."""
+    parameters' shapes).  One step count serves all parameters and lives on the device, so that a captured step() can be replayed.  Steps of one
+    optimiser follow one another: those on different streams have to be ordered by their caller."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, state_bits: int = 32,
                  master_weights: bool = False, seed: int = 0):
@@ -109,6 +110,8 @@ class AdamW:
             raise ValueError(f"AdamW: lr must be >= 0, got {self.lr}")
         if not 0 <= self.eps < math.inf or not 0 <= self.weight_decay < math.inf:
             raise ValueError(f"AdamW: eps and weight_decay must be >= 0, got {self.eps}, {self.weight_decay}")
+        if 0 < self.eps < 2.0 ** -126:
+            raise ValueError(f"AdamW: eps must be 0 or at least 2^-126 (a normal fp32), got {self.eps}")
 
     def _set_step(self, t: int):
         b1, b2 = self.betas
