@@ -686,15 +686,23 @@ static LnSource ln_source(const void* p, int64_t rows, int64_t cols, int64_t ld,
   const char* base = static_cast<const char*>(p);
   return LnSource{base, ld * size, base + ((rows - 1) * ld + cols) * size};
 }
-// The ring of a CTA: a few KB per stage (a row or a batch of them for a CTA-wide row, some for every warp otherwise) and as many stages as the CTA's
-// share of the shared memory holds.  stages < 1: the rows are too long.
+// The ring of a CTA: a few KB per stage (a row or a batch of them for a CTA-wide row, some for every warp otherwise), and two stages or what makes
+// LN_AHEAD_FWD / LN_AHEAD_BWD bytes per SM, where the CTA's share of the shared memory holds them.  stages < 1: the rows are too long.
+// More reads under way than HBM's latency asks for hold up the writes (us, forward, 16384 x 4096 and 65536 x 4096 bf16: 47 and 169 with 72 KB per SM, 50 and 198
+// with 96 KB, 55 and 205 with 196 KB; 4096 x 16384: 63 with two stages, 78 with six).  The backward reads twice as much as it writes and is slowed by
+// fewer (131072 x 512 bf16: 97 with 60 KB, 84 with 110, 81 with 140, 89 with 200).
 constexpr int LN_SMEM = 212 * 1024;     // shared memory that the CTAs of an SM divide
+constexpr int LN_AHEAD_FWD = 60 * 1024, LN_AHEAD_BWD = 140 * 1024;
 static LnRing ln_ring(int64_t cols, int size, int align, int operands, int groups, int per_sm, int batch, int weight_size) {
   LnRing r;
   r.row_bytes = static_cast<int>((cols * size + 15) / 16 * 16) + (align == 16 ? 0 : 16);
   r.stage_rows = groups == 1 ? batch : r.row_bytes * operands <= 256 ? 4 * groups : r.row_bytes * operands <= 1024 || batch == 2 ? 2 * groups : groups;
   r.weight_bytes = static_cast<int>((cols * weight_size + 15) / 16 * 16);
-  const int64_t stages = (static_cast<int64_t>(LN_SMEM) / per_sm - r.weight_bytes) / (static_cast<int64_t>(r.stage_rows) * r.row_bytes * operands);
+  const int64_t stage_bytes = static_cast<int64_t>(r.stage_rows) * r.row_bytes * operands;
+  const int64_t most = (static_cast<int64_t>(LN_SMEM) / per_sm - r.weight_bytes) / stage_bytes;
+  int64_t stages = (operands == 1 ? LN_AHEAD_FWD : LN_AHEAD_BWD) / per_sm / stage_bytes;
+  if (stages < 2) stages = 2;
+  if (stages > most) stages = most;
   r.stages = static_cast<int>(stages > LN_MAX_STAGES ? LN_MAX_STAGES : stages);
   return r;
 }
