@@ -131,10 +131,18 @@ template <int TPR>
 __host__ __device__ constexpr int ln_groups() { return TPR == 32 ? LN_GROUPS : 1; }
 template <int TPR>
 __host__ __device__ constexpr int ln_threads() { return TPR * ln_groups<TPR>() + (TPR == 32 ? 32 : 0); }      // with the fetching warp
-// CTAs of one SM.  The backward writes a partial sum per CTA, so that it takes fewer.
-template <int TPR, int E, bool BWD>
+// CTAs of one SM; E: elements a thread, SIZE: bytes of one.  The backward writes a partial sum per CTA, so that it takes fewer.
+template <int TPR, int E, bool BWD, int SIZE>
 __host__ __device__ constexpr int ln_per_sm() {
-  return TPR == 32 ? (BWD && E > 8 ? 2 : 3) : TPR == 128 ? (BWD ? 4 : E > 8 ? 5 : 6) : TPR == 256 ? (BWD ? 2 : 3) : 1;
+  return TPR == 32 ? (BWD && E > 8 ? 2 : 3) : TPR == 128 ? (BWD ? 4 : E > 8 ? 5 : SIZE == 2 ? 8 : 6) : TPR == 256 ? (BWD ? 2 : 3) : 1;
+}
+// Rows that the forward works on at a time.  A second one fills the waits of the first, and halves the barriers: where one CTA has the SM (8192 x 8192), where
+// a warp mostly waits (rows of up to 256; 512 to 1024 16-bit elements: 65536 x 1024 65 us one at a time on 6 CTAs, 58 on 8, 50 two at a time), and
+// where w and b are read again for every row (4096 x 16384 bf16: 64 against 57 us).  fp32 rows and weights gain nothing there (65536 x 1024 fp32 92 against
+// 94, 4096 x 16384 bf16 with fp32 weights 77 against 80).
+template <int TPR, int E, int SIZE, int WSIZE>
+__host__ __device__ constexpr int ln_batch() {
+  return TPR == 512 ? (E <= 16 || SIZE + WSIZE == 4 ? 2 : 1) : TPR == 128 ? (E <= 8 && SIZE == 2 ? 2 : 1) : TPR == 32 && E <= 8 ? 2 : 1;
 }
 
 // Whether access k of a thread can lie behind the row's end.  A CTA-wide row fills more than half of its shape (ln_shape), so the first half of the
@@ -305,10 +313,9 @@ __device__ __forceinline__ void ln_weight(const W* w, int c, int cols, float dfl
   }
 }
 
-// BATCH rows are worked on at a time (1 or 2): with one CTA on an SM, or a row so short that a warp mostly waits, a second one fills the waits of the
-// first.
+// BATCH: ln_batch.
 template <typename T, typename W, int VEC, int PER, int TPR, int BATCH>
-__global__ void __launch_bounds__(ln_threads<TPR>(), ln_per_sm<TPR, PER * VEC, false>())
+__global__ void __launch_bounds__(ln_threads<TPR>(), ln_per_sm<TPR, PER * VEC, false, sizeof(T)>())
 ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ b, T* __restrict__ y, float* __restrict__ mean,
               float* __restrict__ rstd, int rows, int cols, int64_t ldy, float eps, const LnRing ring, uint32_t* status) {
   constexpr int GROUPS = ln_groups<TPR>();
@@ -443,7 +450,7 @@ ln_fwd_kernel(const LnSource sx, const W* __restrict__ w, const W* __restrict__ 
 
 // Backward.  The columns' sums of dy h and dy stay in registers until the end: one partial sum per CTA (part[2][gridDim.x][cols], first dw's).
 template <typename T, typename W, int VEC, int PER, int TPR>
-__global__ void __launch_bounds__(ln_threads<TPR>(), ln_per_sm<TPR, PER * VEC, true>())
+__global__ void __launch_bounds__(ln_threads<TPR>(), ln_per_sm<TPR, PER * VEC, true, sizeof(T)>())
 ln_bwd_kernel(const LnSource sg, const LnSource sx, const W* __restrict__ w, const float* __restrict__ mean, const float* __restrict__ rstd,
               T* __restrict__ dx, float* __restrict__ part, int rows, int cols, int64_t lddx, const LnRing ring, uint32_t* status) {
   constexpr int GROUPS = ln_groups<TPR>();
@@ -709,7 +716,7 @@ static LnRing ln_ring(int64_t cols, int size, int align, int operands, int group
 
 template <typename T, typename W, int VEC, int PER, int TPR>
 static int ln_fwd_rows(const LayerNormArgs& a, int align, const DeviceInfo* dev, cudaStream_t stream, bool* done) {
-  constexpr int GROUPS = ln_groups<TPR>(), PER_SM = ln_per_sm<TPR, PER * VEC, false>(), BATCH = (TPR == 512 && PER * VEC <= 16) || (TPR == 32 && PER * VEC <= 8) ? 2 : 1;
+  constexpr int GROUPS = ln_groups<TPR>(), PER_SM = ln_per_sm<TPR, PER * VEC, false, sizeof(T)>(), BATCH = ln_batch<TPR, PER * VEC, sizeof(T), sizeof(W)>();
   const LnRing ring = ln_ring(a.cols, sizeof(T), align, 1, GROUPS, PER_SM, BATCH, 0);
   if (ring.stages < 1 || (TPR > 32 && a.cols <= TPR * VEC * (PER / 2))) return B200K_OK;   // the second is what ln_inside relies on
   auto kernel = ln_fwd_kernel<T, W, VEC, PER, TPR, BATCH>;
@@ -727,7 +734,7 @@ static int ln_fwd_rows(const LayerNormArgs& a, int align, const DeviceInfo* dev,
 
 template <typename T, typename W, int VEC, int PER, int TPR>
 static int ln_bwd_rows(const LayerNormArgs& a, int align, const DeviceInfo* dev, float* part, int* parts, cudaStream_t stream, bool* done) {
-  constexpr int GROUPS = ln_groups<TPR>(), PER_SM = ln_per_sm<TPR, PER * VEC, true>();
+  constexpr int GROUPS = ln_groups<TPR>(), PER_SM = ln_per_sm<TPR, PER * VEC, true, sizeof(T)>();
   const LnRing ring = ln_ring(a.cols, sizeof(T), align, 2, GROUPS, PER_SM, 1, PER * VEC > 16 ? sizeof(W) : 0);
   if (ring.stages < 1 || (TPR > 32 && a.cols <= TPR * VEC * (PER / 2))) return B200K_OK;   // the second is what ln_inside relies on
   auto kernel = ln_bwd_kernel<T, W, VEC, PER, TPR>;
