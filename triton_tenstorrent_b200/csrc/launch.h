@@ -173,7 +173,7 @@ struct LayerNormArgs {
   int dtype, wdtype;
   float eps;
 };
-constexpr int LN_MAX_PARTS = 592;   // partial sums of dw / db the backward writes at most: four CTAs on each of 148 SMs
+constexpr int LN_MAX_PARTS = 888;   // partial sums of dw / db the backward writes at most: six CTAs on each of 148 SMs
 int layer_norm_fwd(const LayerNormArgs& a, cudaStream_t s);
 int layer_norm_bwd(const LayerNormArgs& a, cudaStream_t s);
 int64_t layer_norm_bwd_workspace(int64_t rows, int64_t cols);
