@@ -116,14 +116,15 @@ __global__ void __launch_bounds__(256) ln_dw_loop_kernel(const T* __restrict__ d
 // their way into a ring in shared memory meanwhile.
 //
 // A row is worked on in steps that wait for one another (load, row sum, second sum, store), and registers for enough rows at a time do not exist
-// next to the backward's 2 N running sums; the ring keeps 60 to 190 KB per SM on their way instead, whatever the arithmetic waits for.
+// next to the backward's 2 N running sums; the ring keeps 60 KB (backward: 140) per SM on their way instead, whatever the arithmetic waits for.
 // Rows come as untiled bulk copies of the 16-byte blocks that they touch, so that any length and alignment arrives at full rate; only the
 // reads from shared memory and the stores go by VEC, the widest access that the operands' alignment allows.
 // A CTA-wide row is fetched by the CTA's first thread, behind a barrier that the row sum needs anyway; a warp of its own for it, as the CTAs of
 // narrow rows have, would cost the others registers (17 warps leave them 96 each, 16 warps 128: backward, 16384 x 4096 bf16, 82 against 64 us).
 //
-// Measured, inputs larger than L2, of 6460 GB/s: 16384 x 4096 bf16 forward 46 us (5.8 TB/s), backward 64 us (6.3 TB/s); 8192 x 8192 bf16 with fp32
-// weights 49 and 75 us.  Rows on odd boundaries (16384 x 4095 bf16: 76 and 85 us) are bound by their 2-byte stores and the LSU.
+// Measured back to back (the backward with its join), inputs larger than L2, of 6460 GB/s: 16384 x 4096 bf16 forward 47 us (5.7 TB/s), backward 71 us
+// (5.7 TB/s); 65536 x 4096 169 and 246 us (6.4, 6.5 TB/s); 8192 x 8192 bf16 with fp32 weights 48 and 75 us.  Rows on odd boundaries (16384 x 4095
+// bf16: 79 and 87 us) are bound by their 2-byte stores and the LSU.
 // ---------------------------------------------------------------------------------------------
 constexpr int LN_GROUPS = 8;          // rows at a time of a CTA whose warps take a row each
 constexpr int LN_MAX_STAGES = 8;
