@@ -106,15 +106,19 @@ def offsets(sizes):
 
 
 # ---------------------------------------------------------------------------------------------
-# The 8-bit states: BLOCK consecutive elements share a scale, a power of two; a code has 4 exponent bits and 3 (first moment, with a sign) or
-# 4 (root of the second moment) mantissa bits, value(c) = (1 + mantissa / 2^bits) * 2^exponent, value(0) = 0; the largest code is left to NaN.
-# Rounding is stochastic, with 16 random bits that a hash draws from (seed, step, tensor, element); a root above zero takes code 1 at least.
+# The 8-bit states: BLOCK consecutive elements share a 32-bit scale; a code has 4 exponent bits and 3 (first moment, with a sign) or 4 (root
+# of the second moment) mantissa bits, value(c) = (1 + mantissa / 2^bits) * 2^exponent, value(0) = 0; the largest code is left to NaN.
+# Rounding is stochastic, with 16 random bits that a hash draws from (seed, step, tensor, element).
 # ---------------------------------------------------------------------------------------------
 def code_values(bits):
     c = torch.arange(1 << (4 + bits), dtype=torch.float64)
     v = (1 + torch.remainder(c, 1 << bits) / (1 << bits)) * torch.exp2(torch.floor(c / (1 << bits)))
     v[0] = 0.0
     return v
+
+
+def top_value(bits):
+    return (2.0 - 2.0 ** (1 - bits)) * 2.0 ** 15
 
 
 def mix(x):
@@ -145,16 +149,14 @@ def decode(codes, scales, bits):
 def encode(x, random16, bits):
     """Codes and scales of finite x >= 0 (root of the second moment) or of any sign (first moment)."""
     mag = x.abs().view(-1, BLOCK)
-    # the power of two that brings the largest magnitude just below the largest code's value, (2 - 2^(1 - bits)) * 2^15
-    exponent = ((mag.amax(dim=1).view(torch.int32) + ((1 << (24 - bits)) - 1)) >> 23).clamp(min=16)
-    scales, inverse = ((exponent - 15) << 23).view(torch.float32), ((269 - exponent) << 23).view(torch.float32)
-    y = (mag * inverse[:, None]).view(-1)
+    top = torch.full_like(mag[:, 0], top_value(bits))
+    peak = mag.amax(dim=1)
+    scales = peak / top
+    inverse = torch.where(peak > 0, top / peak, torch.zeros_like(peak))
+    y = torch.minimum(mag * inverse[:, None], top[:, None]).view(-1)
     least = 1 + 2.0 ** -bits
     raw = (y.view(torch.int32) - (127 << 23) + (random16 << (7 - bits)).to(torch.int32)) >> (23 - bits)
-    if bits == 3:
-        small = ((2 * random16 + 1).to(torch.float32) * (least * 2.0 ** -17) < y).to(torch.int32)
-    else:
-        small = (y > 0).to(torch.int32)
+    small = ((2 * random16 + 1).to(torch.float32) * (least * 2.0 ** -17) < y).to(torch.int32)
     code = torch.where(y < least, small, raw)
     if bits == 3:
         code = torch.where(x < 0, code + 128, code)
