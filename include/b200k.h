@@ -293,6 +293,8 @@ int64_t b200k_lce_workspace(int T, int D, int V, int backward);
  *                   codes of sqrt(v).  Codes: 4 exponent and 3 (m, after a sign bit) or 4 mantissa bits, value(c) = (1 + mantissa / 2^bits)
  *                   2^exponent, value(0) = 0, largest code NaN; an element is value(code) * scale, the scale a power of two.  Rounding is stochastic, with random
  *                   bits from a hash of (seed, t, index, element); all zero bytes and scales are the zero state.
+ *   state_bits 8 + B200K_ADAMW_PEAK_SCALES   the same codes by an older rule, which goes on with states that were begun with it: scale = the block's largest
+ *                   magnitude / the largest code's value, and an element of v below code 1 is rounded to code 1 or to zero as m is (with 8 alone it takes code 1)
  *   master          fp32 [n] copy that the step works on, p then being its rounded image; for all tensors of the call or for none;
  *                   16-bit parameters only
  * m, v and master are 16-byte aligned; p and g need the alignment of their type only (aligned ones are faster).
@@ -301,6 +303,7 @@ int64_t b200k_lce_workspace(int T, int D, int V, int backward);
  * lr_dev, grad_scale_dev: one device float each that replaces lr / grad_scale, or null.  eps is 0 or at least 2^-126 (the kernel's reciprocal
  * takes subnormal numbers for zero).
  */
+enum { B200K_ADAMW_PEAK_SCALES = 256 /* added to state_bits 8 */ };
 typedef struct b200k_adamw_tensor {
   void* p;
   const void* g;

@@ -480,3 +480,95 @@ def test_8_bit_moments_equal_the_formula_in_ieee_fp32(spread, size):
         assert torch.equal(held["exp_avg_sq_root"], r8)
         got = held["exp_avg"]
         assert bool(((got == m8) | ((got & 127 == 0) & (m8 & 127 == 0))).all())
+
+
+def peak_encode(x, random16, bits):
+    """Codes and scales by the rule scale = a block's peak / the largest code's value, for both moments with the same rounding below code 1."""
+    top = (2.0 - 2.0 ** (1 - bits)) * 2.0 ** 15
+    mag = x.abs().view(-1, BLOCK)
+    peak = mag.amax(dim=1)
+    tops = torch.full_like(peak, top)
+    scales, inverse = peak / tops, torch.where(peak > 0, tops / peak, torch.zeros_like(peak))
+    y = torch.minimum(mag * inverse[:, None], tops[:, None]).view(-1)
+    least = 1 + 2.0 ** -bits
+    raw = (y.view(torch.int32) - (127 << 23) + (random16 << (7 - bits)).to(torch.int32)) >> (23 - bits)
+    small = (2 * random16 + 1).to(torch.float32) * (least * 2.0 ** -17) < y
+    code = torch.where(y < least, small.to(torch.int32), raw)
+    return (torch.where(x < 0, code + 128, code) if bits == 3 else code).to(torch.uint8), scales
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,master", [(torch.float32, False), (torch.bfloat16, False), (torch.float16, True)])
+@pytest.mark.parametrize("spread,size", [(0.0, 1.0), (1.5, 1e-3), (6.0, 1e2), (1.5, 1e-18)])
+def test_a_state_with_other_scales_goes_on_with_their_rule(spread, size, dtype, master):
+    """Codes and scales equal to the formula in IEEE fp32, three steps after load_state_dict took over moments whose scales are the blocks' peaks / the
+    largest code's value; then once more through state_dict.  (The sign of a zero is free.)"""
+    n = (1 << 19) + 3
+    padded = -(-n // BLOCK) * BLOCK
+    g = torch.Generator(device="cuda").manual_seed(int(spread * 10))
+    rn = lambda: torch.randn(n, generator=g, device="cuda") * torch.exp(torch.randn(n, generator=g, device="cuda") * spread)  # noqa: E731
+    pad = lambda x: torch.nn.functional.pad(x, (0, padded - n))  # noqa: E731
+    params = [(torch.randn(n, generator=g, device="cuda")).to(dtype)]
+    opt = tt.AdamW(params, betas=(0.9, 0.999), state_bits=8, seed=9, master_weights=master)
+    half_way = torch.full((padded,), 32768, dtype=torch.int64, device="cuda")
+    live = torch.rand(padded, generator=g, device="cuda") < 0.95
+    live[: 4 * BLOCK] = False
+    m8, ms = peak_encode(pad(rn() * size * 0.1) * live, half_way, 3)
+    r8, rs = peak_encode(pad(rn() * size).abs() * live, half_way, 4)
+    held = opt.state_dict()
+    held.update(step=70, exp_avg=m8, exp_avg_scale=ms, exp_avg_sq_root=r8, exp_avg_sq_root_scale=rs)
+    opt.load_state_dict(held)
+    for t in range(71, 75):
+        if t == 74:
+            opt.load_state_dict(opt.state_dict())
+        grad = rn() * size
+        grad[: 4 * BLOCK] = 0.0
+        opt.step([grad.to(dtype) if dtype == torch.bfloat16 else grad])
+        grad = pad((grad.to(dtype) if dtype == torch.bfloat16 else grad).float())
+        m = plain_decode(m8, ms, 3) * 0.9 + grad * (1 - 0.9)
+        r = plain_decode(r8, rs, 4)
+        root = torch.sqrt(r * r * 0.999 + (grad * grad) * (1 - 0.999))
+        lo, hi = (torch.from_numpy(x).cuda() for x in random16(padded, 0, t, 9))
+        m8, ms = peak_encode(m, lo, 3)
+        r8, rs = peak_encode(root, hi, 4)
+        held = opt.state_dict()
+        assert torch.equal(held["exp_avg_scale"], ms) and torch.equal(held["exp_avg_sq_root_scale"], rs)
+        assert torch.equal(held["exp_avg_sq_root"], r8)
+        got = held["exp_avg"]
+        assert bool(((got == m8) | ((got & 127 == 0) & (m8 & 127 == 0))).all())
+
+
+@pytest.mark.gpu
+def test_peak_scales_of_tiny_and_non_finite_blocks():
+    """Blocks whose peak has no finite inverse keep finite moments, within a step of their codes (1/8, of at least 2^-126), and a non-finite gradient stays with
+    its element."""
+    n = 4 * BLOCK
+    opt = tt.AdamW([torch.zeros(n, device="cuda")], state_bits=8)
+    m = torch.ones(n, device="cuda")
+    m[BLOCK:2 * BLOCK] = torch.linspace(1e-36, 1e-34, BLOCK, device="cuda")
+    m[2 * BLOCK:3 * BLOCK] = 0.0
+    half_way = torch.full((n,), 32768, dtype=torch.int64, device="cuda")
+    m8, ms = peak_encode(m, half_way, 3)
+    m8[BLOCK:2 * BLOCK], ms[1] = 30, 1e-37
+    held = opt.state_dict()
+    held.update(exp_avg=m8, exp_avg_scale=ms)
+    opt.load_state_dict(held)
+    was = opt.moments()[0].clone()
+    grad = torch.zeros(n, device="cuda")
+    grad[2 * BLOCK + 5], grad[3 * BLOCK + 7] = float("nan"), float("inf")
+    opt.step([grad])
+    now = opt.moments()[0]
+    bad = torch.zeros(n, dtype=torch.bool, device="cuda")
+    bad[[2 * BLOCK + 5, 3 * BLOCK + 7]] = True
+    assert bool((now.isnan() == bad).all()) and float(opt._ms[2]) == 0
+    want = was * 0.9
+    assert bool(((now - want).abs()[~bad] <= (want / 8 * 1.001 + 1.25 * 2.0 ** -126)[~bad]).all())
+
+
+def test_state_bits_of_the_entry_point():
+    rows = np.zeros((1, 9), dtype=np.int64)
+    rows[:, [optim._P, optim._G, optim._M, optim._V]] = 4096
+    rows[:, optim._N] = 10
+    for bits in (256, 32 + _lib.ADAMW_PEAK_SCALES, 8 + 2 * _lib.ADAMW_PEAK_SCALES, 8 + _lib.ADAMW_PEAK_SCALES):      # the last one: null scales
+        assert _lib.load().b200k_adamw(rows.ctypes.data, 1, 0, 0, bits, 4096, 1e-3, None, 0.9, 0.999, 1e-8, 0.0, 1.0, None, 0, 1, None) == _lib.ERR_INVALID_ARG
+    assert "null pointer" in _lib.last_error()

@@ -23,6 +23,7 @@ BIAS_NONE, BIAS_ROW_F32, BIAS_FULL_BF16 = 0, 1, 2
 ACT_NONE, ACT_RELU, ACT_LEAKY_RELU = 0, 1, 2
 DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 REDUCE_NONE, REDUCE_MEAN, REDUCE_SUM = 0, 1, 2
+ADAMW_PEAK_SCALES = 256
 ARG_PTR, ARG_I32, ARG_I64, ARG_F32 = 0, 1, 2, 3
 
 

@@ -16,6 +16,8 @@
 // small: a moment that has not changed has the same code in every step, whatever the largest element does.  The 16 random bits of an
 // element come from a hash of (seed, step, tensor, element): the result is a function of the inputs alone.
 // An r above zero takes code 1 at least: with r = 0 beside an m that is not, the next update would be unbounded.
+// B200K_ADAMW_PEAK_SCALES: the older rule, for states that were begun with it: scale = the block's peak / the largest finite code's value, and an r
+// below code 1 is rounded like an m there, up to code 1 with a probability equal to the fraction, else to zero.
 // A non-finite moment takes the NaN code and does not enter the scale, so that it stays with its element.
 //
 // Bound: HBM with fp32 moments (184 M fp32 parameters, 28 bytes each: 800 us, 6.4 TB/s, all of the copy rate); with 8 bits the instructions, about 90 an
@@ -81,6 +83,19 @@ __device__ __forceinline__ uint32_t scale_exponent(float peak) {
   const uint32_t e = (__float_as_uint(peak) + ((1u << (24 - MB)) - 1)) >> 23;
   return e < 16 ? 16 : e;
 }
+template <int MB>
+__device__ __forceinline__ constexpr float top_value() { return (2.f - 2.f / (1 << MB)) * 32768.f; }
+// Scale and inverse of a block by its peak: two divisions, so that each is the formula's.  Where the inverse would overflow (peaks below 2^-112, and zero, whose
+// scale is zero) it is the other rule's for the smallest peaks.
+template <int MB>
+__device__ __forceinline__ void peak_scale(float peak, float& scale, float& inverse) {
+  scale = __fdiv_rn(peak, top_value<MB>());
+  inverse = __fdiv_rn(top_value<MB>(), peak);
+  if (!(inverse <= 3.4028234663852886e38f)) {
+    scale = peak == 0.f ? 0.f : 0x1p-126f;
+    inverse = 0x1p126f;
+  }
+}
 __device__ __forceinline__ float scale_of(uint32_t e) { return __uint_as_float((e - 15) << 23); }
 __device__ __forceinline__ float inverse_scale_of(uint32_t e) { return __uint_as_float((269 - e) << 23); }
 
@@ -132,7 +147,8 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
 // A normal code is the exponent and the MB first mantissa bits of |x| * inverse (in [1, 2^16), so that exponent 127 is 0), after the random bits were
 // added just below them.  Multiplied by 2^(1 + MB) those 4 + MB bits are the top byte of the word (m's with a zero above them), the random bits
 // are bytes 1 and 2 of what is added, and the exponent's offset is a constant in byte 3: a byte permutation and a multiply-add.
-template <int MB>
+// PEAK: by the older rule; a product with the inverse may then pass the largest code's value by a rounding.
+template <int MB, bool PEAK>
 __device__ __forceinline__ uint32_t encode4(const float (&x)[4], float inverse, const uint32_t (&hash)[4], uint32_t up, bool finite) {
   constexpr float LEAST = 1.f + 1.f / (1 << MB);       // value of code 1
   uint32_t c[4];
@@ -140,6 +156,7 @@ __device__ __forceinline__ uint32_t encode4(const float (&x)[4], float inverse, 
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     y[j] = __fmul_rn(fabsf(x[j]), inverse);
+    if (PEAK) y[j] = fminf(y[j], top_value<MB>());
     // -(127 << 23) * up is 8 << 24 and 16 << 24 modulo 2^32
     const uint32_t add = __byte_perm(hash[j], MB == 3 ? 0x08u : 0x10u, MB == 3 ? 0x4105 : 0x4325);
     c[j] = __float_as_uint(y[j]) * up + add;
@@ -147,9 +164,9 @@ __device__ __forceinline__ uint32_t encode4(const float (&x)[4], float inverse, 
   if (min3(min3(y[0], y[1], y[2]), y[3], y[3]) < LEAST) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      // below code 1: an m up to it with probability y / value(1), an r above zero always.  u = 1 + (2 r + 1) / 2^17 for the 16 bits r.
-      const float u = __uint_as_float((hash[j] & 0xFFFFu) * 128u + 0x3F800040u);
-      const uint32_t small = (MB == 3 ? fmaf(u, LEAST, -LEAST) : 0.f) < y[j] ? 1u << 24 : 0u;
+      // below code 1: an m up to it with probability y / value(1), an r above zero always (by the older rule like an m).  u = 1 + (2 r + 1) / 2^17 for the 16 bits r.
+      const float u = __uint_as_float((MB == 3 ? hash[j] & 0xFFFFu : hash[j] >> 16) * 128u + 0x3F800040u);
+      const uint32_t small = (MB == 3 || PEAK ? fmaf(u, LEAST, -LEAST) : 0.f) < y[j] ? 1u << 24 : 0u;
       c[j] = y[j] < LEAST ? small : c[j];
     }
   }
@@ -284,8 +301,11 @@ __device__ __forceinline__ void adamw_read(AdamwBlock<P, G, MASTER, BITS>& k, co
   }
 }
 
-template <typename P, typename G, bool MASTER, int BITS, int CAP>
+// KIND: 32, 8, or 8 + B200K_ADAMW_PEAK_SCALES.
+template <typename P, typename G, bool MASTER, int KIND, int CAP>
 __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const __grid_constant__ AdamwTable<CAP> table, const AdamwParams q) {
+  constexpr int BITS = KIND % B200K_ADAMW_PEAK_SCALES;
+  constexpr bool PEAK = KIND >= B200K_ADAMW_PEAK_SCALES;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const double lr = q.lr_dev != nullptr ? static_cast<double>(*q.lr_dev) : q.lr;
   const float step_size = static_cast<float>(lr * q.state->inv_bc1);
@@ -382,8 +402,17 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const __grid_const
         peak_m = warp_max_nonneg(peak_m);
         peak_r = warp_max_nonneg(peak_r);
       }
-      const uint32_t exp_m = scale_exponent<3>(peak_m), exp_r = scale_exponent<4>(peak_r);
-      const float inv_m = inverse_scale_of(exp_m), inv_r = inverse_scale_of(exp_r);
+      float scale_m, scale_r, inv_m, inv_r;
+      if constexpr (PEAK) {
+        peak_scale<3>(peak_m, scale_m, inv_m);
+        peak_scale<4>(peak_r, scale_r, inv_r);
+      } else {
+        const uint32_t exp_m = scale_exponent<3>(peak_m), exp_r = scale_exponent<4>(peak_r);
+        scale_m = scale_of(exp_m);
+        scale_r = scale_of(exp_r);
+        inv_m = inverse_scale_of(exp_m);
+        inv_r = inverse_scale_of(exp_r);
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int64_t i = base + h * 128 + lane * 4;
@@ -392,12 +421,12 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const __grid_const
         for (int j = 0; j < 4; ++j) hash[j] = mix32(static_cast<uint32_t>(i) + j + salt, q.two16);
         // behind the tensor's end the codes are those of zero
         *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.m) + i) =
-            peak_m == 0.f && finite_m ? 0u : encode4<3>(m1[h], inv_m, hash, q.two4, finite_m);
-        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.v) + i) = peak_r == 0.f && finite_r ? 0u : encode4<4>(root[h], inv_r, hash, q.two5, finite_r);
+            peak_m == 0.f && finite_m ? 0u : encode4<3, PEAK>(m1[h], inv_m, hash, q.two4, finite_m);
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.v) + i) = peak_r == 0.f && finite_r ? 0u : encode4<4, PEAK>(root[h], inv_r, hash, q.two5, finite_r);
       }
       if (lane == 0) {
-        t.m_scale[block] = scale_of(exp_m);
-        t.v_scale[block] = scale_of(exp_r);
+        t.m_scale[block] = scale_m;
+        t.v_scale[block] = scale_r;
       }
     }
   }
@@ -446,7 +475,7 @@ __global__ void __launch_bounds__(256) adamw_moments_kernel(const uint8_t* __res
 // ---------------------------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------------------------
-template <typename P, typename G, bool MASTER, int BITS, int CAP>
+template <typename P, typename G, bool MASTER, int KIND, int CAP>
 static int adamw_launch(const b200k_adamw_tensor* tensors, int n, AdamwParams q, cudaStream_t stream) {
   AdamwTable<CAP> table;
   int used = 0;
@@ -458,7 +487,7 @@ static int adamw_launch(const b200k_adamw_tensor* tensors, int n, AdamwParams q,
       for (int k = used; k <= CAP; ++k) table.first_chunk[k] = static_cast<int>(chunks);
       q.n = used;
       q.advance = i == n ? advance : 0;
-      adamw_kernel<P, G, MASTER, BITS, CAP><<<static_cast<unsigned>(chunks), ADAMW_THREADS, 0, stream>>>(table, q);
+      adamw_kernel<P, G, MASTER, KIND, CAP><<<static_cast<unsigned>(chunks), ADAMW_THREADS, 0, stream>>>(table, q);
       count_launch();
       B200K_CHECK_LAUNCH("adamw_kernel");
       if (i == n) break;
@@ -473,11 +502,14 @@ static int adamw_launch(const b200k_adamw_tensor* tensors, int n, AdamwParams q,
   return B200K_OK;
 }
 
+template <typename P, typename G, bool MASTER, int KIND>
+static int adamw_table(const b200k_adamw_tensor* t, int n, const AdamwParams& q, cudaStream_t s) {
+  return n <= ADAMW_SMALL_TABLE ? adamw_launch<P, G, MASTER, KIND, ADAMW_SMALL_TABLE>(t, n, q, s) : adamw_launch<P, G, MASTER, KIND, ADAMW_LARGE_TABLE>(t, n, q, s);
+}
 template <typename P, typename G, bool MASTER>
 static int adamw_bits(const b200k_adamw_tensor* t, int n, int bits, const AdamwParams& q, cudaStream_t s) {
-  if (n <= ADAMW_SMALL_TABLE)
-    return bits == 8 ? adamw_launch<P, G, MASTER, 8, ADAMW_SMALL_TABLE>(t, n, q, s) : adamw_launch<P, G, MASTER, 32, ADAMW_SMALL_TABLE>(t, n, q, s);
-  return bits == 8 ? adamw_launch<P, G, MASTER, 8, ADAMW_LARGE_TABLE>(t, n, q, s) : adamw_launch<P, G, MASTER, 32, ADAMW_LARGE_TABLE>(t, n, q, s);
+  if (bits == 32) return adamw_table<P, G, MASTER, 32>(t, n, q, s);
+  return bits == 8 ? adamw_table<P, G, MASTER, 8>(t, n, q, s) : adamw_table<P, G, MASTER, 8 + B200K_ADAMW_PEAK_SCALES>(t, n, q, s);
 }
 
 template <typename P>
@@ -491,7 +523,8 @@ int adamw(const AdamwArgs& a, cudaStream_t stream) {
   if (a.dtype < B200K_DTYPE_F32 || a.dtype > B200K_DTYPE_F16) return set_error(B200K_ERR_INVALID_ARG, "adamw: bad parameter type %d", a.dtype);
   if (a.gdtype != a.dtype && a.gdtype != B200K_DTYPE_F32)
     return set_error(B200K_ERR_INVALID_ARG, "adamw: gradients have the parameters' type or fp32 (got %d for parameters of type %d)", a.gdtype, a.dtype);
-  if (a.state_bits != 8 && a.state_bits != 32) return set_error(B200K_ERR_INVALID_ARG, "adamw: state_bits must be 8 or 32 (got %d)", a.state_bits);
+  if (a.state_bits != 8 && a.state_bits != 32 && a.state_bits != 8 + B200K_ADAMW_PEAK_SCALES)
+    return set_error(B200K_ERR_INVALID_ARG, "adamw: state_bits must be 8 (+ B200K_ADAMW_PEAK_SCALES) or 32 (got %d)", a.state_bits);
   if (a.state == nullptr || (reinterpret_cast<uintptr_t>(a.state) & 7u)) return set_error(B200K_ERR_INVALID_ARG, "adamw: null or misaligned state");
   if (!(a.beta1 >= 0.0 && a.beta1 < 1.0 && a.beta2 >= 0.0 && a.beta2 < 1.0))
     return set_error(B200K_ERR_INVALID_ARG, "adamw: betas must be in [0, 1) (got %g, %g)", a.beta1, a.beta2);
@@ -505,7 +538,7 @@ int adamw(const AdamwArgs& a, cudaStream_t stream) {
   for (int i = 0; i < a.n; ++i) {
     const b200k_adamw_tensor& t = a.tensors[i];
     if (t.n <= 0 || t.n > (int64_t(1) << 40)) return set_error(B200K_ERR_INVALID_ARG, "adamw: tensor %d has %lld elements", i, (long long)t.n);
-    if (t.p == nullptr || t.g == nullptr || t.m == nullptr || t.v == nullptr || (a.state_bits == 8 && (t.m_scale == nullptr || t.v_scale == nullptr)))
+    if (t.p == nullptr || t.g == nullptr || t.m == nullptr || t.v == nullptr || (a.state_bits != 32 && (t.m_scale == nullptr || t.v_scale == nullptr)))
       return set_error(B200K_ERR_INVALID_ARG, "adamw: tensor %d has a null pointer", i);
     if ((t.master != nullptr) != master) return set_error(B200K_ERR_INVALID_ARG, "adamw: tensor %d differs in having a master copy", i);
     if ((reinterpret_cast<uintptr_t>(t.p) & (psize - 1)) || (reinterpret_cast<uintptr_t>(t.g) & (gsize - 1)))

@@ -33,7 +33,7 @@ class AdamW:
     lr              a number, or an fp32 CUDA tensor of one element that a captured step reads at each replay; like eps and weight_decay
                     it may be changed between steps (opt.lr = ...)
     state_bits      32: fp32 moments, 8 bytes a parameter.  8: one byte each for m and sqrt(v), with an fp32 scale per 256 elements;
-                    stochastic rounding, reproducible from `seed`
+                    stochastic rounding, reproducible from `seed`.  The scales are powers of two, unless load_state_dict took over a state with others
     master_weights  keep fp32 copies of the 16-bit parameters and update those; without them a 16-bit parameter loses every
                     update below half a unit in its last place
 
@@ -78,6 +78,7 @@ class AdamW:
         else:
             self._m, self._v = (torch.zeros(total, device=self.device, dtype=torch.uint8) for _ in range(2))
             self._ms, self._vs = (torch.zeros(total // _BLOCK, device=self.device) for _ in range(2))
+        self._peak_scales = False
         low = [i for i, p in enumerate(self.params) if p.dtype != torch.float32]
         self.master = None
         if self.master_weights and low:
@@ -185,7 +186,7 @@ class AdamW:
         with _on(self.device):
             stream = _stream()
             for k, (dtype, gdtype, rows) in enumerate(launches):
-                _lib.check(entry(rows.ctypes.data, len(rows), _DTYPES[dtype], _DTYPES[gdtype], self.state_bits, self._state.data_ptr(), lr, lr_ptr,
+                _lib.check(entry(rows.ctypes.data, len(rows), _DTYPES[dtype], _DTYPES[gdtype], self.state_bits + self._peak_scales * _lib.ADAMW_PEAK_SCALES, self._state.data_ptr(), lr, lr_ptr,
                                  b1, b2, self.eps, self.weight_decay, scale, scale_ptr, self.seed, int(k == len(launches) - 1), stream))
         # a backward pass that still needs an old value must fail instead of using the new one
         torch.autograd.graph.increment_version(touched)
@@ -228,7 +229,8 @@ class AdamW:
         return held
 
     def load_state_dict(self, held: dict):
-        """Takes over what state_dict() of an optimiser over the same list of shapes gave."""
+        """Takes over what state_dict() of an optimiser over the same list of shapes gave.  The scales of 8-bit moments say by which rule they were made:
+        powers of two, or each block's largest magnitude / the largest code's value; the steps to come go by the same one."""
         want = {"exp_avg": self._m}
         want.update({"exp_avg_sq": self._v} if self.state_bits == 32 else
                     {"exp_avg_scale": self._ms, "exp_avg_sq_root": self._v, "exp_avg_sq_root_scale": self._vs})
@@ -243,4 +245,7 @@ class AdamW:
             raise ValueError("AdamW: step must be >= 0")
         for name, t in want.items():
             t.copy_(held[name])
+        if self.state_bits == 8:         # a power of two has the mantissa 1/2; blocks of zeros may have the scale zero by either rule
+            mantissa = torch.frexp(torch.cat([self._ms, self._vs])).mantissa
+            self._peak_scales = bool(((mantissa != 0.5) & (mantissa != 0)).any())
         self._set_step(int(held["step"]))
