@@ -3,6 +3,9 @@
 Tolerances: U = 2^-24 is half a unit in the last place of fp32.  m takes three roundings of terms no larger than |b1 m| + |(1 - b1) g|, v four; b1,
 1 - b1, b2 and 1 - b2 are themselves rounded once.  p takes the roundings of decay, step size, root, quotient and two sums: with D the size of the
 update, 4 U |p| + 24 U D covers them."""
+import copy
+import pickle
+
 import numpy as np
 import pytest
 import torch
@@ -572,3 +575,45 @@ def test_state_bits_of_the_entry_point():
     for bits in (256, 32 + _lib.ADAMW_PEAK_SCALES, 8 + 2 * _lib.ADAMW_PEAK_SCALES, 8 + _lib.ADAMW_PEAK_SCALES):      # the last one: null scales
         assert _lib.load().b200k_adamw(rows.ctypes.data, 1, 0, 0, bits, 4096, 1e-3, None, 0.9, 0.999, 1e-8, 0.0, 1.0, None, 0, 1, None) == _lib.ERR_INVALID_ARG
     assert "null pointer" in _lib.last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits,dtype,master", [(32, torch.float32, False), (8, torch.bfloat16, True), (8, torch.float32, False), (32, torch.float16, True)])
+@pytest.mark.parametrize("how", [copy.deepcopy, lambda x: pickle.loads(pickle.dumps(x))])
+def test_a_copied_optimiser_has_memory_of_its_own(bits, dtype, master, how):
+    params, grads = make(SHAPES, dtype, dtype)
+    a = tt.AdamW([torch.nn.Parameter(p) for p in params], state_bits=bits, master_weights=master, seed=4)
+    a.step(grads)
+    b = how(a)
+    addresses = lambda o: {t.data_ptr() for t in (*o.params, o._m, o._v, o._ms, o._vs, o.master, o._state) if t is not None and t.numel()}  # noqa: E731
+    assert not addresses(a) & addresses(b)
+    own = {optim._M: (b._m, 1), optim._V: (b._v, 1), optim._MS: (b._ms, BLOCK), optim._VS: (b._vs, BLOCK), optim._MASTER: (b.master, 1)}
+    for column, (t, per) in own.items():           # every address of the table lies in the copy's own buffers
+        at = b._table[:, column]
+        if t is None:
+            assert not at.any()
+        else:
+            assert (at == t.data_ptr() + np.array(b.offsets) // per * t.element_size()).all()
+    state = lambda o: [t.detach().clone() for t in (*o.params, *o.moments(), *([o.master] if master else []))]  # noqa: E731
+    before = state(a)
+    b.step(grads)
+    assert all(torch.equal(x, y) for x, y in zip(before, state(a))) and a.step_count() == 1 and b.step_count() == 2
+    after = state(b)
+    a.step(grads)
+    assert all(torch.equal(x, y) for x, y in zip(after, state(a))) and all(torch.equal(x, y) for x, y in zip(after, state(b)))
+    del a
+    b.step(grads)
+    assert b.step_count() == 3
+
+
+@pytest.mark.gpu
+def test_a_module_copied_with_its_optimiser():
+    layer = torch.nn.Linear(16, 8, device="cuda")
+    opt = tt.AdamW(layer.parameters())
+    layer2, opt2 = copy.deepcopy((layer, opt))
+    assert all(p is q for p, q in zip(opt2.params, layer2.parameters()))
+    x = torch.randn(4, 16, device="cuda")
+    for net, o in ((layer, opt), (layer2, opt2)):
+        net(x).square().sum().backward()
+        o.step()
+    assert all(torch.equal(p, q) for p, q in zip(layer.parameters(), layer2.parameters()))

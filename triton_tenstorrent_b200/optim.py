@@ -39,7 +39,8 @@ class AdamW:
 
     The moments live in flat buffers in which parameter i begins at element offsets[i], a multiple of 256 (split() gives views in the
     parameters' shapes).  One step count serves all parameters and lives on the device, so that a captured step() can be replayed.  Steps of one
-    optimiser follow one another: those on different streams have to be ordered by their caller."""
+    optimiser follow one another: those on different streams have to be ordered by their caller.  copy.deepcopy and pickle give an optimiser with
+    parameters and moments of its own (together with a module, in one call, its parameters are the copied module's)."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, state_bits: int = 32,
                  master_weights: bool = False, seed: int = 0):
@@ -79,29 +80,40 @@ class AdamW:
             self._m, self._v = (torch.zeros(total, device=self.device, dtype=torch.uint8) for _ in range(2))
             self._ms, self._vs = (torch.zeros(total // _BLOCK, device=self.device) for _ in range(2))
         self._peak_scales = False
-        low = [i for i, p in enumerate(self.params) if p.dtype != torch.float32]
         self.master = None
-        if self.master_weights and low:
+        if self.master_weights and any(p.dtype != torch.float32 for p in self.params):
             self.master = torch.zeros(total, device=self.device)
             for i, view in enumerate(self.split(self.master)):
                 view.copy_(self.params[i].detach())
         self._state = torch.empty(5, device=self.device, dtype=torch.float64)
         self._set_step(0)
-        # the columns that stay: moments, scales, master copies, sizes
+        self._shapes = [p.shape for p in self.params]
+        self._low = [i for i, p in enumerate(self.params) if p.dtype != torch.float32]
+        self._lay_table()
+        kinds = {p.dtype for p in self.params}
+        self._dtype = kinds.pop() if len(kinds) == 1 and all(p.numel() for p in self.params) else None     # the one type, if there is one
+
+    def _lay_table(self):
+        """The columns of the table that stay from step to step: addresses of this object's own moments, scales and master copies, and the sizes."""
         table = np.zeros((len(self.params), 9), dtype=np.int64)
         at = np.array(self.offsets, dtype=np.int64)
         width = self._m.element_size()
         table[:, _M], table[:, _V] = self._m.data_ptr() + at * width, self._v.data_ptr() + at * width
-        if state_bits == 8:
+        if self.state_bits == 8:
             table[:, _MS], table[:, _VS] = self._ms.data_ptr() + at // _BLOCK * 4, self._vs.data_ptr() + at // _BLOCK * 4
         if self.master is not None:
-            table[low, _MASTER] = self.master.data_ptr() + at[low] * 4
-        table[:, _N] = [p.numel() for p in self.params]
+            table[self._low, _MASTER] = self.master.data_ptr() + at[self._low] * 4
+        table[:, _N] = [shape.numel() for shape in self._shapes]
         table[:, _INDEX] = np.arange(len(self.params))
         self._table = table
-        self._shapes = [p.shape for p in self.params]
-        kinds = {p.dtype for p in self.params}
-        self._dtype = kinds.pop() if len(kinds) == 1 and all(p.numel() for p in self.params) else None     # the one type, if there is one
+
+    # A copy (copy.deepcopy, pickle) has buffers of its own: the addresses are taken anew.
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k != "_table"}
+
+    def __setstate__(self, held):
+        self.__dict__.update(held)
+        self._lay_table()
 
     def _check_hyper(self):
         if isinstance(self.lr, torch.Tensor):
