@@ -617,3 +617,15 @@ def test_a_module_copied_with_its_optimiser():
         net(x).square().sum().backward()
         o.step()
     assert all(torch.equal(p, q) for p, q in zip(layer.parameters(), layer2.parameters()))
+
+
+@pytest.mark.gpu
+def test_betas_cannot_be_changed_under_the_step_count():
+    p = torch.zeros(8, device="cuda")
+    opt = tt.AdamW([p], betas=(0.5, 0.75))
+    with pytest.raises(AttributeError):
+        opt.betas = (0.9, 0.999)
+    assert opt.betas == (0.5, 0.75)
+    opt.step([torch.ones(8, device="cuda")])
+    m, v = opt.moments()
+    assert bool((m[:8] == 0.5).all()) and bool((v[:8] == 0.25).all())

@@ -52,7 +52,7 @@ class AdamW:
         b1, b2 = (float(b) for b in betas)
         if not (0 <= b1 < 1 and 0 <= b2 < 1):
             raise ValueError(f"AdamW: betas must be in [0, 1), got {betas}")
-        self.betas, self.lr, self.eps, self.weight_decay = (b1, b2), lr, eps, weight_decay
+        self._betas, self.lr, self.eps, self.weight_decay = (b1, b2), lr, eps, weight_decay
         self._check_hyper()
         self.state_bits, self.master_weights, self.seed = state_bits, bool(master_weights), int(seed) & 0xFFFFFFFF
         for i, p in enumerate(self.params):
@@ -92,6 +92,11 @@ class AdamW:
         self._lay_table()
         kinds = {p.dtype for p in self.params}
         self._dtype = kinds.pop() if len(kinds) == 1 and all(p.numel() for p in self.params) else None     # the one type, if there is one
+
+    @property
+    def betas(self):
+        """(b1, b2), fixed at construction: the device counts their powers from step to step."""
+        return self._betas
 
     def _lay_table(self):
         """The columns of the table that stay from step to step: addresses of this object's own moments, scales and master copies, and the sizes."""
@@ -230,7 +235,8 @@ class AdamW:
         return launches, touched, grads
 
     def state_dict(self) -> dict:
-        """The state as tensors (copies): step, the moments as they are held, and the master copy."""
+        """The state as tensors (copies): step, the moments as they are held, and the master copy.  lr, betas, eps, weight_decay and seed are not part of it:
+        a run that is to go on as it was is given the same ones."""
         held = {"step": self.step_count(), "exp_avg": self._m.clone()}
         if self.state_bits == 32:
             held["exp_avg_sq"] = self._v.clone()
