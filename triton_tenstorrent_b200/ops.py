@@ -12,6 +12,7 @@ import contextlib
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -44,6 +45,12 @@ def _on(device):
 def _require_cuda():
     if not torch.cuda.is_available():
         raise RuntimeError("triton_tenstorrent_b200 needs a CUDA device (sm_100a); there is no CPU fallback")
+
+
+def _refuse_tangents(name: str, *tensors):
+    """Forward-mode derivatives (dual tensors) are not implemented: a result without a tangent would count as one of zero."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name}: forward-mode derivatives are not implemented (an argument carries a tangent)")
 
 
 def _to_device(t: torch.Tensor) -> torch.Tensor:
@@ -429,6 +436,7 @@ def matmul_tma_fused(a: torch.Tensor, b: torch.Tensor, bias: torch.Tensor, warp_
 def attention_with_lse(q, k, v, causal, sm_scale, warp_specialize: bool = True):
     """Returns (O, M): the attention output and the fp32 base-2 log-sum-exp rows the reference saves for
     its backward (examples/fused-attn/06-fused-attention.py:238,269)."""
+    _refuse_tangents("attention", q, k, v)
     HEAD_DIM_Q, HEAD_DIM_K, HEAD_DIM_V = q.shape[-1], k.shape[-1], v.shape[-1]
     assert HEAD_DIM_Q == HEAD_DIM_K and HEAD_DIM_K == HEAD_DIM_V
     assert HEAD_DIM_K in {16, 32, 64, 128, 256}
@@ -601,6 +609,7 @@ def _layer_norm_call(x, weight, bias, eps, stats):
 
 def _layer_norm_check(x, weight, bias, eps):
     _norm_input("layer_norm", x)
+    _refuse_tangents("layer_norm", x, weight, bias)
     if not eps >= 0:
         raise ValueError(f"layer_norm: eps must be >= 0, got {eps}")
     _norm_weight("weight", x, weight)
@@ -609,7 +618,7 @@ def _layer_norm_check(x, weight, bias, eps):
 
 def layer_norm_with_stats(x, weight=None, bias=None, eps: float = 1e-5):
     """Returns (y, mean, rstd): the layer norm of x over its last dimension and the fp32 row statistics (x's shape without its last
-    dimension) that layer_norm_backward takes."""
+    dimension) that layer_norm_backward takes.  Not differentiable itself."""
     _layer_norm_check(x, weight, bias, eps)
     if not x.is_cuda:
         _require_cuda()
@@ -624,6 +633,7 @@ def layer_norm_backward(dy, x, weight, mean, rstd, need_dx: bool = True, need_dw
     layer_norm_with_stats returned.  dw and db have the weight's type (fp32 without a weight).  A gradient that is not needed is None; a
     frozen norm then reads x and dy once only."""
     _norm_input("layer_norm_backward", x)
+    _refuse_tangents("layer_norm_backward", dy, x, weight, mean, rstd)
     shape, rows_shape, dtype, device = x.shape, x.shape[:-1], x.dtype, x.device
     if dy.shape != shape or dy.dtype is not dtype:
         raise ValueError(f"layer_norm_backward: dy must be {dtype} {tuple(shape)} like x, got {dy.dtype} {tuple(dy.shape)}")
@@ -678,7 +688,7 @@ class _layer_norm(torch.autograd.Function):
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5) -> torch.Tensor:
     """y = (x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x (fp32, bf16 or fp16; weight and bias in x's type or in
-    fp32, either may be None).  fp32 arithmetic, one rounding; differentiable in x, weight and bias."""
+    fp32, either may be None).  fp32 arithmetic, one rounding; differentiable in x, weight and bias (backward mode; dual tensors are refused)."""
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         return _layer_norm.apply(x, weight, bias, eps)
     _layer_norm_check(x, weight, bias, eps)
@@ -689,6 +699,7 @@ _REDUCTIONS = {"none": _lib.REDUCE_NONE, "mean": _lib.REDUCE_MEAN, "sum": _lib.R
 
 
 def _lce_check(name, h, weight, targets, ignore_index, reduction):
+    _refuse_tangents(name, h, weight)
     if reduction not in _REDUCTIONS:
         raise ValueError(f"{name}: unknown reduction {reduction!r} (expected 'none', 'mean' or 'sum')")
     if h.dtype not in (torch.bfloat16, torch.float16) or weight.dtype != h.dtype:
@@ -790,7 +801,7 @@ def linear_cross_entropy(h, weight, targets, ignore_index: int = -100, reduction
     """Cross entropy of the logits h . weight^T without ever storing them: h [..., D] and weight [V, D] in bf16 or fp16, targets int64.
     reduction "mean" (over the tokens whose target is not ignore_index; 0 without any), "sum", or "none" (fp32 in the shape of targets, 0 for
     ignored tokens).  What h holds for ignored tokens does not matter, NaN included; any other target outside [0, V) makes its token's loss
-    NaN.  Differentiable in h and weight."""
+    NaN.  Differentiable in h and weight (backward mode; dual tensors are refused)."""
     _lce_check("linear_cross_entropy", h, weight, targets, ignore_index, reduction)
     if torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad):
         return _linear_cross_entropy.apply(h, weight, targets, ignore_index, reduction)
