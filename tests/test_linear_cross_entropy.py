@@ -329,3 +329,59 @@ def test_entry_point_refusals():
         for bad in [dict(h=None), dict(w=None), dict(y=None), dict(lse=None), dict(other=None), dict(work=None), dict(work=264), dict(size=size[backward] - 1), dict(T=-1),
                     dict(D=0), dict(D=60), dict(V=0), dict(ldh=56), dict(ldw=68), dict(h=264), dict(red=3), dict(red=-1), dict(dt=0), dict(dt=3), dict(V=2 ** 30 + 1)]:
             assert call(**bad) == _lib.ERR_INVALID_ARG and "linear_cross_entropy" in _lib.last_error(), (backward, bad)
+
+
+def exactly(h, w, y):
+    """(lse, losses) of exactly representable logits in 64 bits, and the tolerance of either: no product or sum of a logit is rounded, so that what is left is the
+    sum of exponentials (64 U) and four roundings of lse and of the target's logit (its product with log2 e, that constant, the sum, the way back)."""
+    logits = h.double() @ w.double().t()
+    lse = torch.logsumexp(logits, 1)
+    hit = logits.gather(1, y[:, None])[:, 0]
+    return lse, lse - hit, 64 * U + 4 * U * (lse.abs() + hit.abs())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [5, 128, 200, 700])
+@pytest.mark.parametrize("D", [512, 4096, 8192])
+def test_exactly_representable_logits(T, D, dtype):
+    """Sums that are exact at every step must come out exact, whatever D: small whole numbers, a single feature that counts, features that end early,
+    large parts that cancel, and a row that is one feature."""
+    g = torch.Generator(device="cuda").manual_seed(D)
+    V = 777
+    y = torch.randint(0, V, (T,), generator=g, device="cuda")
+    whole = lambda *s: torch.randint(-3, 4, s, generator=g, device="cuda").to(dtype)  # noqa: E731
+    cases = [(whole(T, D), whole(V, D))]
+    h, w = torch.ones(T, D, device="cuda", dtype=dtype), torch.zeros(V, D, device="cuda", dtype=dtype)
+    w[:, 0] = torch.randint(-60, 61, (V,), generator=g, device="cuda").to(dtype)
+    cases.append((h, w))                                                     # all at the first step, then zeros
+    w = torch.zeros_like(w)
+    w[:, :40] = 2 * whole(V, 40)
+    cases.append((whole(T, D), w))                                           # padded columns
+    w = torch.zeros_like(w)
+    w[:, 3], w[:, D // 2 + 1], w[:, D - 1] = 240.0, -240.0, whole(V)         # parts that cancel
+    cases.append((h, w))
+    one = torch.zeros_like(h)
+    one[torch.arange(T), torch.randint(0, D, (T,), generator=g, device="cuda")] = 1.0
+    cases.append((one, 32 * whole(V, D)))                                    # a row that is one feature
+    for h, w in cases:
+        lse, losses = tt.linear_cross_entropy_with_lse(h, w, y)[::-1]
+        want_lse, want, tol = exactly(h, w, y)
+        assert bool(((lse.double() - want_lse).abs() <= tol).all()), float(((lse.double() - want_lse).abs() - tol).max())
+        assert bool(((losses.double() - want).abs() <= tol).all()), float(((losses.double() - want).abs() - tol).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [100, 600])
+def test_the_error_of_a_logit_does_not_grow_with_its_length(T):
+    """Sums of growing size: a part of 512 loses at most 4 U of its own sum with each of its 32 steps of 16, and adding the D / 512 parts rounds to nearest, so that a
+    logit is off by (128 + D / 512) U of its sum of magnitudes, whatever D.  A loss of one entry is the logit's difference to lse, both off by that."""
+    D = 16384
+    g = torch.Generator(device="cuda").manual_seed(2)
+    h, w = (torch.rand(T, D, generator=g, device="cuda") / 8).bfloat16(), (torch.rand(300, D, generator=g, device="cuda") / 8).bfloat16()
+    y = torch.randint(0, 300, (T,), generator=g, device="cuda")
+    losses, lse = tt.linear_cross_entropy_with_lse(h, w, y)
+    want_lse, want, tol = exactly(h, w, y)
+    tol = tol + (128 + D / 512) * U * (h.double() @ w.double().t()).amax(1)
+    assert bool(((lse.double() - want_lse).abs() <= tol).all())
+    assert bool(((losses.double() - want).abs() <= 2 * tol).all())

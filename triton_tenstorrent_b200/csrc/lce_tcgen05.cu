@@ -13,7 +13,7 @@
 // and whatever stands in the rows of the others (padding, infinities) is never read by a product.
 //
 // The products run on CTA pairs (tcgen05, cta_group::2, 256 x 256 tiles, fp32 accumulators in tensor memory): warp 0 loads both operands by
-// TMA into a six-stage ring, one thread of warp 1 issues the MMAs, warps 2-5 run the epilogue of tile i during the main loop of tile i + 1.
+// TMA into a six-stage ring, one thread of warp 1 issues the MMAs, the other warps run the epilogue of tile i during the main loop of tile i + 1.
 // Bound: the tensor pipe; with few tokens the stream of W from HBM.  Measured, single launches at 2048 x 32000 x 4096 bf16: logits 335 us (1600 TFLOP/s, pipe
 // active 90 %), dlogits 338, dW 336, dh 368; 8192 tokens, D = 4096, V = 128000, forward and backward back to back: 26.3 ms, 1310 TFLOP/s at the power cap.
 #include <string.h>
@@ -24,8 +24,15 @@
 
 namespace b200k {
 
-constexpr int LCE_THREADS = 192;
-constexpr int LCE_EPI_WARPS = 4;
+// Each step of 16 along K truncates the tensor cores' running sum towards zero, which takes 2^-25 of it on average: K = 4096 in one go leaves a logit of
+// growing sums 3.8e-6 of itself too small, K = 8192 7.7e-6 (measured).  So the logits are summed over LCE_SEGMENT steps of 64 in tensor memory and these
+// parts in fp32 registers, rounded to nearest: about 2^-22 of it (2.4e-7), whatever K is, and nothing where the products' sums are exact.  Eight epilogue
+// warps hold a tile's sums, 128 columns of a row each (4096 x 65536 x 2048 bf16: 1 % slower than one go on four; parts of 1024 instead: 0.5 %).  The
+// gradients' products, whose results are rounded to 16 bits, sum in one go on four.
+constexpr int LCE_SEGMENT = 8;
+__host__ __device__ constexpr bool lce_logits(int epi) { return epi <= 1; }                          // STATS, DLOGITS
+__host__ __device__ constexpr int lce_epi_warps(int epi) { return lce_logits(epi) ? 8 : 4; }
+__host__ __device__ constexpr int lce_threads(int epi) { return 64 + 32 * lce_epi_warps(epi); }
 constexpr int LCE_STAGES = 6;
 constexpr int LCE_BOX_BYTES = 64 * 128;                     // 64 rows of 128 bytes
 constexpr int LCE_A_BYTES = 2 * LCE_BOX_BYTES;              // a CTA's 128 x 64 share of A
@@ -34,7 +41,7 @@ constexpr int LCE_C_BUF_BYTES = 32 * 128;
 constexpr int LCE_A_OFF = 0;
 constexpr int LCE_B_OFF = LCE_STAGES * LCE_A_BYTES;
 constexpr int LCE_C_OFF = LCE_B_OFF + LCE_STAGES * LCE_B_BYTES;
-constexpr int LCE_BAR_OFF = LCE_C_OFF + LCE_EPI_WARPS * 2 * LCE_C_BUF_BYTES;
+constexpr int LCE_BAR_OFF = LCE_C_OFF + 8 * LCE_C_BUF_BYTES;     // two staging buffers for each of four epilogue warps, one for each of eight
 constexpr int LCE_SMEM = LCE_BAR_OFF + (2 * LCE_STAGES + 4) * 8 + 16 + 1024;
 static_assert(LCE_SMEM <= 232448, "shared memory budget exceeded");
 
@@ -53,7 +60,6 @@ struct LceGemmParams {
   int f16;
   uint32_t idesc, idesc_half;
   uint32_t* status;
-  float log2e;             // STATS, DLOGITS: lce_log2e(K)
   const int* target;       // per row that counts: its target (STATS, DLOGITS)
   const int64_t* token_target;   // STATS without a gather: per token
   int width;               // STATS on single CTAs: columns of a tile
@@ -71,12 +77,6 @@ struct LceGemmParams {
   void* out;               // DH, last piece without splits: dh
   const int* token;        // DH: token of a row
 };
-
-// log2 e, corrected for what the tensor cores lose: each step of 16 along K truncates the running sum towards zero, which takes 2^-25 of it on
-// average, and the running sum is on average the final one times the part of K done, so that a logit comes out K / 16 * 2^-26 of itself too small.
-// (Measured on 2048 x 128000 logits: 8.3e-7, 3.85e-6 and 7.67e-6 at K = 1024, 4096 and 8192; 9.5e-7, 3.8e-6 and 7.6e-6 by the formula.  Without the
-// correction the mean loss is 1.2e-6 off at K = 4096.)
-__host__ __device__ inline float lce_log2e(int K) { return static_cast<float>(1.4426950408889634 * (1.0 + (K + 15) / 16 * 0x1p-26)); }
 
 // Parts that the K axis of the dh product is cut in: with fewer tiles than CTA pairs, or a last wave that is nearly empty, the parts of a tile go to
 // different pairs, which leave fp32 sums that lce_dh_kernel adds.  Cost of s parts, in steps of 64 along K (0.28 us): waves of K / s steps, about 8
@@ -143,10 +143,11 @@ __device__ __forceinline__ LceWork lce_work(const LceSchedule& s, int w) {
 
 __device__ __forceinline__ uint32_t lce_pack2(float lo, float hi, int f16) { return f16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi); }
 
-// 64 columns of a warp's 32 rows, packed to 16 bits, through the warp's staging buffer to the tensor map.
+// 64 columns of a warp's 32 rows, packed to 16 bits, through the warp's BUFS staging buffers in turn to the tensor map.
+template <int BUFS>
 __device__ __forceinline__ void lce_store_chunk(const CUtensorMap* map, const float (&f)[64], int f16, int row0, int col0, int rows, int cols,
                                                 uint8_t* stage, int& buf, uint32_t lane) {
-  if (lane == 0) tma_store_wait_read<1>();   // the buffer's store of two chunks ago
+  if (lane == 0) tma_store_wait_read<BUFS - 1>();   // the buffer's store of BUFS chunks ago
   __syncwarp();
   uint8_t* dst = stage + buf * LCE_C_BUF_BYTES;
 #pragma unroll
@@ -161,13 +162,12 @@ __device__ __forceinline__ void lce_store_chunk(const CUtensorMap* map, const fl
     if (row0 < rows && col0 < cols) tma_store_2d(map, dst, col0, row0);
     tma_store_commit();
   }
-  buf ^= 1;
+  if (BUFS == 2) buf ^= 1;
 }
 
 // 64 columns of a row of logits into its running maximum (in units of log2) and sum of 2^(x - maximum); `in`: the target's place among them, `limit`:
 // the first column that does not count.
-__device__ __forceinline__ void lce_stats_chunk(float (&f)[64], int in, int col0, int limit, float log2e, float* target_logit, float& run_max,
-                                                float& run_sum) {
+__device__ __forceinline__ void lce_stats_chunk(float (&f)[64], int in, int col0, int limit, float* target_logit, float& run_max, float& run_sum) {
   if (in >= 0 && in < 64 && col0 + in < limit) {
     float t = 0.f;
 #pragma unroll
@@ -182,18 +182,30 @@ __device__ __forceinline__ void lce_stats_chunk(float (&f)[64], int in, int col0
 #pragma unroll
   for (int j = 1; j < 63; j += 2) m = fmax3(m, f[j], f[j + 1]);
   m = fmaxf(m, f[63]);
-  const float new_max = fmaxf(run_max, m * log2e);
+  const float new_max = fmaxf(run_max, m * LOG2E);
   const float shift = new_max == -INFINITY ? 0.f : new_max;     // a row of -inf: the sum stays 0
   float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
   for (int j = 0; j < 64; j += 4) {
-    s0 += ex2_approx(fmaf(f[j], log2e, -shift));
-    s1 += ex2_approx(fmaf(f[j + 1], log2e, -shift));
-    s2 += ex2_approx(fmaf(f[j + 2], log2e, -shift));
-    s3 += ex2_approx(fmaf(f[j + 3], log2e, -shift));
+    s0 += ex2_approx(fmaf(f[j], LOG2E, -shift));
+    s1 += ex2_approx(fmaf(f[j + 1], LOG2E, -shift));
+    s2 += ex2_approx(fmaf(f[j + 2], LOG2E, -shift));
+    s3 += ex2_approx(fmaf(f[j + 3], LOG2E, -shift));
   }
   run_sum = fmaf(run_sum, ex2_approx(run_max - shift), (s0 + s1) + (s2 + s3));
   run_max = new_max;
+}
+
+// Adds 128 columns of the part of a row's sums that lies in tensor memory (16 at a time: 32 more registers would be spilled next to the sums).
+__device__ __forceinline__ void lce_add_segment(uint32_t taddr, float (&f)[2][64]) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    uint32_t v[16];
+    tmem_ld_x16(taddr + c * 16, v);
+    tmem_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) f[c / 4][(c & 3) * 16 + j] += __uint_as_float(v[j]);
+  }
 }
 
 // A target as the kernels compare it with columns: outside the vocabulary, or ignored, it matches none.
@@ -202,9 +214,11 @@ __device__ __forceinline__ int lce_target(int64_t y, int V) { return y >= 0 && y
 
 // A_MN / B_MN: the operand's tile is contiguous along M / N in memory (else along K).
 template <int EPI, bool A_MN, bool B_MN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LCE_THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(lce_threads(EPI), 1)
 lce_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                 const __grid_constant__ CUtensorMap tmap_c, const LceGemmParams p) {
+  constexpr bool LOGITS = lce_logits(EPI);
+  constexpr int EPI_WARPS = lce_epi_warps(EPI), BUFS = 8 / EPI_WARPS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* smem_a = smem + LCE_A_OFF;
@@ -231,7 +245,7 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tmem_full_bar[a], 1);
-      mbar_init(&tmem_empty_bar[a], 2 * LCE_EPI_WARPS);
+      mbar_init(&tmem_empty_bar[a], 2 * EPI_WARPS);
     }
     *abort_smem = 0;
     fence_mbar_init();
@@ -299,153 +313,184 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       uint32_t phase = 0;
       int it = 0;
       bool ok = true;
-      for (int work = pair; ok && work < sched.num_work; work += num_pairs, ++it) {
+      for (int work = pair; ok && work < sched.num_work; work += num_pairs) {
         const uint32_t idesc = work >= sched.full_work ? p.idesc_half : p.idesc;
-        const int acc = it & 1;
-        ok = mbar_wait(&tmem_empty_bar[acc], ((it >> 1) & 1) ^ 1u, ctx, 62);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * 256;
         int kb0 = 0, kb1 = num_kb;
         if (EPI == LCE_DH) {
           const LceWork wk = lce_work(sched, work);
           kb0 = kb_begin(wk);
           kb1 = kb_end(wk);
         }
-        for (int kb = kb0; kb < kb1; ++kb) {
-          ok = mbar_wait(&full_bar[stage], phase, ctx, 63);
+        // a part of K (LOGITS: of LCE_SEGMENT steps) per accumulator
+        for (int first = kb0; ok && first < kb1; ++it) {
+          const int next = LOGITS ? min(first + LCE_SEGMENT, kb1) : kb1;
+          const int acc = it & 1;
+          ok = mbar_wait(&tmem_empty_bar[acc], ((it >> 1) & 1) ^ 1u, ctx, 62);
           if (!ok) break;
           tc_fence_after();
-          if (lane == 0) {
-            const uint32_t a_addr = smem_u32(smem_a + stage * LCE_A_BYTES);
-            const uint32_t b_addr = smem_u32(smem_b + stage * LCE_B_BYTES);
+          const uint32_t d_tmem = tmem_base + acc * 256;
+          for (int kb = first; kb < next; ++kb) {
+            ok = mbar_wait(&full_bar[stage], phase, ctx, 63);
+            if (!ok) break;
+            tc_fence_after();
+            if (lane == 0) {
+              const uint32_t a_addr = smem_u32(smem_a + stage * LCE_A_BYTES);
+              const uint32_t b_addr = smem_u32(smem_b + stage * LCE_B_BYTES);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              // K-major: a k step is 32 bytes along the 128-byte rows; M/N-major: 16 rows down, 64-wide chunks one box apart
-              const uint64_t a_desc = umma_smem_desc_sw128(a_addr + k * (A_MN ? 2048 : 32), A_MN ? LCE_BOX_BYTES : 16, 1024);
-              const uint64_t b_desc = umma_smem_desc_sw128(b_addr + k * (B_MN ? 2048 : 32), B_MN ? LCE_BOX_BYTES : 16, 1024);
-              umma_ss_2cta(d_tmem, a_desc, b_desc, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+              for (int k = 0; k < 4; ++k) {
+                // K-major: a k step is 32 bytes along the 128-byte rows; M/N-major: 16 rows down, 64-wide chunks one box apart
+                const uint64_t a_desc = umma_smem_desc_sw128(a_addr + k * (A_MN ? 2048 : 32), A_MN ? LCE_BOX_BYTES : 16, 1024);
+                const uint64_t b_desc = umma_smem_desc_sw128(b_addr + k * (B_MN ? 2048 : 32), B_MN ? LCE_BOX_BYTES : 16, 1024);
+                umma_ss_2cta(d_tmem, a_desc, b_desc, idesc, (kb > first || k > 0) ? 1u : 0u);
+              }
+              const uint32_t e = smem_u32(&empty_bar[stage]);
+              umma_commit_2cta(mapa_shared(e, 0));
+              umma_commit_2cta(mapa_shared(e, 1));
+              if (kb == next - 1) {
+                const uint32_t f = smem_u32(&tmem_full_bar[acc]);
+                umma_commit_2cta(mapa_shared(f, 0));
+                umma_commit_2cta(mapa_shared(f, 1));
+              }
             }
-            const uint32_t e = smem_u32(&empty_bar[stage]);
-            umma_commit_2cta(mapa_shared(e, 0));
-            umma_commit_2cta(mapa_shared(e, 1));
-            if (kb == kb1 - 1) {
-              const uint32_t f = smem_u32(&tmem_full_bar[acc]);
-              umma_commit_2cta(mapa_shared(f, 0));
-              umma_commit_2cta(mapa_shared(f, 1));
-            }
+            __syncwarp();
+            if (++stage == LCE_STAGES) { stage = 0; phase ^= 1u; }
           }
-          __syncwarp();
-          if (++stage == LCE_STAGES) { stage = 0; phase ^= 1u; }
+          first = next;
         }
       }
     }
   } else {
-    // ---------------------------------------------------------------- epilogue (warps 2..5, both CTAs)
+    // ---------------------------------------------------------------- epilogue (warps 2.., both CTAs)
     const int q = warp_idx & 3;
-    uint8_t* my_stage = smem_c + (warp_idx - 2) * 2 * LCE_C_BUF_BYTES;
+    uint8_t* my_stage = smem_c + (warp_idx - 2) * BUFS * LCE_C_BUF_BYTES;
     int it = 0, buf = 0;
     bool ok = true;
-    const float alpha = (EPI == LCE_DW || EPI == LCE_DH) ? *p.alpha : 1.f;
-    for (int work = pair; ok && work < sched.num_work; work += num_pairs, ++it) {
-      const LceWork wk = lce_work(sched, work);
-      const int row0 = wk.pid_m * 256 + static_cast<int>(rank) * 128 + q * 32;
-      const int row = row0 + static_cast<int>(lane);
-      const int chunks = wk.width / 64;
-      const int acc = it & 1;
-      const bool live = row < M;
-      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * 256;
-      // what the row needs, fetched while the main loop still runs
-      int target = -1, token = 0;
-      float lse2 = 0.f, scale = 0.f;
-      if (EPI == LCE_STATS || EPI == LCE_DLOGITS) {
-        if (live) target = (EPI == LCE_STATS && p.token_target != nullptr ? lce_target(p.token_target[row], p.N) : p.target[row]) - p.col_base - wk.col0;
-      }
-      if (EPI == LCE_DLOGITS && live) {
-        lse2 = p.lse2[row];
-        scale = p.row_scale[row];
-      }
-      if (EPI == LCE_DH && live) token = p.token[row];
-      float run_max = -INFINITY, run_sum = 0.f;     // STATS: maximum in units of log2, sum of 2^(x - maximum)
-      if (num_kb > 0) {
-        ok = mbar_wait(&tmem_full_bar[acc], (it >> 1) & 1, ctx, 64);
+    if constexpr (LOGITS) {
+      const int side = (warp_idx - 2) >> 2;          // the warp's 128 columns of a tile
+      for (int work = pair; ok && work < sched.num_work; work += num_pairs) {
+        const LceWork wk = lce_work(sched, work);
+        const int row0 = wk.pid_m * 256 + static_cast<int>(rank) * 128 + q * 32;
+        const int row = row0 + static_cast<int>(lane);
+        const int first_col = wk.col0 + side * 128;
+        const bool live = row < M, mine = side * 128 < wk.width;
+        // what the row needs, fetched while the main loop still runs
+        int target = -1;
+        float lse2 = 0.f, scale = 0.f;
+        if (live) target = (EPI == LCE_STATS && p.token_target != nullptr ? lce_target(p.token_target[row], p.N) : p.target[row]) - p.col_base - first_col;
+        if (EPI == LCE_DLOGITS && live) {
+          lse2 = p.lse2[row];
+          scale = p.row_scale[row];
+        }
+        float f[2][64];
+#pragma unroll
+        for (int j = 0; j < 64; ++j) f[0][j] = f[1][j] = 0.f;
+        for (int first = 0; first < num_kb; first += LCE_SEGMENT, ++it) {
+          const int acc = it & 1;
+          ok = mbar_wait(&tmem_full_bar[acc], (it >> 1) & 1, ctx, 64);
+          if (!ok) break;
+          tc_fence_after();
+          if (mine) lce_add_segment(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * 256 + side * 128, f);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&tmem_empty_bar[acc]), 0));
+        }
         if (!ok) break;
-        tc_fence_after();
+        if (!mine) continue;
+        float run_max = -INFINITY, run_sum = 0.f;     // STATS: maximum in units of log2, sum of 2^(x - maximum)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int col0 = first_col + c * 64;
+          const int in = target - c * 64;              // the target's place in this chunk
+          if constexpr (EPI == LCE_STATS) {
+            lce_stats_chunk(f[c], in, col0, p.N, p.target_logit + row, run_max, run_sum);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) {
+              const float e = ex2_approx(fmaf(f[c][j], LOG2E, -lse2)) - (j == in ? 1.f : 0.f);
+              f[c][j] = live ? e * scale : 0.f;        // rows behind the last one that counts: zeros, for the K tail of dW
+            }
+            if (col0 + 64 > p.N) {                     // columns behind the piece: zeros, for the K tail of dh
+#pragma unroll
+              for (int j = 0; j < 64; ++j) f[c][j] = col0 + j < p.N ? f[c][j] : 0.f;
+            }
+            lce_store_chunk<BUFS>(&tmap_c, f[c], p.f16, row0, col0, p.M, p.N, my_stage, buf, lane);   // the map ends on a multiple of 8 columns
+          }
+        }
+        if (EPI == LCE_STATS && live) p.part[static_cast<int64_t>(first_col >> 7) * p.part_ld + row] = make_float2(run_max, run_sum);
       }
-#pragma unroll 1
-      for (int c = 0; c < chunks; ++c) {
-        float f[64];
+    } else {
+      const float alpha = *p.alpha;
+      for (int work = pair; ok && work < sched.num_work; work += num_pairs, ++it) {
+        const LceWork wk = lce_work(sched, work);
+        const int row0 = wk.pid_m * 256 + static_cast<int>(rank) * 128 + q * 32;
+        const int row = row0 + static_cast<int>(lane);
+        const int chunks = wk.width / 64;
+        const int acc = it & 1;
+        const bool live = row < M;
+        const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * 256;
+        const int token = EPI == LCE_DH && live ? p.token[row] : 0;      // fetched while the main loop still runs
         if (num_kb > 0) {
-          uint32_t v0[32], v1[32];
-          tmem_ld_x32(t_row + c * 64, v0);
-          tmem_ld_x32(t_row + c * 64 + 32, v1);
-          tmem_wait_ld();
-          if (c == chunks - 1) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&tmem_empty_bar[acc]), 0));
-          }
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            f[j] = __uint_as_float(v0[j]);
-            f[32 + j] = __uint_as_float(v1[j]);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 64; ++j) f[j] = 0.f;
+          ok = mbar_wait(&tmem_full_bar[acc], (it >> 1) & 1, ctx, 64);
+          if (!ok) break;
+          tc_fence_after();
         }
-        const int col0 = wk.col0 + c * 64;
-        const int in = target - c * 64;              // the target's place in this chunk
-        if constexpr (EPI == LCE_STATS) {
-          lce_stats_chunk(f, in, col0, p.N, p.log2e, p.target_logit + row, run_max, run_sum);
-        } else if constexpr (EPI == LCE_DLOGITS) {
-#pragma unroll
-          for (int j = 0; j < 64; ++j) {
-            const float e = ex2_approx(fmaf(f[j], p.log2e, -lse2)) - (j == in ? 1.f : 0.f);
-            f[j] = live ? e * scale : 0.f;           // rows behind the last one that counts: zeros, for the K tail of dW
-          }
-          if (col0 + 64 > p.N) {                       // columns behind the piece: zeros, for the K tail of dh
-#pragma unroll
-            for (int j = 0; j < 64; ++j) f[j] = col0 + j < p.N ? f[j] : 0.f;
-          }
-          lce_store_chunk(&tmap_c, f, p.f16, row0, col0, p.M, p.N, my_stage, buf, lane);   // the map ends on a multiple of 8 columns
-        } else if constexpr (EPI == LCE_DW) {
-#pragma unroll
-          for (int j = 0; j < 64; ++j) f[j] *= alpha;
-          lce_store_chunk(&tmap_c, f, p.f16, row0, col0, p.M, p.N, my_stage, buf, lane);
-        } else {
-          // K (= D) is a multiple of 8, so a row of the result ends on a multiple of 8 columns
-          if (live) {
-            const int cols = min(64, p.N - col0);
-            const int64_t at = wk.split * p.split_stride + static_cast<int64_t>(row) * p.N + col0;
-            if (p.add != nullptr) {
-#pragma unroll
-              for (int j = 0; j < 64; j += 4)
-                if (j < cols) {
-                  const float4 a = *reinterpret_cast<const float4*>(p.add + at + j);
-                  f[j] += a.x; f[j + 1] += a.y; f[j + 2] += a.z; f[j + 3] += a.w;
-                }
+#pragma unroll 1
+        for (int c = 0; c < chunks; ++c) {
+          float f[64];
+          if (num_kb > 0) {
+            uint32_t v0[32], v1[32];
+            tmem_ld_x32(t_row + c * 64, v0);
+            tmem_ld_x32(t_row + c * 64 + 32, v1);
+            tmem_wait_ld();
+            if (c == chunks - 1) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&tmem_empty_bar[acc]), 0));
             }
-            if (splits > 1 || !p.last) {
 #pragma unroll
-              for (int j = 0; j < 64; j += 4)
-                if (j < cols) *reinterpret_cast<float4*>(p.sum + at + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
-            } else {
-              uint16_t* out = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(token) * p.N + col0;
+            for (int j = 0; j < 32; ++j) {
+              f[j] = __uint_as_float(v0[j]);
+              f[32 + j] = __uint_as_float(v1[j]);
+            }
+          } else {
 #pragma unroll
-              for (int j = 0; j < 64; j += 8)
-                if (j < cols)
-                  *reinterpret_cast<uint4*>(out + j) =
-                      make_uint4(lce_pack2(f[j] * alpha, f[j + 1] * alpha, p.f16), lce_pack2(f[j + 2] * alpha, f[j + 3] * alpha, p.f16),
-                                 lce_pack2(f[j + 4] * alpha, f[j + 5] * alpha, p.f16), lce_pack2(f[j + 6] * alpha, f[j + 7] * alpha, p.f16));
+            for (int j = 0; j < 64; ++j) f[j] = 0.f;
+          }
+          const int col0 = wk.col0 + c * 64;
+          if constexpr (EPI == LCE_DW) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) f[j] *= alpha;
+            lce_store_chunk<BUFS>(&tmap_c, f, p.f16, row0, col0, p.M, p.N, my_stage, buf, lane);
+          } else {
+            // K (= D) is a multiple of 8, so a row of the result ends on a multiple of 8 columns
+            if (live) {
+              const int cols = min(64, p.N - col0);
+              const int64_t at = wk.split * p.split_stride + static_cast<int64_t>(row) * p.N + col0;
+              if (p.add != nullptr) {
+#pragma unroll
+                for (int j = 0; j < 64; j += 4)
+                  if (j < cols) {
+                    const float4 a = *reinterpret_cast<const float4*>(p.add + at + j);
+                    f[j] += a.x; f[j + 1] += a.y; f[j + 2] += a.z; f[j + 3] += a.w;
+                  }
+              }
+              if (splits > 1 || !p.last) {
+#pragma unroll
+                for (int j = 0; j < 64; j += 4)
+                  if (j < cols) *reinterpret_cast<float4*>(p.sum + at + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+              } else {
+                uint16_t* out = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(token) * p.N + col0;
+#pragma unroll
+                for (int j = 0; j < 64; j += 8)
+                  if (j < cols)
+                    *reinterpret_cast<uint4*>(out + j) =
+                        make_uint4(lce_pack2(f[j] * alpha, f[j + 1] * alpha, p.f16), lce_pack2(f[j + 2] * alpha, f[j + 3] * alpha, p.f16),
+                                   lce_pack2(f[j + 4] * alpha, f[j + 5] * alpha, p.f16), lce_pack2(f[j + 6] * alpha, f[j + 7] * alpha, p.f16));
+              }
             }
           }
         }
       }
-      if (EPI == LCE_STATS && live) p.part[static_cast<int64_t>(wk.col0 >> 7) * p.part_ld + row] = make_float2(run_max, run_sum);
-      // a whole tile spans two 128-column slots of `part`
-      if (EPI == LCE_STATS && live && wk.width == 256)
-        p.part[static_cast<int64_t>((wk.col0 >> 7) + 1) * p.part_ld + row] = make_float2(-INFINITY, 0.f);
     }
     if (lane == 0) tma_store_wait_all<0>();
     __syncwarp();
@@ -480,7 +525,7 @@ static int lce_narrow_width(int V, int sms) {
   return static_cast<int>((width + 15) / 16 * 16);
 }
 
-__global__ void __launch_bounds__(LCE_THREADS, 1)
+__global__ void __launch_bounds__(lce_threads(LCE_STATS), 1)
 lce_stats_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const LceGemmParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -492,17 +537,22 @@ lce_stats_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
   uint64_t* tmem_empty_bar = tmem_full_bar + 2;
   uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(tmem_empty_bar + 2);
   uint32_t* abort_smem = tmem_ptr_smem + 1;
+  // What the warps of a tile's second 128 columns hand to those of the first, in three buffers in turn: the writers are two tiles ahead of a reader at
+  // most, since a tile's accumulator is that of the tile two before it, which the readers empty after they have joined the one before that.
+  __shared__ float2 second[3][128];
+  __shared__ uint64_t second_bar[3];
   const int warp_idx = threadIdx.x >> 5;
   const uint32_t lane = lane_id();
   WaitCtx ctx{abort_smem, p.status};
   if (threadIdx.x == 0) {
+    for (int i = 0; i < 3; ++i) mbar_init(&second_bar[i], lce_epi_warps(LCE_STATS) / 2);
     for (int s = 0; s < LCE1_STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tmem_full_bar[a], 1);
-      mbar_init(&tmem_empty_bar[a], LCE_EPI_WARPS);
+      mbar_init(&tmem_empty_bar[a], lce_epi_warps(LCE_STATS));
     }
     *abort_smem = 0;
     fence_mbar_init();
@@ -541,26 +591,29 @@ lce_stats_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
     int stage = 0, it = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++it) {
-      const int acc = it & 1;
-      ok = mbar_wait(&tmem_empty_bar[acc], ((it >> 1) & 1) ^ 1u, ctx, 66);
-      if (!ok) break;
-      tc_fence_after();
-      for (int kb = 0; kb < num_kb; ++kb) {
-        ok = mbar_wait(&full_bar[stage], phase, ctx, 67);
+    for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+      for (int first = 0; ok && first < num_kb; first += LCE_SEGMENT, ++it) {
+        const int next = min(first + LCE_SEGMENT, num_kb);
+        const int acc = it & 1;
+        ok = mbar_wait(&tmem_empty_bar[acc], ((it >> 1) & 1) ^ 1u, ctx, 66);
         if (!ok) break;
         tc_fence_after();
-        if (lane == 0) {
-          const uint32_t a_addr = smem_u32(smem_a + stage * LCE1_A_BYTES), b_addr = smem_u32(smem_b + stage * LCE1_B_BYTES);
+        for (int kb = first; kb < next; ++kb) {
+          ok = mbar_wait(&full_bar[stage], phase, ctx, 67);
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t a_addr = smem_u32(smem_a + stage * LCE1_A_BYTES), b_addr = smem_u32(smem_b + stage * LCE1_B_BYTES);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_ss(tmem_base + acc * 256, umma_smem_desc_sw128(a_addr + k * 32, 16, 1024), umma_smem_desc_sw128(b_addr + k * 32, 16, 1024), p.idesc,
-                    (kb > 0 || k > 0) ? 1u : 0u);
-          umma_commit(&empty_bar[stage]);
-          if (kb == num_kb - 1) umma_commit(&tmem_full_bar[acc]);
+            for (int k = 0; k < 4; ++k)
+              umma_ss(tmem_base + acc * 256, umma_smem_desc_sw128(a_addr + k * 32, 16, 1024), umma_smem_desc_sw128(b_addr + k * 32, 16, 1024), p.idesc,
+                      (kb > first || k > 0) ? 1u : 0u);
+            umma_commit(&empty_bar[stage]);
+            if (kb == next - 1) umma_commit(&tmem_full_bar[acc]);
+          }
+          __syncwarp();
+          if (++stage == LCE1_STAGES) { stage = 0; phase ^= 1u; }
         }
-        __syncwarp();
-        if (++stage == LCE1_STAGES) { stage = 0; phase ^= 1u; }
       }
     }
   } else {
@@ -568,38 +621,45 @@ lce_stats_narrow_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
     const int row = q * 32 + static_cast<int>(lane);
     const bool live = row < p.M;
     const int target = live ? lce_target(p.token_target[row], p.N) : LCE_NO_TARGET;
-    int it = 0;
+    const int side = (warp_idx - 2) >> 2;          // the warp's 128 columns of a tile
+    int it = 0, buf = 0;
+    uint32_t buf_phase = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++it) {
-      const int acc = it & 1;
-      const int first = tile * p.width, limit = min(p.N, first + p.width);
-      float run_max = -INFINITY, run_sum = 0.f;
-      ok = mbar_wait(&tmem_full_bar[acc], (it >> 1) & 1, ctx, 68);
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * 256;
-      const int chunks = (p.width + 63) >> 6;
-#pragma unroll 1
-      for (int c = 0; c < chunks; ++c) {
-        uint32_t v0[32], v1[32];
-        tmem_ld_x32(t_row + c * 64, v0);
-        tmem_ld_x32(t_row + c * 64 + 32, v1);
-        tmem_wait_ld();
-        if (c == chunks - 1) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&tmem_empty_bar[acc]);
-        }
-        float f[64];
+    for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+      const int first_col = tile * p.width + side * 128, limit = min(p.N, (tile + 1) * p.width);
+      float f[2][64];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          f[j] = __uint_as_float(v0[j]);
-          f[32 + j] = __uint_as_float(v1[j]);
-        }
-        const int col0 = first + c * 64;
-        lce_stats_chunk(f, target - col0, col0, limit, p.log2e, p.target_logit + row, run_max, run_sum);
+      for (int j = 0; j < 64; ++j) f[0][j] = f[1][j] = 0.f;
+      for (int first = 0; first < num_kb; first += LCE_SEGMENT, ++it) {
+        const int acc = it & 1;
+        ok = mbar_wait(&tmem_full_bar[acc], (it >> 1) & 1, ctx, 68);
+        if (!ok) break;
+        tc_fence_after();
+        lce_add_segment(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * 256 + side * 128, f);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tmem_empty_bar[acc]);
       }
-      if (live) p.part[static_cast<int64_t>(tile) * p.part_ld + row] = make_float2(run_max, run_sum);
+      if (!ok) break;
+      float run_max = -INFINITY, run_sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int col0 = first_col + c * 64;
+        if (col0 < limit) lce_stats_chunk(f[c], target - col0, col0, limit, p.target_logit + row, run_max, run_sum);
+      }
+      if (side == 1) {
+        second[buf][row] = make_float2(run_max, run_sum);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&second_bar[buf]);
+      } else {
+        ok = mbar_wait(&second_bar[buf], buf_phase, ctx, 69);
+        if (!ok) break;
+        const float2 o = second[buf][row];
+        const float top = fmaxf(run_max, o.x), shift = top == -INFINITY ? 0.f : top;
+        run_sum = fmaf(run_sum, ex2_approx(run_max - shift), o.y * ex2_approx(o.x - shift));
+        if (live) p.part[static_cast<int64_t>(tile) * p.part_ld + row] = make_float2(top, run_sum);
+      }
+      if (++buf == 3) { buf = 0; buf_phase ^= 1u; }
     }
   }
   drain_after_abort(abort_smem);
@@ -744,7 +804,7 @@ __global__ void __launch_bounds__(1024) lce_gmax_kernel(const float* __restrict_
 // Joins the tiles' (maximum, sum) of 32 rows: 32 slices of the slots, one row per lane.  Without a gather (token == null) row and token are the same.
 __global__ void __launch_bounds__(1024) lce_join_kernel(const float2* __restrict__ part, int64_t part_ld, int slots, const int* __restrict__ count, int T,
                                                         const float* __restrict__ target_logit, const int* __restrict__ token,
-                                                        const int64_t* __restrict__ target, int64_t ignore, int V, float log2e,
+                                                        const int64_t* __restrict__ target, int64_t ignore, int V,
                                                         float* __restrict__ losses, float* __restrict__ lse) {
   __shared__ float2 joined[32][33];
   grid_launch_dependents();
@@ -783,7 +843,7 @@ __global__ void __launch_bounds__(1024) lce_join_kernel(const float2* __restrict
     const int64_t y = target[t];
     const bool counts = y != ignore, valid = y >= 0 && y < V;
     lse[t] = counts ? lse2 * LN2 : 0.f;
-    losses[t] = !counts ? 0.f : valid ? fmaf(-target_logit[mine], log2e, lse2) * LN2 : __int_as_float(0x7FC00000);
+    losses[t] = !counts ? 0.f : valid ? fmaf(-target_logit[mine], LOG2E, lse2) * LN2 : __int_as_float(0x7FC00000);
   }
 }
 
@@ -945,9 +1005,9 @@ static int lce_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensor
   const int pairs = lce_pairs(p, dev);
   // the forward's with few tokens is the first of its chain
   if (p.count == nullptr) {
-    lce_gemm_kernel<EPI, A_MN, B_MN><<<2 * pairs, LCE_THREADS, LCE_SMEM, stream>>>(ta, tb, tc, p);
+    lce_gemm_kernel<EPI, A_MN, B_MN><<<2 * pairs, lce_threads(EPI), LCE_SMEM, stream>>>(ta, tb, tc, p);
   } else {
-    B200K_CHECK_CUDA(launch_dependent(lce_gemm_kernel<EPI, A_MN, B_MN>, dim3(2 * pairs), dim3(LCE_THREADS), LCE_SMEM, stream, ta, tb, tc, p));
+    B200K_CHECK_CUDA(launch_dependent(lce_gemm_kernel<EPI, A_MN, B_MN>, dim3(2 * pairs), dim3(lce_threads(EPI)), LCE_SMEM, stream, ta, tb, tc, p));
   }
   count_launch();
   B200K_CHECK_LAUNCH("lce_gemm_kernel");
@@ -984,7 +1044,6 @@ int lce_fwd(const LceArgs& a, cudaStream_t stream) {
   LceGemmParams p{};
   p.M = a.T; p.N = a.V; p.K = a.D;
   p.f16 = a.dtype == B200K_DTYPE_F16;
-  p.log2e = lce_log2e(a.D);
   p.part = reinterpret_cast<float2*>(ws + l.part);
   p.part_ld = a.T;
   p.target_logit = target_logit;
@@ -1026,7 +1085,7 @@ int lce_fwd(const LceArgs& a, cudaStream_t stream) {
     p.idesc = umma_idesc_16bit_f32(128, p.width, 0, 0, p.f16);
     p.status = dev->status_word;
     B200K_CHECK_CUDA(cudaFuncSetAttribute(lce_stats_narrow_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LCE1_SMEM));
-    lce_stats_narrow_kernel<<<slots < dev->sm_count ? slots : dev->sm_count, LCE_THREADS, LCE1_SMEM, stream>>>(th, tw, p);
+    lce_stats_narrow_kernel<<<slots < dev->sm_count ? slots : dev->sm_count, lce_threads(LCE_STATS), LCE1_SMEM, stream>>>(th, tw, p);
     count_launch();
     B200K_CHECK_LAUNCH("lce_stats_narrow_kernel");
   } else {
@@ -1035,7 +1094,7 @@ int lce_fwd(const LceArgs& a, cudaStream_t stream) {
     if ((rc = lce_gemm<LCE_STATS, false, false>(th, tw, th, p, dev, stream)) != 0) return rc;
   }
   B200K_CHECK_CUDA(launch_dependent(lce_join_kernel, dim3((a.T + 31) / 32), dim3(1024), 0, stream, p.part, p.part_ld, slots, p.count, a.T, target_logit,
-                                    p.token, a.target, a.ignore_index, a.V, p.log2e, a.losses, a.lse));
+                                    p.token, a.target, a.ignore_index, a.V, a.losses, a.lse));
   count_launch();
   B200K_CHECK_LAUNCH("lce_join_kernel");
   if (a.reduction != B200K_REDUCE_NONE) {
@@ -1114,7 +1173,6 @@ int lce_bwd(const LceArgs& a, cudaStream_t stream) {
     p.count = g.count;
     p.f16 = a.dtype == B200K_DTYPE_F16;
     p.alpha = g.alpha;
-    p.log2e = lce_log2e(a.D);
     p.M = a.T; p.N = n; p.K = a.D;
     p.target = g.row_target;
     p.col_base = v0;
