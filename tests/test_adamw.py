@@ -629,3 +629,58 @@ def test_betas_cannot_be_changed_under_the_step_count():
     opt.step([torch.ones(8, device="cuda")])
     m, v = opt.moments()
     assert bool((m[:8] == 0.5).all()) and bool((v[:8] == 0.25).all())
+
+
+def walk(params, grads, shapes=None, device=0, dtype=0, count=None):
+    """fill_rows over `params`; (its answer, the two columns that it fills)."""
+    dims = np.array([n for s in (shapes or [p.shape for p in params]) for n in (len(s), *s)], dtype=np.int64)
+    count = len(params) if count is None else count
+    table = np.zeros((max(1, len(params)), 9), dtype=np.int64)
+    return _lib.tensor_list().fill_rows(params, grads, count, dims.ctypes.data, table.ctypes.data, 9, device, dtype), table[:, :2]
+
+
+def test_the_walk_over_host_tensors_and_wrong_lists_leaves_all_to_the_general_case():
+    p = [torch.zeros(3), torch.zeros(2, 2)]
+    for params, grads, kw in [(p, p, {}), (p, None, {}), (tuple(p), p, {}), (p, tuple(p), {}), (p, p[:1], {}), (p, [None, p[1]], {}), (["x", p[1]], p, dict(shapes=[(3,), (2, 2)])),
+                              (p, p, dict(count=1)), (p, p, dict(count=3)), (p, p, dict(dtype=7)), ([], [], {})]:
+        assert walk(params, grads, **kw)[0] == -1
+    with pytest.raises(TypeError):
+        _lib.tensor_list().fill_rows(p, p)
+    with pytest.raises(TypeError):
+        walk(p, p, device="cuda")
+
+
+@pytest.mark.gpu
+def test_the_walk_takes_only_what_fits():
+    p = [torch.zeros(3, device="cuda"), torch.zeros(2, 2, device="cuda"), torch.zeros((), device="cuda")]
+    g = [torch.ones_like(t) for t in p]
+    at = p[0].get_device()
+    got, columns = walk(p, g, device=at)
+    assert got == 1 and columns.tolist() == [[x.data_ptr(), y.data_ptr()] for x, y in zip(p, g)]
+    for x, y in zip(p, g):
+        x.grad = y
+    assert walk(p, None, device=at)[0] == 1 and (walk(p, None, device=at)[1] == columns).all()
+    half = [t.bfloat16() for t in p]
+    assert walk(half, [t.bfloat16() for t in g], device=at, dtype=1)[0] == 0 and walk(half, g, device=at, dtype=1)[0] == 1
+    for i, wrong in [(0, g[0][:2]), (0, g[0].half()), (0, g[0].cpu()), (0, None), (1, g[1].view(4)), (1, torch.zeros(2, 4, device="cuda")[:, ::2]), (1, g[1].to_sparse()),
+                     (2, g[2].view(1)), (1, torch.zeros(2, 2, device="meta"))]:
+        assert walk(p, [wrong if k == i else t for k, t in enumerate(g)], device=at)[0] == -1, i
+        if wrong is not None:
+            assert walk([wrong if k == i else t for k, t in enumerate(p)], g, [t.shape for t in p], device=at)[0] == -1, i
+    assert walk(half, [g[0], g[1].bfloat16(), g[2]], device=at, dtype=1)[0] == -1          # mixed gradients
+    assert walk(p, g, device=at + 1)[0] == -1 and walk(p, g, device=at, dtype=1)[0] == -1
+    p[1].grad = None
+    assert walk(p, None, device=at)[0] == -1
+
+
+@pytest.mark.gpu
+def test_gradients_as_a_tuple_and_from_the_parameters_give_the_same_step():
+    params, grads = make([(40, 3), (7,), (1,)], torch.float32, torch.float32)
+    sets = [[torch.nn.Parameter(p.clone()) for p in params] for _ in range(3)]
+    for p, g in zip(sets[2], grads):
+        p.grad = g.clone()
+    for ps, g in zip(sets, (grads, tuple(grads), None)):
+        opt = tt.AdamW(ps)
+        opt.step(g)
+        opt.step(g)
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(*sets))

@@ -134,6 +134,21 @@ def load() -> ctypes.CDLL:
     return lib
 
 
+_tensor_list = None
+
+
+def tensor_list():
+    """The extension module that walks lists of tensors (csrc/tensor_list.cpp), loaded once.  Raises if it is not built."""
+    global _tensor_list
+    if _tensor_list is None:
+        try:
+            from . import _tensor_list as module
+        except ImportError as e:
+            raise ImportError(f"_tensor_list.so is missing or does not fit this torch: build it with `python -m triton_tenstorrent_b200.build` ({e})") from e
+        _tensor_list = module
+    return _tensor_list
+
+
 def last_error() -> str:
     msg = load().b200k_last_error()
     return msg.decode() if msg else ""

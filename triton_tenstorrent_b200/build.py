@@ -1,4 +1,4 @@
-"""Builds libb200kernels.so in-tree with nvcc for sm_100a.
+"""Builds libb200kernels.so in-tree with nvcc for sm_100a, and the extension module _tensor_list.so with g++ against torch's headers.
 
 Usage: ``python -m triton_tenstorrent_b200.build [--force] [--verbose]``.
 The library sits next to this file so that it travels with the source tree; nothing is
@@ -16,6 +16,7 @@ from pathlib import Path
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libb200kernels.so"
+TENSOR_LIST_PATH = PKG_DIR / "_tensor_list.so"
 BUILD_DIR = PKG_DIR / "build"
 
 SOURCES = ["capi.cu", "elementwise.cu", "matmul_tcgen05.cu", "attn_fwd_tcgen05.cu", "attn_bwd_tcgen05.cu", "layer_norm.cu", "lce_tcgen05.cu",
@@ -45,6 +46,19 @@ def _stale(target: Path, deps) -> bool:
     return any(Path(d).stat().st_mtime > t for d in deps)
 
 
+def _tensor_list_command(source: Path):
+    """The command that compiles and links the extension module; torch's libraries are those that the process has loaded already."""
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    include = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", sysconfig.get_paths()["include"], PKG_DIR.parent / "include",
+               Path(_nvcc()).resolve().parent.parent / "include"]
+    return ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-I{p}" for p in include),
+            f"-L{root / 'lib'}", "-Wl,--no-as-needed", "-lc10", "-ltorch_cpu", "-ltorch_python", str(source), "-o", str(TENSOR_LIST_PATH)]
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compiles every .cu under csrc/ and links the shared library.  Returns its path."""
     nvcc = _nvcc()
@@ -63,16 +77,18 @@ def build(force: bool = False, verbose: bool = False) -> Path:
                 cmd.insert(2, "-v")
             jobs.append(cmd)
 
+    tensor_list = _tensor_list_command(CSRC / "tensor_list.cpp") if force or _stale(TENSOR_LIST_PATH, [CSRC / "tensor_list.cpp", *headers]) else None
+
     def run(cmd):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if verbose or r.returncode != 0:
             sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
         if r.returncode != 0:
-            raise RuntimeError(f"nvcc failed on {cmd[-3]}")
+            raise RuntimeError(f"{Path(cmd[0]).name} failed on {cmd[-3]}")
 
-    if jobs:
-        with ThreadPoolExecutor(max_workers=min(4, len(jobs))) as ex:
-            list(ex.map(run, jobs))
+    if jobs or tensor_list:
+        with ThreadPoolExecutor(max_workers=min(4, len(jobs) + 1)) as ex:
+            list(ex.map(run, jobs + ([tensor_list] if tensor_list else [])))
     if jobs or force or _stale(LIB_PATH, objs):
         link = [nvcc, "-shared", "-o", str(LIB_PATH), *map(str, objs), "-gencode", "arch=compute_100a,code=sm_100a"]
         run(link)

@@ -3,7 +3,6 @@ include/b200k.h)."""
 from __future__ import annotations
 
 import math
-import operator
 import struct
 
 import numpy as np
@@ -16,11 +15,6 @@ __all__ = ["AdamW"]
 
 _BLOCK = 256                       # elements that share a scale of the 8-bit moments
 _P, _G, _MASTER, _M, _V, _MS, _VS, _N, _INDEX = range(9)     # columns of the table: fields of b200k_adamw_tensor
-
-
-# per-tensor queries of step(), called through map
-_size, _data_ptr, _is_contiguous, _get_device, _get_dtype = (torch.Tensor.size, torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.get_device,
-                                                             operator.attrgetter("dtype"))
 
 
 class AdamW:
@@ -100,7 +94,7 @@ class AdamW:
 
     def _lay_table(self):
         """The columns of the table that stay from step to step: addresses of this object's own moments, scales and master copies, and the sizes."""
-        table = np.zeros((len(self.params), 9), dtype=np.int64)
+        table = np.zeros((len(self._shapes), 9), dtype=np.int64)
         at = np.array(self.offsets, dtype=np.int64)
         width = self._m.element_size()
         table[:, _M], table[:, _V] = self._m.data_ptr() + at * width, self._v.data_ptr() + at * width
@@ -109,12 +103,14 @@ class AdamW:
         if self.master is not None:
             table[self._low, _MASTER] = self.master.data_ptr() + at[self._low] * 4
         table[:, _N] = [shape.numel() for shape in self._shapes]
-        table[:, _INDEX] = np.arange(len(self.params))
+        table[:, _INDEX] = np.arange(len(self._shapes))
         self._table = table
+        self._dims = np.array([n for shape in self._shapes for n in (len(shape), *shape)], dtype=np.int64)     # what step() compares the tensors with
+        self._addresses = self._dims.ctypes.data, table.ctypes.data
 
     # A copy (copy.deepcopy, pickle) has buffers of its own: the addresses are taken anew.
     def __getstate__(self):
-        return {k: v for k, v in self.__dict__.items() if k != "_table"}
+        return {k: v for k, v in self.__dict__.items() if k not in ("_table", "_dims", "_addresses")}
 
     def __setstate__(self, held):
         self.__dict__.update(held)
@@ -163,9 +159,10 @@ class AdamW:
         alone (with its moments) in this step; by default the parameters' .grad.  grad_scale multiplies every gradient: a number, or
         an fp32 CUDA tensor of one element (loss scaling, clipping by a norm)."""
         params = self.params
-        grads = [p.grad for p in params] if grads is None else grads
-        if len(grads) != len(params):
-            raise ValueError(f"AdamW: {len(params)} gradients expected, got {len(grads)}")
+        if grads is not None:
+            grads = grads if type(grads) is list else list(grads)
+            if len(grads) != len(params):
+                raise ValueError(f"AdamW: {len(params)} gradients expected, got {len(grads)}")
         self._check_hyper()
         scale, scale_ptr = 1.0, 0
         if isinstance(grad_scale, torch.Tensor):
@@ -179,23 +176,14 @@ class AdamW:
             if lr.device != self.device:
                 raise ValueError(f"AdamW: lr must be on {self.device}")
             lr, lr_ptr = 0.0, lr.data_ptr()
-        # The usual case first, with few steps per tensor: every gradient there, one type each, nothing to copy.
-        table, dtype, gdtype = self._table, self._dtype, getattr(grads[0], "dtype", None)
-        try:
-            usual = (dtype is not None and (gdtype is dtype or gdtype is torch.float32) and list(map(_size, grads)) == self._shapes
-                     and all(map(_is_contiguous, grads)) and all(map(_is_contiguous, params))
-                     and set(map(_get_device, grads)) == {self.device.index} and set(map(_get_dtype, grads)) == {gdtype}
-                     and list(map(_size, params)) == self._shapes and set(map(_get_device, params)) == {self.device.index}
-                     and set(map(_get_dtype, params)) == {dtype})
-            if usual:
-                table[:, _P] = list(map(_data_ptr, params))
-                table[:, _G] = list(map(_data_ptr, grads))
-        except (TypeError, RuntimeError):        # a gradient that is None, or has no contiguity
-            usual = False
-        if usual:
-            launches, touched = [(dtype, gdtype, table)], params
+        # The usual case first: every gradient there, one type each, nothing to copy
+        dtype, wide = self._dtype, -1
+        if dtype is not None:
+            wide = _lib.tensor_list().fill_rows(params, grads, len(self._shapes), *self._addresses, 9, self.device.index, _DTYPES[dtype])
+        if wide >= 0:
+            launches, touched = [(dtype, torch.float32 if wide else dtype, self._table)], params
         else:
-            launches, touched, grads = self._sort(grads)
+            launches, touched, grads = self._sort([p.grad for p in params] if grads is None else grads)
             if not touched:
                 return
         entry = _lib.load().b200k_adamw
