@@ -307,3 +307,26 @@ def test_nothing_outside_the_rows_is_written(cols, pad, dtype):
             check(name, buf[i, :n], ref[name])
             assert bool((buf[i, n:] == 777).all())
     assert bool((work[floats:] == 777).all()) and want_grads[0].shape == x.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_row_of_a_million_elements(dtype):
+    """The bound G for sums of any length.  Equal terms are the worst case: their roundings all go one way for as long as the sum stays in one binade."""
+    x, w, b, dy = make(3, (1 << 20) + 3, dtype, dtype)
+    run_and_check(x, w, b, dy)
+    x[1], dy[1] = 0.3, 0.7
+    x[2] = x[2].abs() + 1
+    run_and_check(x, w, b, dy)
+
+
+@pytest.mark.gpu
+def test_many_long_rows():
+    """Column sums over 5000 rows of 16400 elements, terms all of one sign: at most 32 additions in a row in fp32, 888 parts joined by 32 threads of 28 each, and a tree."""
+    x, w, b, dy = make(5000, 16400, torch.bfloat16, torch.float32)
+    dy.fill_(0.7)
+    x, w = x.abs(), None
+    _, mean, rstd = tt.layer_norm_with_stats(x, w, b)
+    _, _, db = tt.layer_norm_backward(dy, x, w, mean, rstd, need_dx=False, need_dw=False)
+    want = 5000 * float(dy[0, 0])
+    assert float((db.double() - want).abs().max()) <= (32 + 28 + 5 + 1) * U * want
