@@ -330,3 +330,48 @@ def test_many_long_rows():
     _, _, db = tt.layer_norm_backward(dy, x, w, mean, rstd, need_dx=False, need_dw=False)
     want = 5000 * float(dy[0, 0])
     assert float((db.double() - want).abs().max()) <= (32 + 28 + 5 + 1) * U * want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [40, 128, 515, 600, 1024, 2051, 4104, 5000, 8192, 8200, 9001, 12000, 16384, 16400])
+def test_non_finite_rows_leave_the_others_as_they_are(cols, dtype):
+    """At every row shape: rows that share a reduction, a warp or a stage of the ring, rows that are read twice, and rows off any alignment."""
+    x, w, b, dy = make(13, cols, dtype, dtype, seed=cols)
+    y, mean, rstd = tt.layer_norm_with_stats(x, w, b)
+    dx = tt.layer_norm_backward(dy, x, w, mean, rstd)[0]
+    bad_x, bad_dy = [2, 5, 12], 8
+    x2, dy2 = x.clone(), dy.clone()
+    x2[2, cols - 1], x2[5, 0], x2[12, cols // 2] = float("nan"), float("inf"), float("-inf")
+    dy2[bad_dy, cols // 3] = float("inf")
+    y2, mean2, rstd2 = tt.layer_norm_with_stats(x2, w, b)
+    dx2, dw2, db2 = tt.layer_norm_backward(dy2, x2, w, mean2, rstd2)
+    keep = torch.ones(13, dtype=torch.bool, device="cuda")
+    keep[bad_x] = False
+    assert torch.equal(y2[keep], y[keep]) and torch.equal(mean2[keep], mean[keep]) and torch.equal(rstd2[keep], rstd[keep])
+    assert bool(y2[bad_x].isnan().all()) and not bool(mean2[bad_x].isfinite().any())
+    keep[bad_dy] = False
+    assert torch.equal(dx2[keep], dx[keep]) and bool(dx2[bad_x].isnan().all()) and not bool(dx2[bad_dy].isfinite().any())
+    assert bool(dw2.isnan().all()) and bool(db2.isfinite().sum() == cols - 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols,dtype", [(700, 40, torch.bfloat16), (333, 600, torch.float16), (301, 8192, torch.bfloat16), (150, 16384, torch.float32), (7, 20000, torch.bfloat16),
+                                             (200, 2051, torch.bfloat16)])
+def test_captured_and_replayed_with_other_inputs(rows, cols, dtype):
+    x, w, b, dy = make(rows, cols, dtype, torch.float32)
+    call = lambda: (lambda s: s + tt.layer_norm_backward(dy, x, w, *s[1:]))(tt.layer_norm_with_stats(x, w, b))  # noqa: E731
+    call()
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(call())
+        graphs.append(graph)
+    for seed in (1, 2):
+        for t, new in zip((x, w, b, dy), make(rows, cols, dtype, torch.float32, seed)):
+            t.copy_(new)
+        for graph in graphs:
+            graph.replay()
+        want = call()
+        assert all(torch.equal(p, q) for out in outs for p, q in zip(want, out))
