@@ -34,6 +34,8 @@ namespace b200k {
 constexpr int ADAMW_BLOCK = 256;                      // elements that share a scale: one warp, 8 elements a lane
 constexpr int ADAMW_THREADS = 256;
 constexpr int ADAMW_CHUNK = 64 * ADAMW_BLOCK;         // elements of one CTA
+// Tensors of a launch: the table is a kernel parameter, which the host copies whole.  40 tensors take 13.1 us a step (host) with the small table and 16.7 with the
+// large one, the kernel 5.0 us with either; a small table of 120 costs 0.6 us with up to 40 tensors and saves 3 with more.
 constexpr int ADAMW_SMALL_TABLE = 40, ADAMW_LARGE_TABLE = 400;
 
 // What the kernels read of the step number; one per optimiser, in device memory.

@@ -144,14 +144,15 @@ __global__ void __launch_bounds__(256) ln_dw_loop_kernel(const T* __restrict__ d
 // their way into a ring in shared memory meanwhile.
 //
 // A row is worked on in steps that wait for one another (load, row sum, second sum, store), and registers for enough rows at a time do not exist
-// next to the backward's 2 N running sums; the ring keeps 60 KB (backward: 140) per SM on their way instead, whatever the arithmetic waits for.
+// next to the backward's 2 N running sums; the ring keeps up to 60 KB (backward: 140; two stages at least) per SM on their way instead, whatever the arithmetic
+// waits for.
 // Rows come as untiled bulk copies of the 16-byte blocks that they touch, so that any length and alignment arrives at full rate; only the
 // reads from shared memory and the stores go by VEC, the widest access that the operands' alignment allows.
 // A CTA-wide row is fetched by the CTA's first thread, behind a barrier that the row sum needs anyway; a warp of its own for it, as the CTAs of
 // narrow rows have, would cost the others registers (17 warps leave them 96 each, 16 warps 128: backward, 16384 x 4096 bf16, 82 against 64 us).
 //
-// Measured back to back (the backward with its join), inputs larger than L2, of 6460 GB/s: 16384 x 4096 bf16 forward 47 us (5.7 TB/s), backward 71 us
-// (5.7 TB/s); 65536 x 4096 169 and 246 us (6.4, 6.5 TB/s); 8192 x 8192 bf16 with fp32 weights 48 and 75 us.  Rows on odd boundaries (16384 x 4095
+// Measured back to back (the backward with its join), inputs larger than L2, of 6460 GB/s: 16384 x 4096 bf16 forward 47 us (5.7 TB/s), backward 70 us
+// (5.8 TB/s); 65536 x 4096 168 and 246 us (6.4, 6.5 TB/s); 8192 x 8192 bf16 with fp32 weights 48 and 75 us.  Rows on odd boundaries (16384 x 4095
 // bf16: 79 and 87 us) are bound by their 2-byte stores and the LSU.
 // ---------------------------------------------------------------------------------------------
 constexpr int LN_GROUPS = 8;          // rows at a time of a CTA whose warps take a row each
@@ -725,9 +726,12 @@ static LnSource ln_source(const void* p, int64_t rows, int64_t cols, int64_t ld,
 }
 // The ring of a CTA: a few KB per stage (a row or a batch of them for a CTA-wide row, some for every warp otherwise), and two stages or what makes
 // LN_AHEAD_FWD / LN_AHEAD_BWD bytes per SM, where the CTA's share of the shared memory holds them.  stages < 1: the rows are too long.
-// More reads under way than HBM's latency asks for hold up the writes (us, forward, 16384 x 4096 and 65536 x 4096 bf16: 47 and 169 with 72 KB per SM, 50 and 198
-// with 96 KB, 55 and 205 with 196 KB; 4096 x 16384: 63 with two stages, 78 with six).  The backward reads twice as much as it writes and is slowed by
-// fewer (131072 x 512 bf16: 97 with 60 KB, 84 with 110, 81 with 140, 89 with 200).
+// More reads under way than HBM's latency asks for hold up the writes.  bf16, us by the stages of a CTA and what they hold per SM (the first is what the
+// constants make):
+//   forward   16384 x 4096   2 (48 KB) 47, 3 (72) 47, 4 (96) 50, 8 (192) 55        65536 x 4096   168, 190, 198, 204
+//             32768 x 2048   3 (60 KB) 45, 4 (80) 48, 8 (160) 55                   4096 x 16384   2 (128 KB) 50, 3 (192) 60
+//   backward  131072 x 512   4 (128 KB) 81, 2 (64) 97, 3 (96) 84, 6 (192) 89       16384 x 4096   4 (128 KB) 70, 2 (64) 71, 3 (96) 70, 6 (192) 72
+// The backward reads twice as much as it writes and is slowed by fewer.
 constexpr int LN_SMEM = 212 * 1024;     // shared memory that the CTAs of an SM divide
 constexpr int LN_AHEAD_FWD = 60 * 1024, LN_AHEAD_BWD = 140 * 1024;
 static LnRing ln_ring(int64_t cols, int size, int align, int operands, int groups, int per_sm, int batch, int weight_size) {

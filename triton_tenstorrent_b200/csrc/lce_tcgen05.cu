@@ -6,7 +6,7 @@
 // Forward: one matrix product whose epilogue reduces each 256-column tile of the fp32 accumulators to a maximum and a sum of exponentials per
 // row; a second kernel joins the tiles' pairs.  Backward, for one piece of the vocabulary after the other: the logits of the piece again,
 // turned in the epilogue into dlogits in 16 bits; then dW of the piece (all tokens summed in one accumulator) and the piece's share of dh
-// (summed over the pieces in fp32).  8 T V D multiply-adds of which 2 are the recomputation.
+// (summed over the pieces in fp32).  8 T V D floating-point operations (forward 2, backward 6 of which 2 are the recomputation).
 //
 // Tokens whose target is `ignore_index` are left out before the first product: a gather kernel moves the rows that count to the front of a
 // copy of h and writes their number to device memory, where the products read it.  Work and time shrink with the tokens that carry a loss,
@@ -688,7 +688,6 @@ struct LceGatherParams {
   int* token;
   int* row_target;
   // forward
-  float* target_logit;
   float* losses;
   float* lse;
   // backward
@@ -951,7 +950,7 @@ static LceLayout lce_layout(int T, int D, int V, bool backward) {
     // as many parts as could fill the pairs eight times over
     const int64_t tiles = static_cast<int64_t>((T + 255) / 256) * ((D + 255) / 256);
     const int64_t splits = 8 * 74 / tiles;
-    // (several pieces carry one sum from piece to piece: their dlogits take up the 512 MiB, so that there are tiles enough)
+    // (several pieces carry one sum from piece to piece, and dW is never cut: with few tiles of dh or dW, as for a small D, some pairs then idle)
     l.max_splits = static_cast<int>(l.pieces > 1 || splits < 1 ? 1 : splits > LCE_MAX_SPLITS ? LCE_MAX_SPLITS : splits);
     if (l.pieces > 1 || l.max_splits > 1) l.sum = take(4ll * T * D * l.max_splits);
   }
