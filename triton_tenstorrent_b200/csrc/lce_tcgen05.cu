@@ -14,8 +14,8 @@
 //
 // The products run on CTA pairs (tcgen05, cta_group::2, 256 x 256 tiles, fp32 accumulators in tensor memory): warp 0 loads both operands by
 // TMA into a six-stage ring, one thread of warp 1 issues the MMAs, the other warps run the epilogue of tile i during the main loop of tile i + 1.
-// Bound: the tensor pipe; with few tokens the stream of W from HBM.  Measured, single launches at 2048 x 32000 x 4096 bf16: logits 335 us (1600 TFLOP/s, pipe
-// active 90 %), dlogits 338, dW 336, dh 368; 8192 tokens, D = 4096, V = 128000, forward and backward back to back: 26.3 ms, 1310 TFLOP/s at the power cap.
+// Bound: the tensor pipe; with few tokens the stream of W from HBM.  Measured, single launches at 2048 x 32000 x 4096 bf16: logits 340 us (1580 TFLOP/s, pipe
+// active 88 %), dlogits 347, dW 332, dh 364; 8192 tokens, D = 4096, V = 128000, forward and backward back to back: 26.3 ms, 1310 TFLOP/s at the power cap.
 #include <string.h>
 
 #include "attn_common.cuh"
