@@ -684,3 +684,13 @@ def test_gradients_as_a_tuple_and_from_the_parameters_give_the_same_step():
         opt.step(g)
         opt.step(g)
     assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(*sets))
+
+
+@pytest.mark.gpu
+def test_a_step_out_of_range_is_refused_before_anything_is_taken_over():
+    opt = tt.AdamW([torch.zeros(8, device="cuda")])
+    held = opt.state_dict()
+    for step in (-1, 1 << 63):
+        with pytest.raises(ValueError, match="step"):
+            opt.load_state_dict({**held, "step": step, "exp_avg": torch.ones_like(held["exp_avg"])})
+    assert opt.step_count() == 0 and not bool(opt.moments()[0].any())

@@ -23,7 +23,8 @@ class AdamW:
         m <- b1 m + (1 - b1) g,  v <- b2 v + (1 - b2) g^2
         p <- p - lr weight_decay p - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 
-    params          contiguous fp32, bf16 or fp16 CUDA tensors on one device that do not overlap (types may be mixed)
+    params          contiguous fp32, bf16 or fp16 CUDA tensors on one device that do not overlap (types may be mixed).  lr, eps and weight_decay hold for
+                    all of them: parameters that are to have others (norm weights without decay, say) get an optimiser of their own
     lr              a number, or an fp32 CUDA tensor of one element that a captured step reads at each replay; like eps and weight_decay
                     it may be changed between steps (opt.lr = ...)
     state_bits      32: fp32 moments, 8 bytes a parameter.  8: one byte each for m and sqrt(v), with an fp32 scale per 256 elements;
@@ -247,8 +248,8 @@ class AdamW:
         for name, t in want.items():
             if held[name].dtype != t.dtype or held[name].shape != t.shape:
                 raise ValueError(f"AdamW: {name} must be {t.dtype} {tuple(t.shape)}, got {held[name].dtype} {tuple(held[name].shape)}")
-        if int(held["step"]) < 0:
-            raise ValueError("AdamW: step must be >= 0")
+        if not 0 <= int(held["step"]) < 1 << 63:
+            raise ValueError(f"AdamW: step must be >= 0 and below 2^63, got {held['step']}")
         for name, t in want.items():
             t.copy_(held[name])
         if self.state_bits == 8:         # a power of two has the mantissa 1/2; blocks of zeros may have the scale zero by either rule
